@@ -124,6 +124,7 @@ struct DevBuf {
 
 struct gh_model;
 struct gh_q4;
+struct gh_kv8;
 
 struct gh_ctx {
     int device = 0;
@@ -137,6 +138,7 @@ struct gh_ctx {
     // called (released) is freed when the last of them is destroyed
     std::vector<gh_model*> models;
     std::vector<gh_q4*> q4s;
+    std::vector<gh_kv8*> kv8s;
     bool released = false;
     bool dying = false;  // chosen for freeing (by the one thread that saw it collectable)
 };

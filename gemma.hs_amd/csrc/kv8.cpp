@@ -1,0 +1,312 @@
+// Host side of the 8-bit KV cache: the handle, the checks of its calls and
+// the split of an attention call into workgroups.
+#include <cstring>
+#include <memory>
+
+#include "host.h"
+#include "kv8.h"
+
+using namespace gh;
+
+namespace {
+
+constexpr int MAX_SEQ = 1 << 22;   // tokens a sequence
+constexpr int MAX_ROWS = 1 << 20;  // query rows a kv head and sequence
+constexpr int MAX_GRID = 1 << 23;  // workgroups of 256 threads in a grid's x (2^32 threads at most)
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+Kv8Dev dev(const gh_kv8* kv) { return {kv->kc, kv->vc, kv->ks, kv->vs, kv->kt, kv->vt, kv->nkv, kv->nb}; }
+
+// The host arrays of a call: present, and every sequence known.
+int check_seqs(const char* fn, const gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* a, const int32_t* b) {
+    if (n < 0 || (n > 0 && (!seqs || !a || !b))) return set_error(GH_ERR_INVALID, "%s: bad arguments", fn);
+    for (int i = 0; i < n; ++i)
+        if (seqs[i] < 0 || seqs[i] >= kv->n_seq)
+            return set_error(GH_ERR_INVALID, "%s: sequence %d outside [0, %d)", fn, seqs[i], kv->n_seq);
+    return GH_OK;
+}
+
+// No sequence twice (calls that change them).
+int check_once(const char* fn, gh_kv8* kv, int32_t n, const int32_t* seqs) {
+    if (++kv->call == INT32_MAX) {
+        std::fill(kv->mark.begin(), kv->mark.end(), 0);
+        kv->call = 1;
+    }
+    for (int i = 0; i < n; ++i) {
+        if (kv->mark[seqs[i]] == kv->call) return set_error(GH_ERR_INVALID, "%s: sequence %d twice", fn, seqs[i]);
+        kv->mark[seqs[i]] = kv->call;
+    }
+    return GH_OK;
+}
+
+// Calls that change the cache's length, which the host keeps, cannot be
+// replayed from a graph.
+int check_not_capturing(const char* fn, gh_ctx* ctx) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    GH_HIP(hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone)
+        return set_error(GH_ERR_STATE, "%s changes the cache's length and cannot be captured", fn);
+    return GH_OK;
+}
+
+int blocks_of(int begin, int end) {  // blocks that [begin, end) touches
+    return end > begin ? (end - 1) / KV8_BLOCK - begin / KV8_BLOCK + 1 : 0;
+}
+
+}  // namespace
+
+gh_kv8::~gh_kv8() {
+    if (mem) hipFree(mem);
+}
+
+extern "C" int gh_kv8_create(gh_ctx* ctx, int32_t n_seq, int32_t max_seq, int32_t n_kv_heads, int32_t head_dim,
+                             gh_kv8** out) {
+    GH_CHECK(ctx_bind(ctx));
+    if (!out) return set_error(GH_ERR_INVALID, "gh_kv8_create: null output");
+    if (n_seq <= 0 || n_seq > (1 << 20) || max_seq <= 0 || max_seq > MAX_SEQ || n_kv_heads <= 0 || n_kv_heads > 1024)
+        return set_error(GH_ERR_INVALID, "gh_kv8_create: bad shape (%d sequences of %d tokens, %d kv heads)", n_seq,
+                         max_seq, n_kv_heads);
+    if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return set_error(GH_ERR_INVALID, "gh_kv8_create: head_dim %d is not 32, 64, 128 or 256", head_dim);
+    Lock lk(ctx->mu);
+    std::unique_ptr<gh_kv8> kv(new gh_kv8);
+    kv->ctx = ctx;
+    kv->n_seq = n_seq;
+    kv->max_seq = max_seq;
+    kv->nkv = n_kv_heads;
+    kv->hd = head_dim;
+    kv->nb = (max_seq + KV8_BLOCK - 1) / KV8_BLOCK;
+    const size_t heads = (size_t)n_seq * n_kv_heads, blocks = heads * kv->nb;
+    struct {
+        void** p;
+        size_t bytes;
+    } parts[] = {{(void**)&kv->kc, blocks * KV8_BLOCK * kv8_k_row(head_dim)},
+                 {(void**)&kv->vc, blocks * KV8_BLOCK * head_dim},
+                 {(void**)&kv->ks, blocks * 4},
+                 {(void**)&kv->vs, blocks * 4},
+                 {(void**)&kv->kt, heads * KV8_BLOCK * head_dim * 4},
+                 {(void**)&kv->vt, heads * KV8_BLOCK * head_dim * 4}};
+    size_t total = 0;
+    for (auto& p : parts) total += (p.bytes + 255) / 256 * 256;
+    hipError_t e = hipMalloc(&kv->mem, total);
+    if (e != hipSuccess) {
+        kv->mem = nullptr;
+        return set_error(GH_ERR_OOM, "gh_kv8_create: hipMalloc(%zu): %s", total, hipGetErrorString(e));
+    }
+    char* at = (char*)kv->mem;
+    for (auto& p : parts) {
+        *p.p = at;
+        at += (p.bytes + 255) / 256 * 256;
+    }
+    kv->len.assign(n_seq, 0);
+    kv->mark.assign(n_seq, 0);
+    ctx->kv8s.push_back(kv.get());
+    *out = kv.release();
+    handle_add(*out, HK_KV8);
+    return GH_OK;
+}
+
+extern "C" int gh_kv8_destroy(gh_kv8* kv) {
+    if (!kv) return GH_OK;
+    if (!handle_take(kv, HK_KV8)) return dead_handle("gh_kv8_destroy", HK_KV8);
+    gh_ctx* ctx = kv->ctx;
+    bool dead = false;
+    {
+        Lock lk(ctx->mu);
+        hipSetDevice(ctx->device);
+        hipStreamSynchronize(ctx->stream);
+        auto& v = ctx->kv8s;
+        v.erase(std::remove(v.begin(), v.end(), kv), v.end());
+        delete kv;
+        dead = ctx_dead(ctx);
+    }
+    if (dead) ctx_free(ctx);
+    return GH_OK;
+}
+
+extern "C" void gh_kv8_release(gh_kv8* kv) { gh_kv8_destroy(kv); }
+
+extern "C" int gh_kv8_length(gh_kv8* kv, int32_t seq, int32_t* len_out) {
+    GH_LIVE(kv, HK_KV8);
+    if (!len_out) return set_error(GH_ERR_INVALID, "gh_kv8_length: null output");
+    Lock lk(kv->ctx->mu);
+    if (seq < 0 || seq >= kv->n_seq)
+        return set_error(GH_ERR_INVALID, "gh_kv8_length: sequence %d outside [0, %d)", seq, kv->n_seq);
+    *len_out = kv->len[seq];
+    return GH_OK;
+}
+
+extern "C" int gh_kv8_append(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* n_tok, const float* k,
+                             const float* v) {
+    GH_LIVE(kv, HK_KV8);
+    gh_ctx* ctx = kv->ctx;
+    GH_CHECK(dev_bind(ctx));
+    Lock lk(ctx->mu);
+    GH_CHECK(check_seqs("gh_kv8_append", kv, n, seqs, n_tok, n_tok));
+    GH_CHECK(check_once("gh_kv8_append", kv, n, seqs));
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) {
+        if (n_tok[i] < 0) return set_error(GH_ERR_INVALID, "gh_kv8_append: %d tokens", n_tok[i]);
+        if (n_tok[i] > kv->max_seq - kv->len[seqs[i]])
+            return set_error(GH_ERR_RANGE, "gh_kv8_append: %d tokens behind %d of sequence %d pass max_seq %d", n_tok[i],
+                             kv->len[seqs[i]], seqs[i], kv->max_seq);
+        total += n_tok[i];
+    }
+    if (total == 0) return GH_OK;
+    if (!k || !v || !aligned(k) || !aligned(v))
+        return set_error(GH_ERR_INVALID, "gh_kv8_append: k and v must be 16-byte aligned device pointers");
+    GH_CHECK(check_not_capturing("gh_kv8_append", ctx));
+    const size_t row = (size_t)kv->nkv * kv->hd;
+    for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
+        const int m = std::min(n - i0, KV8_BATCH);
+        Kv8Batch b;
+        int blocks = 0;
+        b.off[0] = 0;
+        for (int i = 0; i < m; ++i) {
+            const int s = seqs[i0 + i], t = n_tok[i0 + i];
+            b.seq[i] = s;
+            b.pos[i] = kv->len[s];
+            b.off[i + 1] = b.off[i] + t;
+            blocks = std::max(blocks, blocks_of(kv->len[s], kv->len[s] + t));
+        }
+        if (blocks) GH_CHECK(launch_kv8_append(dev(kv), kv->hd, b, m, blocks, k, v, ctx->stream));
+        k += (size_t)b.off[m] * row;
+        v += (size_t)b.off[m] * row;
+    }
+    for (int i = 0; i < n; ++i) kv->len[seqs[i]] += n_tok[i];
+    return op_sync(ctx);
+}
+
+extern "C" int gh_kv8_truncate(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* lens) {
+    GH_LIVE(kv, HK_KV8);
+    gh_ctx* ctx = kv->ctx;
+    GH_CHECK(dev_bind(ctx));
+    Lock lk(ctx->mu);
+    GH_CHECK(check_seqs("gh_kv8_truncate", kv, n, seqs, lens, lens));
+    GH_CHECK(check_once("gh_kv8_truncate", kv, n, seqs));
+    for (int i = 0; i < n; ++i)
+        if (lens[i] < 0 || lens[i] > kv->len[seqs[i]])
+            return set_error(GH_ERR_RANGE, "gh_kv8_truncate: sequence %d holds %d tokens, not %d", seqs[i],
+                             kv->len[seqs[i]], lens[i]);
+    GH_CHECK(check_not_capturing("gh_kv8_truncate", ctx));
+    bool ran = false;
+    for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
+        // only sequences that end inside a block afterwards have anything to redo
+        Kv8Batch b;
+        int m = 0;
+        for (int i = i0; i < std::min(n, i0 + KV8_BATCH); ++i) {
+            if (lens[i] == kv->len[seqs[i]] || lens[i] % KV8_BLOCK == 0) continue;
+            b.seq[m] = seqs[i];
+            b.pos[m] = kv->len[seqs[i]];
+            b.off[m++] = lens[i];
+        }
+        if (m) GH_CHECK(launch_kv8_truncate(dev(kv), kv->hd, b, m, ctx->stream));
+        ran = ran || m;
+    }
+    for (int i = 0; i < n; ++i) kv->len[seqs[i]] = lens[i];
+    return ran ? op_sync(ctx) : GH_OK;
+}
+
+extern "C" int gh_kv8_read(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* begins, const int32_t* ends,
+                           float* k_out, float* v_out) {
+    GH_LIVE(kv, HK_KV8);
+    gh_ctx* ctx = kv->ctx;
+    GH_CHECK(dev_bind(ctx));
+    Lock lk(ctx->mu);
+    GH_CHECK(check_seqs("gh_kv8_read", kv, n, seqs, begins, ends));
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) {
+        if (begins[i] < 0 || ends[i] < begins[i] || ends[i] > kv->len[seqs[i]])
+            return set_error(GH_ERR_RANGE, "gh_kv8_read: tokens [%d, %d) of sequence %d, which holds %d", begins[i],
+                             ends[i], seqs[i], kv->len[seqs[i]]);
+        total += ends[i] - begins[i];
+    }
+    if (total == 0 || (!k_out && !v_out)) return GH_OK;
+    if (!aligned(k_out) || !aligned(v_out))
+        return set_error(GH_ERR_INVALID, "gh_kv8_read: k_out and v_out must be 16-byte aligned device pointers");
+    const size_t row = (size_t)kv->nkv * kv->hd;
+    for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
+        const int m = std::min(n - i0, KV8_BATCH);
+        Kv8Batch b;
+        int blocks = 0;
+        b.off[0] = 0;
+        for (int i = 0; i < m; ++i) {
+            const int at = begins[i0 + i], end = ends[i0 + i];
+            b.seq[i] = seqs[i0 + i];
+            b.pos[i] = at;
+            b.off[i + 1] = b.off[i] + end - at;
+            blocks = std::max(blocks, blocks_of(at, end));
+        }
+        if (blocks) GH_CHECK(launch_kv8_read(dev(kv), kv->hd, b, m, blocks, k_out, v_out, ctx->stream));
+        if (k_out) k_out += (size_t)b.off[m] * row;
+        if (v_out) v_out += (size_t)b.off[m] * row;
+    }
+    return op_sync(ctx);
+}
+
+extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* n_q, const float* q,
+                                int32_t n_heads, int32_t window, float* out) {
+    GH_LIVE(kv, HK_KV8);
+    gh_ctx* ctx = kv->ctx;
+    GH_CHECK(dev_bind(ctx));
+    Lock lk(ctx->mu);
+    GH_CHECK(check_seqs("gh_kv8_attention", kv, n, seqs, n_q, n_q));
+    if (n_heads <= 0 || n_heads % kv->nkv || window < 0)
+        return set_error(GH_ERR_INVALID, "gh_kv8_attention: %d heads over %d kv heads, window %d", n_heads, kv->nkv, window);
+    const int group = n_heads / kv->nkv;
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) {
+        if (n_q[i] < 0) return set_error(GH_ERR_INVALID, "gh_kv8_attention: %d query tokens", n_q[i]);
+        if ((int64_t)n_q[i] * group > MAX_ROWS)
+            return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query tokens of %d heads a kv head", n_q[i], group);
+        total += n_q[i];
+    }
+    if (total == 0) return GH_OK;
+    if (!q || !out || !aligned(q) || !aligned(out))
+        return set_error(GH_ERR_INVALID, "gh_kv8_attention: q and out must be 16-byte aligned device pointers");
+    const size_t row = (size_t)n_heads * kv->hd;
+    for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
+        const int m = std::min(n - i0, KV8_BATCH);
+        Kv8Batch b;
+        Att8 a{};
+        b.off[0] = 0;
+        int most = 0;       // blocks of the longest row tile
+        int64_t work = 0;   // blocks of all row tiles
+        for (int i = 0; i < m; ++i) {
+            const int len = kv->len[seqs[i0 + i]], t = n_q[i0 + i];
+            b.seq[i] = seqs[i0 + i];
+            b.pos[i] = len;
+            b.off[i + 1] = b.off[i] + t;
+            const int tiles = (t * group + ATT8_ROWS - 1) / ATT8_ROWS;
+            a.tiles = std::max(a.tiles, tiles);
+            // tokens a tile may see: up to the window and its own rows
+            const int span = window ? (int)std::min<int64_t>(len, (int64_t)window + ATT8_ROWS / group + 1) : len;
+            const int blocks = std::min((len + KV8_BLOCK - 1) / KV8_BLOCK, span / KV8_BLOCK + 2);
+            if (t) most = std::max(most, blocks);
+            work += (int64_t)tiles * kv->nkv * blocks;
+        }
+        if (!a.tiles) continue;
+        // chunks of whole rounds of a workgroup's 4 waves, about 512 workgroups
+        a.chunk = (int)std::max<int64_t>(4, (work / 512 + 3) / 4 * 4);
+        a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
+        if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
+            return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows of %d kv heads in one call",
+                             a.tiles * ATT8_ROWS, kv->nkv);
+        a.q = q;
+        a.out = out;
+        a.heads = n_heads;
+        a.group = group;
+        a.window = window;
+        a.rows = (size_t)b.off[m] * n_heads;
+        if (a.ns > 1) {
+            void* part = nullptr;
+            GH_CHECK(ctx_scratch(ctx, a.rows * a.ns * (kv->hd + 2) * sizeof(float), &part));
+            a.part = (float*)part;
+        }
+        GH_CHECK(launch_kv8_attention(dev(kv), kv->hd, b, m, a, ctx->stream));
+        q += (size_t)b.off[m] * row;
+        out += (size_t)b.off[m] * row;
+    }
+    return op_sync(ctx);
+}

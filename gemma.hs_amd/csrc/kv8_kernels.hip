@@ -1,0 +1,615 @@
+// gfx950 kernels of the 8-bit KV cache: quantising append, truncation,
+// read-back, and the attention that reads the codes on the int8 matrix cores.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "kv8.h"
+
+namespace gh {
+
+namespace {
+
+constexpr int NT = 256;  // threads per workgroup (4 wave64)
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+constexpr uint32_t INF_BITS = 0x7f800000u;
+
+// Max over the 256 threads (two barriers; `slot`: 4 words of LDS).
+__device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* slot) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return max(max(slot[0], slot[1]), max(slot[2], slot[3]));
+}
+
+// ------------------------------------------------------------------
+// quantisation of one block (64 tokens of one kv head), one workgroup
+// ------------------------------------------------------------------
+// Scale of values whose largest magnitude has these bits; NaN where one of
+// them is not finite (an int8 cannot hold it, and a wrong number would not
+// show).  2^-100 keeps the scale, and half of it, a normal number.
+__device__ __forceinline__ float scale_of(uint32_t a) {
+    return a >= INF_BITS ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(a) / 127.0f, 0x1p-100f);
+}
+
+// x / s rounded half to even, exactly.  c = rint(x * inv) is off by one at
+// most, and only near the middle between two codes; x - c s fits into 24
+// bits there (a multiple of the smaller ulp, no larger than s / 2 and a bit),
+// so one fma gives it without rounding and its comparison with s / 2 decides.
+__device__ __forceinline__ int code_of(float x, float s, float inv) {
+    const float c = rintf(x * inv), r = fmaf(-c, s, x), h = 0.5f * s;
+    int k = (int)c;
+    if (fabsf(r) > h || (fabsf(r) == h && (k & 1))) k += r > 0.0f ? 1 : -1;
+    return k;
+}
+
+// A thread's items of a block: 16 values that share 16 bytes of codes.  K:
+// 16 dims of one row; V: 16 rows of one dim (the layout in kv8.h).
+template <int HD, bool V>
+struct Item {
+    static constexpr int N = 64 * HD / 16;              // items of a block
+    static constexpr int PER = (N + NT - 1) / NT;       // per thread
+    int at;  // byte offset of the item's codes in the block
+    int row, col;  // K: row, first dim; V: first row (g), dim
+    __device__ __forceinline__ explicit Item(int e) {
+        if (V) {
+            const int d = e % HD, g = e / HD;
+            row = 4 * g;
+            col = d;
+            at = ((d / 16) * 64 + g * 16 + d % 16) * 16;
+        } else {
+            constexpr int KC = HD / 16, KD = HD < 64 ? 1 : HD / 64;
+            const int rr = e % 16, c = e / 16 % KC, t = e / (16 * KC);
+            row = 16 * t + rr;
+            col = 16 * c;
+            at = ((t * KD + c / 4) * 64 + (c % 4) * 16 + rr) * 16;
+        }
+    }
+    // row of value j
+    __device__ __forceinline__ int row_of(int j) const { return V ? row + 16 * (j / 4) + j % 4 : row; }
+};
+
+template <int HD, bool V>
+using Items = float[Item<HD, V>::PER][16];
+
+// Values of the item's rows in [lo, hi) from src (row 0 of the block, `ld` floats a row).
+template <int HD, bool V>
+__device__ __forceinline__ void load_item(const Item<HD, V>& it, const float* src, size_t ld, int lo, int hi, float (&x)[16]) {
+    if (V) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int r = it.row_of(j);
+            if (r >= lo && r < hi) x[j] = src[(size_t)r * ld + it.col];
+        }
+    } else if (it.row >= lo && it.row < hi) {
+        const f32x4* p = (const f32x4*)(src + (size_t)it.row * ld + it.col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 v = p[j];
+            x[4 * j] = v.x;
+            x[4 * j + 1] = v.y;
+            x[4 * j + 2] = v.z;
+            x[4 * j + 3] = v.w;
+        }
+    }
+}
+
+template <int HD, bool V>
+__device__ __forceinline__ void store_rows(const Item<HD, V>& it, float* dst, int lo, int hi, const float (&x)[16]) {
+    if (V) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int r = it.row_of(j);
+            if (r >= lo && r < hi) dst[r * HD + it.col] = x[j];
+        }
+    } else if (it.row >= lo && it.row < hi) {
+        f32x4* p = (f32x4*)(dst + it.row * HD + it.col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = f32x4{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
+    }
+}
+
+// Codes of the item's rows in [lo, hi); the rows in front of lo stay as they are.
+template <int HD, bool V>
+__device__ __forceinline__ void store_codes(const Item<HD, V>& it, int8_t* block, int lo, int hi, float s, const float (&x)[16]) {
+    const float inv = 1.0f / s;
+    const bool ok = s == s;
+    union {
+        int8_t b[16];
+        i32x4 w;
+    } u;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) u.b[j] = ok ? (int8_t)code_of(x[j], s, inv) : 0;
+    if (V && lo > 0) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int r = it.row_of(j);
+            if (r >= lo && r < hi) block[it.at + j] = u.b[j];
+        }
+    } else if (V || (it.row >= lo && it.row < hi)) {
+        *(i32x4*)(block + it.at) = u.w;
+    }
+}
+
+template <int HD, bool V>
+__device__ __forceinline__ void zero_items(Items<HD, V>& x) {
+#pragma unroll
+    for (int i = 0; i < Item<HD, V>::PER; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+}
+
+template <int HD, bool V>
+__device__ __forceinline__ uint32_t amax_items(const Items<HD, V>& x, uint32_t* slot) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < Item<HD, V>::PER; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) a = max(a, abs_bits(x[i][j]));
+    return block_max_u32(a, slot);
+}
+
+// f(item, its values) for each of the thread's items
+template <int HD, bool V, class F>
+__device__ __forceinline__ void each_item(Items<HD, V>& x, F&& f) {
+#pragma unroll
+    for (int i = 0; i < Item<HD, V>::PER; ++i) {
+        const int e = i * NT + threadIdx.x;
+        if (Item<HD, V>::N % NT == 0 || e < Item<HD, V>::N) f(Item<HD, V>(e), x[i]);
+    }
+}
+
+// Rows [r0, r1) of a block come from src (its row 0), the first r0 are there
+// already: codes and f32 rows.
+template <int HD, bool V>
+__device__ __forceinline__ void append_block(int8_t* block, float* scale, float* tail, const float* src, size_t ld, int r0,
+                                             int r1, bool keep_rows, uint32_t* slot) {
+    Items<HD, V> x;
+    zero_items<HD, V>(x);
+    const float old = r0 > 0 ? *scale : 0.0f;
+    each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { load_item<HD, V>(it, src, ld, r0, r1, v); });
+    float s = scale_of(amax_items<HD, V>(x, slot));  // its barriers: every thread has read the old scale
+    if (r0 > 0 && !(s == s && old == old)) s = __uint_as_float(0x7fc00000u);
+    else if (r0 > 0) s = fmaxf(s, old);
+    const int lo = r0 > 0 && !(s > old) ? r0 : 0;  // a larger scale: the rows before again, from their f32 values
+    if (lo < r0)
+        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { load_item<HD, V>(it, tail, HD, 0, r0, v); });
+    each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) {
+        store_codes<HD, V>(it, block, lo, r1, s, v);
+        if (keep_rows) store_rows<HD, V>(it, tail, r0, r1, v);
+    });
+    if (threadIdx.x == 0) *scale = s;
+}
+
+// One workgroup per block that the new tokens touch, kv head and K or V.
+// Reads 4 bytes an element and writes 1: bound by memory.
+template <int HD>
+__global__ __launch_bounds__(NT) void k_kv8_append(Kv8Dev c, Kv8Batch b, const float* k, const float* v) {
+    __shared__ uint32_t slot[4];
+    const int i = blockIdx.z, h = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    const int pos = b.pos[i], cnt = b.off[i + 1] - b.off[i], end = pos + cnt;
+    const int first = pos / KV8_BLOCK, blk = first + blockIdx.x;
+    if (cnt == 0 || blk * KV8_BLOCK >= end) return;
+    const int r0 = max(pos - blk * KV8_BLOCK, 0), r1 = min(end - blk * KV8_BLOCK, KV8_BLOCK);
+    const size_t ld = (size_t)c.nkv * HD, head = (size_t)b.seq[i] * c.nkv + h, at = head * c.nb + blk;
+    // row 0 of the block (in front of the input where the block holds tokens already)
+    const float* in = is_v ? v : k;
+    const float* src = in + ((ptrdiff_t)b.off[i] + (blk * KV8_BLOCK - pos)) * (ptrdiff_t)ld + h * HD;
+    float* tail = (is_v ? c.vt : c.kt) + head * KV8_BLOCK * HD;
+    // The f32 rows of the last block, if it is not full.  Where the first
+    // block needs the old ones, its workgroup puts the new ones there, after
+    // it has read them.
+    const bool shared_tail = pos % KV8_BLOCK != 0 && (end - 1) / KV8_BLOCK != first;
+    const bool keep = r1 < KV8_BLOCK && !(shared_tail && blk != first);
+    if (is_v)
+        append_block<HD, true>(c.vc + at * KV8_BLOCK * HD, c.vs + at, tail, src, ld, r0, r1, keep, slot);
+    else
+        append_block<HD, false>(c.kc + at * KV8_BLOCK * kv8_k_row(HD), c.ks + at, tail, src, ld, r0, r1, keep, slot);
+    const int left = end % KV8_BLOCK;
+    if (shared_tail && blk == first && left) {
+        __syncthreads();
+        const float* from = in + ((size_t)b.off[i] + cnt - left) * ld + h * HD;
+        for (int e = threadIdx.x; e < left * (HD / 4); e += NT)
+            ((f32x4*)tail)[e] = *(const f32x4*)(from + (size_t)(e / (HD / 4)) * ld + e % (HD / 4) * 4);
+    }
+}
+
+// f32 value of a code: one product, rounded once
+template <int HD, bool V>
+__device__ __forceinline__ void read_item(const Item<HD, V>& it, const int8_t* block, float s, float (&x)[16]) {
+    union {
+        int8_t b[16];
+        i32x4 w;
+    } u;
+    u.w = *(const i32x4*)(block + it.at);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = (float)u.b[j] * s;
+}
+
+// A block that keeps its first r1 rows.  same: it was the last one already,
+// its f32 rows are there and are quantised anew; else its values become them.
+template <int HD, bool V>
+__device__ __forceinline__ void truncate_block(int8_t* block, float* scale, float* tail, int r1, bool same, uint32_t* slot) {
+    Items<HD, V> x;
+    zero_items<HD, V>(x);
+    if (same) {
+        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { load_item<HD, V>(it, tail, HD, 0, r1, v); });
+        const float s = scale_of(amax_items<HD, V>(x, slot));
+        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { store_codes<HD, V>(it, block, 0, r1, s, v); });
+        if (threadIdx.x == 0) *scale = s;
+    } else {
+        const float s = *scale;
+        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) {
+            read_item<HD, V>(it, block, s, v);
+            store_rows<HD, V>(it, tail, 0, r1, v);
+        });
+    }
+}
+
+template <int HD>
+__global__ __launch_bounds__(NT) void k_kv8_truncate(Kv8Dev c, Kv8Batch b) {
+    __shared__ uint32_t slot[4];
+    const int i = blockIdx.z, h = blockIdx.y >> 1;
+    const int blk = b.off[i] / KV8_BLOCK, r1 = b.off[i] % KV8_BLOCK;
+    const bool same = blk == b.pos[i] / KV8_BLOCK;
+    const size_t head = (size_t)b.seq[i] * c.nkv + h, at = head * c.nb + blk;
+    if (blockIdx.y & 1)
+        truncate_block<HD, true>(c.vc + at * KV8_BLOCK * HD, c.vs + at, c.vt + head * KV8_BLOCK * HD, r1, same, slot);
+    else
+        truncate_block<HD, false>(c.kc + at * KV8_BLOCK * kv8_k_row(HD), c.ks + at, c.kt + head * KV8_BLOCK * HD, r1, same,
+                                  slot);
+}
+
+template <int HD>
+__global__ __launch_bounds__(NT) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k, float* v) {
+    const int i = blockIdx.z, h = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    float* out = is_v ? v : k;
+    const int pos = b.pos[i], cnt = b.off[i + 1] - b.off[i], end = pos + cnt;
+    const int blk = pos / KV8_BLOCK + blockIdx.x;
+    if (!out || cnt == 0 || blk * KV8_BLOCK >= end) return;
+    const int r0 = max(pos - blk * KV8_BLOCK, 0), r1 = min(end - blk * KV8_BLOCK, KV8_BLOCK);
+    const size_t ld = (size_t)c.nkv * HD, at = ((size_t)b.seq[i] * c.nkv + h) * c.nb + blk;
+    float* dst = out + ((ptrdiff_t)b.off[i] + (blk * KV8_BLOCK - pos)) * (ptrdiff_t)ld + h * HD;  // row 0 of the block
+    auto go = [&](auto vv) {
+        constexpr bool V = decltype(vv)::value;
+        const int8_t* block = V ? c.vc + at * KV8_BLOCK * HD : c.kc + at * KV8_BLOCK * kv8_k_row(HD);
+        const float s = V ? c.vs[at] : c.ks[at];
+        Items<HD, V> x;
+        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&val)[16]) {
+            read_item<HD, V>(it, block, s, val);
+            if (V) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int r = it.row_of(j);
+                    if (r >= r0 && r < r1) dst[(ptrdiff_t)r * (ptrdiff_t)ld + it.col] = val[j];
+                }
+            } else if (it.row >= r0 && it.row < r1) {
+                f32x4* p = (f32x4*)(dst + (ptrdiff_t)it.row * (ptrdiff_t)ld + it.col);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = f32x4{val[4 * j], val[4 * j + 1], val[4 * j + 2], val[4 * j + 3]};
+            }
+        });
+    };
+    if (is_v) go(std::true_type{});
+    else go(std::false_type{});
+}
+
+// ------------------------------------------------------------------
+// attention
+// ------------------------------------------------------------------
+// Products of the codes run on the int8 matrix cores, which sum them exactly.
+// The other operand, a row of q or of probabilities, is an integer of 23 bits
+// and sign, relative to the row's (or block's) largest magnitude, in three
+// signed digits to the base 256: with L = 127 (65536 + 256 + 1) the largest
+// such integer, x = a / L * (65536 d2 + 256 d1 + d0), off by at most a / 2 L
+// (2^-24 a: what rounding a to f32 costs).  Three products give the integer
+// dot product; no code is ever converted.
+constexpr float DIGIT_MAX = 8355711.0f;
+// digits of v, |v| <= DIGIT_MAX, as the three low bytes: adding 128 (65536 +
+// 256 + 1) makes every digit an unsigned byte, 128 too large
+__device__ __forceinline__ uint32_t digits_of(int v) { return ((uint32_t)(v + 0x808080)) ^ 0x808080u; }
+
+// digit `n` of four packed values as four bytes
+__device__ __forceinline__ int digit_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int n) {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, n == 0 ? 0x0c0c0400u : n == 1 ? 0x0c0c0501u : 0x0c0c0602u);
+    const uint32_t hi = __builtin_amdgcn_perm(d, c, n == 0 ? 0x04000c0cu : n == 1 ? 0x05010c0cu : 0x06020c0cu);
+    return (int)(lo | hi);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// One workgroup: 16 query rows of one kv head (ATT8_ROWS) x one chunk of key
+// blocks, the blocks dealt to its 4 waves; each wave keeps its own running
+// maximum, sum and output, joined through LDS at the end.
+//   S^T = K Q^T   operand A: codes of 16 tokens, B: digits of 16 query rows;
+//                 lane (g, r) gets tokens 16 t + 4 g + i of query row r
+//   O^T = V^T P^T operand A: codes of 16 dims, B: digits of the lane's own
+//                 16 probabilities (the layout of V has their order)
+template <int HD>
+__global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
+    constexpr int KR = HD < 64 ? 64 : HD, KD = KR / 64, VD = HD / 16;
+    __shared__ i32x4 qd[3][KD][64];
+    __shared__ float qmax[KR / 16][16];
+    __shared__ float st_m[4][16], st_l[4][16];
+    __shared__ __align__(16) float ob[2][16][HD + 4];
+    const int i = blockIdx.z, chunk = blockIdx.x % a.ns, h = blockIdx.x / a.ns % c.nkv;
+    const int row0 = blockIdx.x / a.ns / c.nkv * ATT8_ROWS;
+    const int n_q = b.off[i + 1] - b.off[i], rows = min(n_q * a.group - row0, ATT8_ROWS);
+    if (rows <= 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+    // positions of the tile's first and last row, and the blocks they see
+    const int p0 = b.pos[i] - n_q + row0 / a.group, p1 = b.pos[i] - n_q + (row0 + rows - 1) / a.group;
+    const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
+    const int blk0 = begin + chunk * a.chunk, blk1 = min(blk0 + a.chunk, end);
+    // row r of the tile: its index among the call's output rows, position
+    const int my = row0 + r, pos = r < rows ? b.pos[i] - n_q + my / a.group : -1;
+    const size_t slot = ((size_t)b.off[i] + my / a.group) * a.heads + h * a.group + my % a.group;
+    const int from = a.window ? pos - a.window + 1 : 0;
+    if (blk0 >= blk1) {  // nothing to see in this chunk
+        if (a.ns > 1) {
+            if (tid < rows) {
+                a.part[slot * a.ns + chunk] = -INFINITY;
+                a.part[(a.rows + slot) * a.ns + chunk] = 0.0f;
+            }
+        } else {
+            for (int e = tid; e < rows * HD; e += NT) {
+                const int rr = row0 + e / HD;
+                a.out[(((size_t)b.off[i] + rr / a.group) * a.heads + h * a.group + rr % a.group) * HD + e % HD] = 0.0f;
+            }
+        }
+        return;
+    }
+
+    // digits of the query rows: a thread takes 16 dims of one row
+    float qscale;
+    {
+        float x[16];
+        const int rr = tid & 15, cc = tid >> 4, qr = row0 + rr;
+        uint32_t am = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+        if (tid < KR && rr < rows && cc < HD / 16) {
+            const f32x4* p = (const f32x4*)(a.q + (((size_t)b.off[i] + qr / a.group) * a.heads + h * a.group + qr % a.group) * HD + 16 * cc);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 v = p[j];
+                x[4 * j] = v.x;
+                x[4 * j + 1] = v.y;
+                x[4 * j + 2] = v.z;
+                x[4 * j + 3] = v.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) am = max(am, abs_bits(x[j]));
+        }
+        if (tid < KR) qmax[cc][rr] = __uint_as_float(am);
+        __syncthreads();
+        uint32_t m = 0, mine = 0;
+#pragma unroll
+        for (int j = 0; j < KR / 16; ++j) {
+            m = max(m, __float_as_uint(qmax[j][rr]));
+            mine = max(mine, __float_as_uint(qmax[j][r]));
+        }
+        // rows that are nearly zero: their digits vanish
+        const float inv = DIGIT_MAX / fmaxf(__uint_as_float(m), 0x1p-100f);
+        if (tid < KR) {
+            uint32_t d[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) d[j] = digits_of((int)rintf(fminf(fmaxf(x[j] * inv, -DIGIT_MAX), DIGIT_MAX)));
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                i32x4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = digit_bytes(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3], n);
+                qd[n][cc >> 2][(cc & 3) * 16 + rr] = w;
+            }
+        }
+        // score = q . k / sqrt(HD) in units of ln 2; a row that is not finite gives NaN
+        qscale = mine >= INF_BITS ? __uint_as_float(0x7fc00000u)
+                                  : fmaxf(__uint_as_float(mine), 0x1p-100f) / DIGIT_MAX * (1.44269504088896340736f / __builtin_sqrtf((float)HD));
+        __syncthreads();
+    }
+
+    float m_run = -INFINITY, l_run = 0.0f;
+    f32x4 o[VD];
+#pragma unroll
+    for (int d = 0; d < VD; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const size_t head = ((size_t)b.seq[i] * c.nkv + h) * c.nb;
+    for (int blk = blk0 + wave; blk < blk1; blk += 4) {
+        const i32x4* kp = (const i32x4*)(c.kc + (head + blk) * KV8_BLOCK * KR) + lane;
+        const i32x4* vp = (const i32x4*)(c.vc + (head + blk) * KV8_BLOCK * HD) + lane;
+        const float f = qscale * c.ks[head + blk], vs = c.vs[head + blk];
+        i32x4 kk[4][KD], vv[VD];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < KD; ++d) kk[t][d] = kp[(t * KD + d) * 64];
+#pragma unroll
+        for (int d = 0; d < VD; ++d) vv[d] = vp[d * 64];
+        float s[16], mb = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            i32x4 acc[3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                acc[n] = i32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < KD; ++d) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[t][d], qd[n][d][lane], acc[n], 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // each sum is below 2^24; the middle one is added to the low one first
+                const float v = fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j])) * f;
+                const int p = blk * KV8_BLOCK + 16 * t + 4 * g + j;
+                const bool in = p <= pos && p >= from;
+                s[4 * t + j] = in ? v : -INFINITY;
+                mb = fmaxf(mb, s[4 * t + j]);
+            }
+        }
+        mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
+        mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+        // probabilities relative to the block's own maximum
+        float lb = 0.0f;
+        uint32_t pd[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int p = blk * KV8_BLOCK + 16 * (j / 4) + 4 * g + j % 4;
+            const float e = p <= pos && p >= from ? exp2_fast(s[j] - mb) : 0.0f;
+            lb += e;
+            pd[j] = digits_of((int)rintf(e * DIGIT_MAX));
+        }
+        const float m_new = fmaxf(m_run, mb);
+        const float alpha = m_run == m_new ? 1.0f : exp2_fast(m_run - m_new);
+        const float beta = mb == -INFINITY ? 0.0f : exp2_fast(mb - m_new);
+        m_run = m_new;
+        l_run = l_run * alpha + (mb == -INFINITY ? lb : lb * beta);  // lb is NaN where every score is
+        // a row that sees nothing of the block takes nothing from it, whatever its scale is
+        const float w = mb == -INFINITY ? 0.0f : beta * vs * (1.0f / DIGIT_MAX);
+        i32x4 pb[3];
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) pb[n][t] = digit_bytes(pd[4 * t], pd[4 * t + 1], pd[4 * t + 2], pd[4 * t + 3], n);
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
+            i32x4 acc[3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pb[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float v = fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j]));
+                o[d][j] = fmaf(v, w, o[d][j] * alpha);
+            }
+        }
+    }
+    // join the waves
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (g == 0) {
+        st_m[wave][r] = m_run;
+        st_l[wave][r] = l_run;
+    }
+    __syncthreads();
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, st_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) L += st_l[w][r] * (st_m[w][r] == -INFINITY ? 0.0f : exp2_fast(st_m[w][r] - M));
+    const float mine = m_run == -INFINITY ? 0.0f : exp2_fast(m_run - M);
+#pragma unroll
+    for (int d = 0; d < VD; ++d) o[d] *= mine;
+#pragma unroll
+    for (int half = 2; half > 0; half >>= 1) {
+        if (wave >= half && wave < 2 * half)
+#pragma unroll
+            for (int d = 0; d < VD; ++d) *(f32x4*)&ob[wave - half][r][16 * d + 4 * g] = o[d];
+        __syncthreads();
+        if (wave < half)
+#pragma unroll
+            for (int d = 0; d < VD; ++d) o[d] += *(const f32x4*)&ob[wave][r][16 * d + 4 * g];
+        __syncthreads();
+    }
+    if (wave != 0 || r >= rows) return;
+    if (a.ns > 1) {
+        const size_t at = slot * a.ns + chunk;
+        if (g == 0) {
+            a.part[at] = M;
+            a.part[a.rows * a.ns + at] = L;
+        }
+        f32x4* dst = (f32x4*)(a.part + 2 * a.rows * a.ns + at * HD);
+#pragma unroll
+        for (int d = 0; d < VD; ++d) dst[4 * d + g] = o[d];
+    } else {
+        const float inv = M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L;
+        f32x4* dst = (f32x4*)(a.out + slot * HD);
+#pragma unroll
+        for (int d = 0; d < VD; ++d) dst[4 * d + g] = o[d] * inv;
+    }
+}
+
+// Joins the chunk states of one output row.
+template <int HD>
+__global__ __launch_bounds__(NT) void k_kv8_combine(Att8 a) {
+    constexpr int LN = HD / 4, GR = NT / LN;  // float4 lanes, groups that share the chunks
+    __shared__ float red[8];
+    __shared__ __align__(16) f32x4 sum[GR][LN];
+    const size_t slot = blockIdx.x;
+    const float* pm = a.part + slot * a.ns;
+    const float* pl = a.part + (a.rows + slot) * a.ns;
+    const f32x4* po = (const f32x4*)(a.part + 2 * a.rows * a.ns + slot * a.ns * HD);
+    const int tid = threadIdx.x, ln = tid % LN, gr = tid / LN;
+    float m = -INFINITY;
+    for (int j = tid; j < a.ns; j += NT) m = fmaxf(m, pm[j]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float l = 0.0f;
+    for (int j = tid; j < a.ns; j += NT) l += pl[j] * (pm[j] == -INFINITY ? 0.0f : exp2_fast(pm[j] - M));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
+    if ((tid & 63) == 0) red[4 + (tid >> 6)] = l;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = gr; j < a.ns; j += GR)
+        if (pm[j] != -INFINITY) acc += po[(size_t)j * LN + ln] * exp2_fast(pm[j] - M);  // a chunk that saw nothing wrote no output
+    sum[gr][ln] = acc;
+    __syncthreads();
+    if (tid < LN) {
+        const float L = (red[4] + red[5]) + (red[6] + red[7]);
+#pragma unroll
+        for (int j = 1; j < GR; ++j) acc += sum[j][ln];
+        const float inv = M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L;
+        ((f32x4*)(a.out + slot * HD))[ln] = acc * inv;
+    }
+}
+
+template <class F>
+int with_hd(int hd, F&& f) {
+    switch (hd) {
+        case 32: f(std::integral_constant<int, 32>{}); break;
+        case 64: f(std::integral_constant<int, 64>{}); break;
+        case 128: f(std::integral_constant<int, 128>{}); break;
+        case 256: f(std::integral_constant<int, 256>{}); break;
+        default: return set_error(GH_ERR_INVALID, "unsupported head_dim %d", hd);
+    }
+    GH_HIP(hipGetLastError());
+    return GH_OK;
+}
+
+}  // namespace
+
+int launch_kv8_append(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, const float* k, const float* v,
+                      hipStream_t s) {
+    return with_hd(hd, [&](auto h) {
+        hipLaunchKernelGGL(k_kv8_append<h.value>, dim3(blocks, 2 * c.nkv, n), dim3(NT), 0, s, c, b, k, v);
+    });
+}
+
+int launch_kv8_truncate(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, hipStream_t s) {
+    return with_hd(hd, [&](auto h) {
+        hipLaunchKernelGGL(k_kv8_truncate<h.value>, dim3(1, 2 * c.nkv, n), dim3(NT), 0, s, c, b);
+    });
+}
+
+int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, float* k, float* v, hipStream_t s) {
+    return with_hd(hd, [&](auto h) {
+        hipLaunchKernelGGL(k_kv8_read<h.value>, dim3(blocks, 2 * c.nkv, n), dim3(NT), 0, s, c, b, k, v);
+    });
+}
+
+int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t s) {
+    return with_hd(hd, [&](auto h) {
+        hipLaunchKernelGGL(k_kv8_attention<h.value>, dim3(a.ns * c.nkv * a.tiles, 1, n), dim3(NT), 0, s, c, b, a);
+        if (a.ns > 1) hipLaunchKernelGGL(k_kv8_combine<h.value>, dim3(a.rows), dim3(NT), 0, s, a);
+    });
+}
+
+}  // namespace gh

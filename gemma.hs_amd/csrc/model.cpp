@@ -9,6 +9,7 @@
 #include <unordered_map>
 
 #include "common.h"
+#include "host.h"
 
 namespace gh {
 
@@ -64,10 +65,6 @@ PfCut pf_cut(const DMat& w, int Pp) {
 
 using namespace gh;
 
-namespace {
-
-using Lock = std::lock_guard<std::recursive_mutex>;
-
 // ---------------------------------------------------------------------
 // Handle lifetimes.  Every handle the ABI returns is registered until its
 // destroy call.  A destroy (or any other call) on a handle that is not
@@ -87,7 +84,8 @@ using Lock = std::lock_guard<std::recursive_mutex>;
 // A finaliser destroying one handle while another thread steps on the same
 // context therefore waits for the step and cannot deadlock with it.
 // ---------------------------------------------------------------------
-enum HandleKind { HK_CTX = 1, HK_MODEL, HK_KV, HK_Q4 };
+namespace {
+
 std::mutex& handles_mu() {
     static auto* m = new std::mutex();  // never destroyed, as the map below
     return *m;
@@ -96,6 +94,18 @@ std::unordered_map<const void*, int>& handles() {
     static auto* h = new std::unordered_map<const void*, int>();  // never destroyed: finalisers may run at exit
     return *h;
 }
+const char* kind_name(int kind) {
+    return kind == HK_CTX     ? "context"
+           : kind == HK_MODEL ? "model"
+           : kind == HK_KV    ? "KV cache"
+           : kind == HK_KV8   ? "8-bit KV cache"
+                              : "Q4_0 tensor";
+}
+
+}  // namespace
+
+namespace gh {
+
 void handle_add(const void* h, int kind) {
     std::lock_guard<std::mutex> g(handles_mu());
     handles()[h] = kind;
@@ -105,7 +115,6 @@ bool handle_live(const void* h, int kind) {
     auto it = handles().find(h);
     return it != handles().end() && it->second == kind;
 }
-// Unregisters an open handle of `kind`; false if it is not one.
 bool handle_take(const void* h, int kind) {
     std::lock_guard<std::mutex> g(handles_mu());
     auto it = handles().find(h);
@@ -113,19 +122,10 @@ bool handle_take(const void* h, int kind) {
     handles().erase(it);
     return true;
 }
-const char* kind_name(int kind) {
-    return kind == HK_CTX ? "context" : kind == HK_MODEL ? "model" : kind == HK_KV ? "KV cache" : "Q4_0 tensor";
-}
 int dead_handle(const char* fn, int kind) {
     return set_error(GH_ERR_STATE, "%s: not an open %s handle (destroyed already or never created)", fn, kind_name(kind));
 }
-#define GH_LIVE(h, kind)                                                  \
-    do {                                                                  \
-        if (!(h)) return set_error(GH_ERR_INVALID, "%s: null handle", __func__); \
-        if (!handle_live((h), (kind))) return dead_handle(__func__, (kind)); \
-    } while (0)
 
-// Entry points taking a context handle: it must be open.
 int ctx_bind(gh_ctx* ctx) {
     if (!ctx) return set_error(GH_ERR_INVALID, "null context");
     if (!handle_live(ctx, HK_CTX)) return dead_handle("context", HK_CTX);
@@ -133,12 +133,14 @@ int ctx_bind(gh_ctx* ctx) {
     return GH_OK;
 }
 
-// Entry points taking a model / cache / tensor handle (checked open by the
-// caller): its context is alive, released or not.
 int dev_bind(gh_ctx* ctx) {
     GH_HIP(hipSetDevice(ctx->device));
     return GH_OK;
 }
+
+}  // namespace gh
+
+namespace {
 
 template <class T>
 int dev_alloc(gh_model* m, T** out, size_t count) {
@@ -624,18 +626,14 @@ extern "C" int gh_ctx_create(int device, gh_ctx** out) {
 
 // Lifetime helpers.  ctx_dead and model_collect_locked run with the
 // context mutex held; ctx_free runs after it is released.
-namespace {
+namespace gh {
 
-// True when a released context has no open model or Q4_0 tensor left; the
-// caller that sees this (once: `dying` is set) frees it with ctx_free.
 bool ctx_dead(gh_ctx* ctx) {
-    if (ctx->dying || !ctx->released || !ctx->models.empty() || !ctx->q4s.empty()) return false;
+    if (ctx->dying || !ctx->released || !ctx->models.empty() || !ctx->q4s.empty() || !ctx->kv8s.empty()) return false;
     ctx->dying = true;
     return true;
 }
 
-// Frees a context that ctx_dead selected.  No other thread holds a handle
-// made from it, so nothing else can be waiting on its mutex.
 void ctx_free(gh_ctx* ctx) {
     hipSetDevice(ctx->device);
     hipStreamSynchronize(ctx->stream);
@@ -646,6 +644,10 @@ void ctx_free(gh_ctx* ctx) {
     hipStreamDestroy(ctx->stream);
     delete ctx;
 }
+
+}  // namespace gh
+
+namespace {
 
 // Frees a released model that has no open KV cache left (context mutex
 // held); returns whether its context is now to be freed.
@@ -865,17 +867,16 @@ extern "C" int gh_q4_0_free(gh_q4* t) {
     return GH_OK;
 }
 
-// Op-level calls are synchronous, except while the context stream is being
-// captured (gh_capture_begin): then they only enqueue.
-static int op_sync(gh_ctx* ctx) {
+namespace gh {
+
+int op_sync(gh_ctx* ctx) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     GH_HIP(hipStreamIsCapturing(ctx->stream, &st));
     if (st == hipStreamCaptureStatusNone) GH_HIP(hipStreamSynchronize(ctx->stream));
     return GH_OK;
 }
 
-// Per-context device scratch for op-level temporaries; grows outside capture.
-static int ctx_scratch(gh_ctx* ctx, size_t bytes, void** out) {
+int ctx_scratch(gh_ctx* ctx, size_t bytes, void** out) {
     if (bytes > ctx->scratch_bytes) {
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         GH_HIP(hipStreamIsCapturing(ctx->stream, &st));
@@ -891,6 +892,8 @@ static int ctx_scratch(gh_ctx* ctx, size_t bytes, void** out) {
     *out = ctx->scratch;
     return GH_OK;
 }
+
+}  // namespace gh
 
 extern "C" int gh_q4_0_dequant(gh_q4* t, float* out) {
     GH_LIVE(t, HK_Q4);
@@ -940,10 +943,6 @@ extern "C" int gh_linear_q4(gh_ctx* ctx, const uint32_t* raw_words, size_t n_wor
 // =====================================================================
 // op-level entry points (device pointers)
 // =====================================================================
-#define OP_ENTER(ctx)             \
-    GH_CHECK(ctx_bind(ctx));      \
-    Lock lk((ctx)->mu)
-
 extern "C" int gh_rmsnorm(gh_ctx* ctx, const float* x, const float* w, int n, float eps, int zc, float* y) {
     OP_ENTER(ctx);
     if (!x || !w || !y || n <= 0) return set_error(GH_ERR_INVALID, "gh_rmsnorm: bad arguments");

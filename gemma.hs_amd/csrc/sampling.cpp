@@ -1,0 +1,32 @@
+// Host side of the batched sampler: the checks of its rules.
+#include <cmath>
+
+#include "host.h"
+#include "sampling.h"
+
+using namespace gh;
+
+extern "C" int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, int32_t vocab, const gh_sampling* rules,
+                              int32_t* tokens_out) {
+    OP_ENTER(ctx);
+    if (n_rows < 0 || vocab <= 0 || vocab > SMP_MAX_VOCAB)
+        return set_error(GH_ERR_INVALID, "gh_sample_rows: %d rows of %d logits", n_rows, vocab);
+    if (n_rows == 0) return GH_OK;
+    if (!logits || !rules || !tokens_out) return set_error(GH_ERR_INVALID, "gh_sample_rows: null argument");
+    for (int i = 0; i < n_rows; ++i) {
+        const gh_sampling& r = rules[i];
+        if (!(r.temperature >= 0.0f) || std::isinf(r.temperature))
+            return set_error(GH_ERR_RANGE, "gh_sample_rows: row %d: temperature must be finite and >= 0", i);
+        if (r.top_k < 0) return set_error(GH_ERR_RANGE, "gh_sample_rows: row %d: top_k %d", i, r.top_k);
+        if (!(r.top_p >= 0.0f && r.top_p <= 1.0f) || !(r.min_p >= 0.0f && r.min_p <= 1.0f))
+            return set_error(GH_ERR_RANGE, "gh_sample_rows: row %d: top_p %g or min_p %g outside [0, 1]", i, r.top_p, r.min_p);
+        if (!(r.u >= 0.0f && r.u < 1.0f)) return set_error(GH_ERR_RANGE, "gh_sample_rows: row %d: u %g outside [0, 1)", i, r.u);
+    }
+    for (int i = 0; i < n_rows; i += SMP_BATCH) {
+        SmpRules b;
+        const int m = std::min(n_rows - i, SMP_BATCH);
+        std::copy(rules + i, rules + i + m, b.r);
+        GH_CHECK(launch_sample_rows(logits + (size_t)i * vocab, m, vocab, b, tokens_out + i, ctx->stream));
+    }
+    return op_sync(ctx);
+}

@@ -28,7 +28,8 @@ from ._lib import (DTYPE_F16, DTYPE_F32, DTYPE_Q4_0, FLAG_IEEE_SCALES, FLAG_POST
 GemmaConfig = GhConfig
 
 __all__ = [
-    "GemmaConfig", "GemmaHipError", "Context", "DeviceBuffer", "Q4Tensor", "GemmaModel", "KVCache",
+    "GemmaConfig", "GemmaHipError", "Context", "DeviceBuffer", "Q4Tensor", "GemmaModel", "KVCache", "KVCache8",
+    "KV8_BLOCK", "SAMPLING", "sampling", "sample_rows",
     "preset", "runLinearQ4", "runGemmaInferenceCached", "runGemmaInferenceCachedWithLayer0",
     "generate", "prefill", "bench_decode", "profile_steps", "profile_prefill", "sample_logits", "time_kernel", "KernelTiming", "STEP_KERNELS", "synth_f32", "synth_q4_0", "synth_tokens",
     "tensor_list", "synth_tensors", "synth_kv", "center_q4_0", "device_count", "DTYPE_F32", "DTYPE_F16", "DTYPE_Q4_0",
@@ -208,6 +209,43 @@ def _dev(ctx, a):
     return DeviceBuffer.from_numpy(ctx, np.ascontiguousarray(a, dtype=np.float32))
 
 
+class _OnDevice:
+    """Device addresses of a call's arguments: a DeviceBuffer's, an address as
+    it is, or an upload of a numpy array of the given shape (f32) that lives
+    until the block ends."""
+
+    def __init__(self, ctx: Context):
+        self.ctx, self.held = ctx, []
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        for b in self.held:
+            b.free()
+
+    def new(self, nbytes: int) -> DeviceBuffer:
+        b = DeviceBuffer(self.ctx, nbytes)
+        self.held.append(b)
+        return b
+
+    def __call__(self, a, shape=None):
+        if a is None or isinstance(a, C.c_void_p):
+            return a
+        if isinstance(a, int):
+            return C.c_void_p(a)
+        if isinstance(a, DeviceBuffer):
+            if shape is not None and a.nbytes < 4 * int(np.prod(shape, dtype=np.int64)):
+                raise ValueError(f"a buffer of {a.nbytes} bytes is too small for f32 {tuple(shape)}")
+            return a.ptr
+        a = np.ascontiguousarray(a, dtype=np.float32)
+        if shape is not None and a.size != int(np.prod(shape, dtype=np.int64)):
+            raise ValueError(f"an array of {a.size} values does not hold {tuple(shape)}")
+        b = self.new(a.nbytes)
+        b.upload(a)
+        return b.ptr
+
+
 def rmsnorm(ctx: Context, x, w, eps: float = 1e-6, zero_centered: bool = True) -> np.ndarray:
     xb, wb, yb = _dev(ctx, x), _dev(ctx, w), DeviceBuffer(ctx, 4 * len(x))
     check(lib().gh_rmsnorm(ctx.h, xb.ptr, wb.ptr, len(x), eps, int(zero_centered), yb.ptr))
@@ -265,6 +303,39 @@ def sample_logits(ctx: Context, logits, temperature: float, seed: int, counter: 
         return t.value
     finally:
         lb.free()
+
+
+# The rules of one row of sample_rows (gh_sampling), as a numpy record.
+SAMPLING = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32),
+                     ("min_p", np.float32), ("u", np.float32)])
+
+
+def sampling(n_rows: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=0.0) -> np.ndarray:
+    """Rules for n_rows rows of sample_rows; each argument is one value or one a row."""
+    r = np.zeros(n_rows, SAMPLING)
+    r["temperature"], r["top_k"], r["top_p"], r["min_p"], r["u"] = temperature, top_k, top_p, min_p, u
+    return r
+
+
+def sample_rows(ctx: Context, logits, vocab: int, rules: np.ndarray, out=None):
+    """One token a row by the row's own rules (a SAMPLING array, one record a
+    row) and random number (gh_sample_rows): temperature, top-k, top-p, min-p.
+    logits [len(rows), vocab] f32: a numpy array, a DeviceBuffer or a device
+    address.  out: a DeviceBuffer or device address of len(rules) int32 that
+    takes the tokens; without it they come back as a numpy array.  -1 for a
+    row with a NaN or with nothing above -inf."""
+    rules = np.ascontiguousarray(rules)
+    if rules.dtype != SAMPLING or rules.ndim != 1:
+        raise ValueError("rules must be a one-dimensional array of gemma_hip.SAMPLING")
+    n = len(rules)
+    with _OnDevice(ctx) as dev:
+        lp = dev(logits, (n, vocab))
+        if out is not None:
+            check(lib().gh_sample_rows(ctx.h, lp, n, int(vocab), _ptr(rules), dev(out)))
+            return out
+        tb = dev.new(4 * n)
+        check(lib().gh_sample_rows(ctx.h, lp, n, int(vocab), _ptr(rules), tb.ptr))
+        return tb.numpy(np.int32, n)
 
 
 def gelu_mul(ctx: Context, g, u) -> np.ndarray:
@@ -489,6 +560,97 @@ class KVCache:
     def close(self) -> None:
         if self.h:
             lib().gh_kv_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+KV8_BLOCK = 64  # tokens that share a scale (GH_KV8_BLOCK)
+
+
+class KVCache8:
+    """K and V of a batch of sequences in 8 bits, with a scale for each
+    KV8_BLOCK tokens of a kv head (gh_kv8), and the attention over them.
+
+    seqs, n_tok, ... are host sequences of ints, one entry a sequence of the
+    call.  k, v and q are numpy arrays, DeviceBuffers or device addresses of
+    f32 rows, sequence after sequence in the order of seqs; an `out` argument
+    is a DeviceBuffer or address, and without it the result is a numpy
+    array."""
+
+    def __init__(self, ctx: Context, n_seq: int, max_seq: int, n_kv_heads: int, head_dim: int):
+        self.h = None
+        h = C.c_void_p()
+        check(lib().gh_kv8_create(ctx.h, n_seq, max_seq, n_kv_heads, head_dim, C.byref(h)))
+        self.ctx, self.h = ctx, h
+        self.n_seq, self.max_seq, self.n_kv_heads, self.head_dim = n_seq, max_seq, n_kv_heads, head_dim
+
+    @staticmethod
+    def _ints(*arrays):
+        out = [np.ascontiguousarray(a, dtype=np.int32) for a in arrays]
+        if any(a.ndim != 1 or a.size != out[0].size for a in out):
+            raise ValueError("one entry for each sequence")
+        return out
+
+    def cacheLength(self, seq: int = 0) -> int:
+        n = C.c_int32()
+        check(lib().gh_kv8_length(self.h, int(seq), C.byref(n)))
+        return n.value
+
+    def append(self, seqs, n_tok, k, v) -> None:
+        """Append n_tok[i] tokens to sequence seqs[i]; k, v [sum n_tok, n_kv_heads, head_dim]."""
+        seqs, n_tok = self._ints(seqs, n_tok)
+        shape = (int(n_tok.sum(dtype=np.int64)), self.n_kv_heads, self.head_dim)
+        with _OnDevice(self.ctx) as dev:
+            check(lib().gh_kv8_append(self.h, seqs.size, _ptr(seqs), _ptr(n_tok), dev(k, shape), dev(v, shape)))
+
+    def truncate(self, seqs, lens) -> None:
+        """Rewind sequence seqs[i] to its first lens[i] tokens."""
+        seqs, lens = self._ints(seqs, lens)
+        check(lib().gh_kv8_truncate(self.h, seqs.size, _ptr(seqs), _ptr(lens)))
+
+    def read(self, seqs, begins, ends, k_out=None, v_out=None):
+        """The f32 values of tokens [begins[i], ends[i]) of sequence seqs[i]:
+        into k_out and v_out (either may be None), or, with neither, as a pair
+        of numpy arrays [sum, n_kv_heads, head_dim]."""
+        seqs, begins, ends = self._ints(seqs, begins, ends)
+        total = int((ends.astype(np.int64) - begins).sum())
+        shape = (max(total, 0), self.n_kv_heads, self.head_dim)
+        with _OnDevice(self.ctx) as dev:
+            if k_out is not None or v_out is not None:
+                check(lib().gh_kv8_read(self.h, seqs.size, _ptr(seqs), _ptr(begins), _ptr(ends), dev(k_out, shape),
+                                        dev(v_out, shape)))
+                return k_out, v_out
+            n = int(np.prod(shape, dtype=np.int64))
+            kb, vb = dev.new(4 * n), dev.new(4 * n)
+            check(lib().gh_kv8_read(self.h, seqs.size, _ptr(seqs), _ptr(begins), _ptr(ends), kb.ptr, vb.ptr))
+            return kb.numpy(count=n).reshape(shape), vb.numpy(count=n).reshape(shape)
+
+    def attention(self, seqs, n_q, q, n_heads: int, window: int = 0, out=None):
+        """Attention of the last n_q[i] tokens of sequence seqs[i] (their K
+        and V appended before) over it; q, result [sum n_q, n_heads, head_dim].
+        A query sees its own position and those before, with window > 0 only
+        the last `window` of them."""
+        seqs, n_q = self._ints(seqs, n_q)
+        shape = (int(n_q.sum(dtype=np.int64)), int(n_heads), self.head_dim)
+        with _OnDevice(self.ctx) as dev:
+            qp = dev(q, shape)
+            if out is not None:
+                check(lib().gh_kv8_attention(self.h, seqs.size, _ptr(seqs), _ptr(n_q), qp, int(n_heads), int(window),
+                                             dev(out, shape)))
+                return out
+            n = int(np.prod(shape, dtype=np.int64))
+            ob = dev.new(4 * n)
+            check(lib().gh_kv8_attention(self.h, seqs.size, _ptr(seqs), _ptr(n_q), qp, int(n_heads), int(window), ob.ptr))
+            return ob.numpy(count=n).reshape(shape)
+
+    def close(self) -> None:
+        if self.h:
+            lib().gh_kv8_destroy(self.h)
             self.h = None
 
     def __del__(self):

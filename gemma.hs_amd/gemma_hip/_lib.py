@@ -69,6 +69,7 @@ SIGNATURES = {
     "gh_model_release": (None, [_P]),
     "gh_kv_release": (None, [_P]),
     "gh_q4_0_release": (None, [_P]),
+    "gh_kv8_release": (None, [_P]),
     "gh_ctx_sync": (C.c_int, [_P]),
     "gh_buf_alloc": (C.c_int, [_P, C.c_size_t, C.POINTER(_P)]),
     "gh_buf_free": (C.c_int, [_P, _P]),
@@ -118,6 +119,14 @@ SIGNATURES = {
     "gh_sample_logits": (C.c_int, [_P, _P, C.c_int, C.c_float, C.c_uint64, C.c_uint64, _I32]),
     "gh_sample_logits_top_k": (C.c_int, [_P, _P, C.c_int, C.c_float, C.c_int32, C.c_uint64, C.c_uint64, _I32]),
     "gh_kv_set_top_k": (C.c_int, [_P, C.c_int32]),
+    "gh_sample_rows": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, _P]),
+    "gh_kv8_create": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "gh_kv8_destroy": (C.c_int, [_P]),
+    "gh_kv8_length": (C.c_int, [_P, C.c_int32, _I32]),
+    "gh_kv8_append": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P]),
+    "gh_kv8_truncate": (C.c_int, [_P, C.c_int32, _P, _P]),
+    "gh_kv8_read": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, _P]),
+    "gh_kv8_attention": (C.c_int, [_P, C.c_int32, _P, _P, _P, C.c_int32, C.c_int32, _P]),
     "gh_time_kernel": (C.c_int, [_P, _P, C.c_char_p, C.c_int32, C.POINTER(C.c_double), C.POINTER(C.c_double), _I32]),
     "gh_time_stream_read": (C.c_int, [_P, C.c_size_t, C.c_int32, C.POINTER(C.c_double)]),
     "gh_time_exchange": (C.c_int, [_P, C.c_int32, C.c_int32, C.POINTER(C.c_double)]),

@@ -11,7 +11,7 @@
  *    caches, gh_q4 tensors and gh_buf_alloc buffers).
  *  - One HIP stream per context; calls on one context are serialised by a
  *    mutex, so a Haskell RTS running with -N may call from any thread.
- *  - Handles (gh_ctx, gh_model, gh_kv, gh_q4) may be destroyed in any
+ *  - Handles (gh_ctx, gh_model, gh_kv, gh_q4, gh_kv8) may be destroyed in any
  *    order, as garbage-collector finalisers run them: destroying a context
  *    or model that still has open handles made from it only releases it,
  *    and the library frees it with the last of them.  A call on a handle
@@ -88,7 +88,8 @@ int gh_timer_stop(gh_ctx* ctx, float* ms_out);
 /* Graph timing of op-level calls (no reference counterpart; used by the
  * matvec and attention microbenchmarks): after gh_capture_begin the
  * launch-only op calls (gh_q4_0_matvec, gh_attention_decode, gh_rmsnorm,
- * gh_qk_norm, gh_gelu_mul, gh_q4_0_dequant) enqueue without
+ * gh_qk_norm, gh_gelu_mul, gh_q4_0_dequant, gh_sample_rows, gh_kv8_read,
+ * gh_kv8_attention) enqueue without
  * synchronising; gh_capture_replay ends the capture, replays the graph
  * n_replays times between two events and returns the ms per replay. */
 int gh_capture_begin(gh_ctx* ctx);
@@ -172,6 +173,88 @@ int gh_sample_logits(gh_ctx* ctx, const float* logits, int n, float temperature,
 int gh_sample_logits_top_k(gh_ctx* ctx, const float* logits, int n, float temperature, int32_t top_k,
                            uint64_t seed, uint64_t counter, int32_t* token_out);
 
+/* One row's sampling rules and its random number. */
+typedef struct gh_sampling {
+    float temperature; /* 0: the lowest index of the largest logit */
+    int32_t top_k;     /* 0: off; else the top_k first in rank order */
+    float top_p;       /* 1: off; else the shortest prefix of those with at least this share of their mass */
+    float min_p;       /* 0: off; else only weights of at least this share of the largest one */
+    float u;           /* uniform in [0, 1) */
+} gh_sampling;
+/* One token for each of n_rows rows of logits [n_rows][vocab] (device, f32),
+ * by rules of its own (rules[n_rows], host memory) and from a given random
+ * number, so that the caller's generator decides (no reference counterpart:
+ * the reference's sampler is an argmax, app/Main.hs:505-507).  With w =
+ * exp((logit - largest logit) / temperature), in rank order (value
+ * descending, then lower index): top_k keeps the first top_k; top_p the
+ * shortest prefix whose mass is at least top_p times the mass that top_k
+ * left; min_p the weights >= min_p (the largest is 1); the shortest of the
+ * three prefixes is what the draw is made from, and the token is its first
+ * whose running mass exceeds u times its whole mass.  Weights are summed as
+ * 64-bit integers: a token depends on the row and its rules alone.
+ * A logit of -inf is never drawn; +inf takes all the mass (shared by equal
+ * ones).  tokens_out[n_rows] is device memory; a row with a NaN, or with
+ * nothing above -inf, gets -1.  Launch-only.  GH_ERR_RANGE for a rule outside
+ * its range (temperature not finite or negative, top_k < 0, top_p or min_p
+ * outside [0, 1], u outside [0, 1)); GH_ERR_INVALID for vocab above 2^24. */
+int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, int32_t vocab, const gh_sampling* rules,
+                   int32_t* tokens_out);
+
+/* ================================================================
+ * 8-bit KV cache of a batch of sequences: a handle of its own beside gh_kv
+ * (no reference counterpart: Gemma.KVCache holds one sequence in f32,
+ * src/Gemma/KVCache.hs:45-82).  Each sequence holds tokens [0, length) of
+ * K and V rows [n_kv_heads][head_dim] as signed 8-bit codes, with one f32
+ * scale for each GH_KV8_BLOCK tokens of one kv head, K and V apart:
+ *   a = largest |x| of the block's tokens, scale = max(a / 127, 2^-100),
+ *   code = x / scale rounded half to even, x is read as code * scale.
+ * The f32 rows of a partly filled last block are kept beside it and its
+ * codes redone when a new token raises the scale, so that what a cache holds
+ * does not depend on how its tokens were cut into appends.  A block with a
+ * value that is not finite reads as NaN.
+ *
+ * The calls take n entries: seqs[i] (0 <= seqs[i] < n_seq), in any order;
+ * host arrays.  Rows of several sequences lie one sequence after the other,
+ * in the order of seqs.  Device pointers are 16-byte aligned
+ * (GH_ERR_INVALID).  Nothing changes where a call returns an error.
+ * ================================================================ */
+#define GH_KV8_BLOCK 64
+typedef struct gh_kv8 gh_kv8;
+/* head_dim 32, 64, 128 or 256; max_seq tokens a sequence (at most 2^22).
+ * Device memory: about 2 * n_kv_heads * head_dim bytes a token, and
+ * 2 * 64 * n_kv_heads * head_dim floats a sequence for the last blocks. */
+int gh_kv8_create(gh_ctx* ctx, int32_t n_seq, int32_t max_seq, int32_t n_kv_heads, int32_t head_dim, gh_kv8** out);
+int gh_kv8_destroy(gh_kv8* kv);
+void gh_kv8_release(gh_kv8* kv); /* gh_kv8_destroy for finalisers */
+int gh_kv8_length(gh_kv8* kv, int32_t seq, int32_t* len_out);
+/* Append n_tok[i] >= 0 tokens to sequence seqs[i], no sequence twice
+ * (GH_ERR_INVALID); k, v [sum n_tok][n_kv_heads][head_dim] f32.
+ * GH_ERR_RANGE where a sequence would pass max_seq. */
+int gh_kv8_append(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* n_tok, const float* k, const float* v);
+/* Rewind sequence seqs[i] (none twice) to its first lens[i] tokens.  Within
+ * the last block the removed tokens leave no trace: the rest is what it would
+ * be had they never come.  Further back a block that becomes the last one
+ * keeps its codes and scale, and counts as the values these stand for when
+ * tokens come behind it.  lens[i] 0 empties a sequence. */
+int gh_kv8_truncate(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* lens);
+/* The f32 values of tokens [begins[i], ends[i]) of sequence seqs[i]:
+ * k_out, v_out [sum (ends - begins)][n_kv_heads][head_dim], either may be
+ * NULL.  Launch-only. */
+int gh_kv8_read(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* begins, const int32_t* ends, float* k_out,
+                float* v_out);
+/* Attention of n_q[i] >= 0 query tokens over sequence seqs[i] as it stands,
+ * their own K and V appended before: query t stands at position
+ * P = length - n_q[i] + t and sees positions [0, P], with window > 0 only the
+ * last `window` of them; a query that sees none (P < 0) gives zeros.
+ * n_heads query heads (a multiple of n_kv_heads; head h reads kv head
+ * h / (n_heads / n_kv_heads)), scores scaled by 1 / sqrt(head_dim) as in
+ * gh_attention_decode.  q, out [sum n_q][n_heads][head_dim] f32, not
+ * overlapping.  A decode step of a batch has n_q 1, a draft a few, a prompt
+ * all its tokens.  Launch-only (a captured call keeps the lengths that the
+ * cache had then).  GH_ERR_RANGE where n_heads / n_kv_heads * n_q passes
+ * 2^20 for a sequence. */
+int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* n_q, const float* q, int32_t n_heads,
+                     int32_t window, float* out);
 
 /* ================================================================
  * Model: replaces GemmaConfig / loadGemmaModel / loadGemmaModelFromGGUF
