@@ -22,11 +22,13 @@ extern "C" int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, 
             return set_error(GH_ERR_RANGE, "gh_sample_rows: row %d: top_p %g or min_p %g outside [0, 1]", i, r.top_p, r.min_p);
         if (!(r.u >= 0.0f && r.u < 1.0f)) return set_error(GH_ERR_RANGE, "gh_sample_rows: row %d: u %g outside [0, 1)", i, r.u);
     }
+    void* scratch = nullptr;
+    if (smp_chunks(1, vocab)) GH_CHECK(ctx_scratch(ctx, sizeof(SmpRow) * std::min(n_rows, SMP_BATCH), &scratch));
     for (int i = 0; i < n_rows; i += SMP_BATCH) {
         SmpRules b;
         const int m = std::min(n_rows - i, SMP_BATCH);
         std::copy(rules + i, rules + i + m, b.r);
-        GH_CHECK(launch_sample_rows(logits + (size_t)i * vocab, m, vocab, b, tokens_out + i, ctx->stream));
+        GH_CHECK(launch_sample_rows(logits + (size_t)i * vocab, m, vocab, b, (SmpRow*)scratch, tokens_out + i, ctx->stream));
     }
     return op_sync(ctx);
 }

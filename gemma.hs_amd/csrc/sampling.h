@@ -20,6 +20,25 @@ inline int smp_bits(int n) {
     return std::min(52, 62 - b);
 }
 
-int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRules& rules, int32_t* tokens, hipStream_t s);
+// Steps between a row's largest and smallest logit, elements that the exact
+// search sorts, and workgroups a row at most.
+constexpr int SMP_BINS = 2048, SMP_LIST = 4096, SMP_CHUNKS = 64;
+
+// Device scratch of a row that several workgroups read.
+struct SmpRow {
+    unsigned long long mass[SMP_BINS], list[SMP_LIST], first[SMP_CHUNKS];
+    unsigned count[SMP_BINS];
+    float low[SMP_CHUNKS];
+    unsigned nan[SMP_CHUNKS], n_list, pad[15];
+};
+
+// Workgroups a row; 0: one, which runs every step (no scratch).
+inline int smp_chunks(int n_rows, int vocab) {
+    if (vocab <= 16384) return 0;
+    return std::max(1, std::min({SMP_CHUNKS, 512 / n_rows, (vocab + 4095) / 4096}));
+}
+
+int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRules& rules, SmpRow* scratch, int32_t* tokens,
+                       hipStream_t s);
 
 }  // namespace gh
