@@ -271,28 +271,32 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
         Kv8Batch b;
         Att8 a{};
         b.off[0] = 0;
+        int rows = 0;       // query rows of the longest entry
+        for (int i = 0; i < m; ++i) {
+            b.seq[i] = seqs[i0 + i];
+            b.pos[i] = kv->len[b.seq[i]];
+            b.off[i + 1] = b.off[i] + n_q[i0 + i];
+            rows = std::max(rows, n_q[i0 + i] * group);
+        }
+        if (rows == 0) continue;
+        a.tile = rows <= 4 ? 4 : 16;
+        a.tiles = (rows + a.tile - 1) / a.tile;
         int most = 0;       // blocks of the longest row tile
         int64_t work = 0;   // blocks of all row tiles
         for (int i = 0; i < m; ++i) {
-            const int len = kv->len[seqs[i0 + i]], t = n_q[i0 + i];
-            b.seq[i] = seqs[i0 + i];
-            b.pos[i] = len;
-            b.off[i + 1] = b.off[i] + t;
-            const int tiles = (t * group + ATT8_ROWS - 1) / ATT8_ROWS;
-            a.tiles = std::max(a.tiles, tiles);
+            const int len = b.pos[i], t = b.off[i + 1] - b.off[i];
             // tokens a tile may see: up to the window and its own rows
-            const int span = window ? (int)std::min<int64_t>(len, (int64_t)window + ATT8_ROWS / group + 1) : len;
+            const int span = window ? (int)std::min<int64_t>(len, (int64_t)window + a.tile / group + 1) : len;
             const int blocks = std::min((len + KV8_BLOCK - 1) / KV8_BLOCK, span / KV8_BLOCK + 2);
             if (t) most = std::max(most, blocks);
-            work += (int64_t)tiles * kv->nkv * blocks;
+            work += (int64_t)((t * group + a.tile - 1) / a.tile) * kv->nkv * blocks;
         }
-        if (!a.tiles) continue;
         // chunks of whole rounds of a workgroup's 4 waves, about 512 workgroups
         a.chunk = (int)std::max<int64_t>(4, (work / 512 + 3) / 4 * 4);
         a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
         if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
             return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows of %d kv heads in one call",
-                             a.tiles * ATT8_ROWS, kv->nkv);
+                             rows, kv->nkv);
         a.q = q;
         a.out = out;
         a.heads = n_heads;

@@ -55,8 +55,8 @@ int launch_kv8_append(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blo
 int launch_kv8_truncate(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, hipStream_t s);
 int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, float* k, float* v, hipStream_t s);
 
-// Query rows of a kv head: (token, head of its group), ATT8_ROWS a tile.
-constexpr int ATT8_ROWS = 16;
+// Query rows of a kv head are (token, head of its group) pairs, 4 or 16 of them
+// a tile.
 struct Att8 {
     const float* q;
     float* out;
@@ -64,6 +64,7 @@ struct Att8 {
     size_t rows;
     int heads, group;  // query heads, per kv head
     int window;
+    int tile;   // rows a tile
     int tiles;  // row tiles of the longest entry
     int ns;     // key chunks
     int chunk;  // blocks a chunk

@@ -315,259 +315,400 @@ __global__ __launch_bounds__(NT) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k,
 constexpr float DIGIT_MAX = 8355711.0f;
 // digits of v, |v| <= DIGIT_MAX, as the three low bytes: adding 128 (65536 +
 // 256 + 1) makes every digit an unsigned byte, 128 too large
-__device__ __forceinline__ uint32_t digits_of(int v) { return ((uint32_t)(v + 0x808080)) ^ 0x808080u; }
-
-// digit `n` of four packed values as four bytes
-__device__ __forceinline__ int digit_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int n) {
-    const uint32_t lo = __builtin_amdgcn_perm(b, a, n == 0 ? 0x0c0c0400u : n == 1 ? 0x0c0c0501u : 0x0c0c0602u);
-    const uint32_t hi = __builtin_amdgcn_perm(d, c, n == 0 ? 0x04000c0cu : n == 1 ? 0x05010c0cu : 0x06020c0cu);
-    return (int)(lo | hi);
-}
+__device__ __forceinline__ uint32_t digits_of(float v) { return ((uint32_t)((int)rintf(v) + 0x808080)) ^ 0x808080u; }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// One workgroup: 16 query rows of one kv head (ATT8_ROWS) x one chunk of key
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+constexpr int DPP_ROW_ROR4 = 0x124, DPP_ROW_ROR8 = 0x128;
+
+__device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+// The 16 columns of a product: 16 query rows, a product for each digit
+// (Wide), or 4 query rows with their three digits side by side, column 4 n + r
+// digit n of row r and the last four zero (Narrow).  Narrow is for decoding,
+// where a kv head has few query rows: a third of the products, and of the
+// conversions of their results.
+struct Wide {
+    static constexpr int ROWS = 16, DIG = 3;
+    int row;
+    __device__ __forceinline__ explicit Wide(int col) : row(col) {}
+    // digit n of four packed values as four bytes
+    __device__ __forceinline__ int bytes(const uint32_t* d, int n) const {
+        const uint32_t lo = __builtin_amdgcn_perm(d[1], d[0], n == 0 ? 0x0c0c0400u : n == 1 ? 0x0c0c0501u : 0x0c0c0602u);
+        const uint32_t hi = __builtin_amdgcn_perm(d[3], d[2], n == 0 ? 0x04000c0cu : n == 1 ? 0x05010c0cu : 0x06020c0cu);
+        return (int)(lo | hi);
+    }
+    // a product's values: each sum is below 2^24
+    __device__ __forceinline__ float value(const i32x4* acc, int j) const {
+        return fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j]));
+    }
+    __device__ __forceinline__ float partial(const i32x4* acc, int j) const { return value(acc, j); }
+    __device__ __forceinline__ float join(float v) const { return v; }
+};
+struct Narrow {
+    static constexpr int ROWS = 4, DIG = 1;
+    int row, digit;
+    uint32_t lo, hi;  // byte selectors of the lane's digit
+    float weight;
+    __device__ __forceinline__ explicit Narrow(int col) : row(col & 3), digit(col >> 2) {
+        lo = digit == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * digit;
+        hi = digit == 3 ? 0x0c0c0c0cu : 0x04000c0cu + 0x01010000u * digit;
+        weight = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
+    }
+    __device__ __forceinline__ int bytes(const uint32_t* d, int) const {
+        return (int)(__builtin_amdgcn_perm(d[1], d[0], lo) | __builtin_amdgcn_perm(d[3], d[2], hi));
+    }
+    // the lane's digit alone; join() adds the row's other two
+    __device__ __forceinline__ float partial(const i32x4* acc, int j) const { return (float)acc[0][j] * weight; }
+    __device__ __forceinline__ float join(float v) const {
+        v += dpp<DPP_ROW_ROR8>(v);
+        return v + dpp<DPP_ROW_ROR4>(v);
+    }
+    __device__ __forceinline__ float value(const i32x4* acc, int j) const { return join(partial(acc, j)); }
+};
+
+// One workgroup: the columns' query rows of one kv head x one chunk of key
 // blocks, the blocks dealt to its 4 waves; each wave keeps its own running
 // maximum, sum and output, joined through LDS at the end.
-//   S^T = K Q^T   operand A: codes of 16 tokens, B: digits of 16 query rows;
-//                 lane (g, r) gets tokens 16 t + 4 g + i of query row r
+//   S^T = K Q^T   operand A: codes of 16 tokens, B: digits of the query rows;
+//                 lane (g, col) gets tokens 16 t + 4 g + i of its row
 //   O^T = V^T P^T operand A: codes of 16 dims, B: digits of the lane's own
 //                 16 probabilities (the layout of V has their order)
-template <int HD>
+// The codes of the next block are on their way while the present one is
+// worked on: K's from its products on, V's from the end of the block on.
+template <int HD, class Cols>
 __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
-    constexpr int KR = HD < 64 ? 64 : HD, KD = KR / 64, VD = HD / 16;
-    __shared__ i32x4 qd[3][KD][64];
-    __shared__ float qmax[KR / 16][16];
-    __shared__ float st_m[4][16], st_l[4][16];
-    __shared__ __align__(16) float ob[2][16][HD + 4];
+    constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Cols::ROWS, DIG = Cols::DIG;
+    constexpr bool LATE_K = HD == 256, LATE_V = HD == 256 && ROWS == 16;
+    __shared__ float st_m[4][ROWS], st_l[4][ROWS];
+    __shared__ __align__(16) float ob[ROWS == 4 ? 4 : 2][ROWS][HD + 4];
     const int i = blockIdx.z, chunk = blockIdx.x % a.ns, h = blockIdx.x / a.ns % c.nkv;
-    const int row0 = blockIdx.x / a.ns / c.nkv * ATT8_ROWS;
-    const int n_q = b.off[i + 1] - b.off[i], rows = min(n_q * a.group - row0, ATT8_ROWS);
+    const int row0 = blockIdx.x / a.ns / c.nkv * ROWS;
+    const int n_q = b.off[i + 1] - b.off[i], rows = min(n_q * a.group - row0, ROWS), len = b.pos[i];
     if (rows <= 0) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, r = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    const Cols col(lane & 15);
     // positions of the tile's first and last row, and the blocks they see
-    const int p0 = b.pos[i] - n_q + row0 / a.group, p1 = b.pos[i] - n_q + (row0 + rows - 1) / a.group;
+    const int p0 = len - n_q + row0 / a.group, p1 = len - n_q + (row0 + rows - 1) / a.group;
     const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
     const int blk0 = begin + chunk * a.chunk, blk1 = min(blk0 + a.chunk, end);
-    // row r of the tile: its index among the call's output rows, position
-    const int my = row0 + r, pos = r < rows ? b.pos[i] - n_q + my / a.group : -1;
-    const size_t slot = ((size_t)b.off[i] + my / a.group) * a.heads + h * a.group + my % a.group;
-    const int from = a.window ? pos - a.window + 1 : 0;
+    // output row of the tile's row r
+    auto slot_of = [&](int r) {
+        const int my = row0 + r;
+        return ((size_t)b.off[i] + my / a.group) * a.heads + h * a.group + my % a.group;
+    };
     if (blk0 >= blk1) {  // nothing to see in this chunk
         if (a.ns > 1) {
             if (tid < rows) {
-                a.part[slot * a.ns + chunk] = -INFINITY;
-                a.part[(a.rows + slot) * a.ns + chunk] = 0.0f;
+                a.part[slot_of(tid) * a.ns + chunk] = -INFINITY;
+                a.part[(a.rows + slot_of(tid)) * a.ns + chunk] = 0.0f;
             }
         } else {
-            for (int e = tid; e < rows * HD; e += NT) {
-                const int rr = row0 + e / HD;
-                a.out[(((size_t)b.off[i] + rr / a.group) * a.heads + h * a.group + rr % a.group) * HD + e % HD] = 0.0f;
-            }
+            for (int e = tid; e < rows * HD; e += NT) a.out[slot_of(e / HD) * HD + e % HD] = 0.0f;
         }
         return;
     }
-
-    // digits of the query rows: a thread takes 16 dims of one row
-    float qscale;
-    {
-        float x[16];
-        const int rr = tid & 15, cc = tid >> 4, qr = row0 + rr;
-        uint32_t am = 0;
+    const size_t head = ((size_t)b.seq[i] * c.nkv + h) * c.nb;
+    i32x4 kk[4][KD], vv[VD];
+    float ks, vs;
+    auto load_k = [&](int blk) {
+        const i32x4* p = (const i32x4*)(c.kc + (head + blk) * KV8_BLOCK * KR) + lane;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = 0.0f;
-        if (tid < KR && rr < rows && cc < HD / 16) {
-            const f32x4* p = (const f32x4*)(a.q + (((size_t)b.off[i] + qr / a.group) * a.heads + h * a.group + qr % a.group) * HD + 16 * cc);
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < KD; ++d) kk[t][d] = p[(t * KD + d) * 64];
+        ks = c.ks[head + blk];
+    };
+    auto load_v = [&](int blk) {
+        const i32x4* p = (const i32x4*)(c.vc + (head + blk) * KV8_BLOCK * HD) + lane;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) vv[d] = p[d * 64];
+        vs = c.vs[head + blk];
+    };
+    int blk = blk0 + wave;
+    if (blk < blk1) {
+        load_k(blk);
+        if (!LATE_V) load_v(blk);
+    }
+
+    // digits of the query rows
+    float qscale;
+    __shared__ i32x4 qs[ROWS == 4 ? 1 : 3][ROWS == 4 ? 1 : KD][ROWS == 4 ? 1 : 64];
+    i32x4 qr[ROWS == 4 ? KD : 1];
+    // score = q . k / sqrt(HD) in units of ln 2; a row that is not finite gives NaN
+    auto score_scale = [](uint32_t m) {
+        return m >= INF_BITS ? __uint_as_float(0x7fc00000u)
+                             : fmaxf(__uint_as_float(m), 0x1p-100f) / DIGIT_MAX * (1.44269504088896340736f / __builtin_sqrtf((float)HD));
+    };
+    // rows that are nearly zero: their digits vanish
+    auto digit_scale = [](uint32_t m) { return DIGIT_MAX / fmaxf(__uint_as_float(m), 0x1p-100f); };
+    auto clamp = [](float v) { return fminf(fmaxf(v, -DIGIT_MAX), DIGIT_MAX); };
+    if constexpr (ROWS == 4) {  // every lane its own, in registers
+        f32x4 x[KD][4];
+        uint32_t m = 0;
+        const f32x4* p = (const f32x4*)(a.q + slot_of(min(col.row, rows - 1)) * HD);
+#pragma unroll
+        for (int d = 0; d < KD; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const f32x4 v = p[j];
-                x[4 * j] = v.x;
-                x[4 * j + 1] = v.y;
-                x[4 * j + 2] = v.z;
-                x[4 * j + 3] = v.w;
-            }
+                x[d][j] = 64 * d + 16 * g < HD ? p[16 * d + 4 * g + j] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 16; ++j) am = max(am, abs_bits(x[j]));
+                for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[d][j][e]));
+            }
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+        const float inv = digit_scale(m);
+#pragma unroll
+        for (int d = 0; d < KD; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t dg[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dg[e] = digits_of(clamp(x[d][j][e] * inv));
+                qr[d][j] = col.bytes(dg, 0);
+            }
+        qscale = score_scale(m);
+    } else {  // a thread 16 dims of one row, through LDS
+        __shared__ uint32_t qmax[KR / 16][16];
+        f32x4 x[4];
+        const int rr = tid & 15, cc = tid >> 4;
+        uint32_t am = 0;
+        const bool in = tid < KR && rr < rows && cc < HD / 16;
+        const f32x4* p = (const f32x4*)(a.q + slot_of(min(rr, rows - 1)) * HD) + 4 * cc;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = in ? p[j] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) am = max(am, abs_bits(x[j][e]));
         }
-        if (tid < KR) qmax[cc][rr] = __uint_as_float(am);
+        if (tid < KR) qmax[cc][rr] = am;
         __syncthreads();
         uint32_t m = 0, mine = 0;
 #pragma unroll
         for (int j = 0; j < KR / 16; ++j) {
-            m = max(m, __float_as_uint(qmax[j][rr]));
-            mine = max(mine, __float_as_uint(qmax[j][r]));
+            m = max(m, qmax[j][rr]);
+            mine = max(mine, qmax[j][col.row]);
         }
-        // rows that are nearly zero: their digits vanish
-        const float inv = DIGIT_MAX / fmaxf(__uint_as_float(m), 0x1p-100f);
+        const float inv = digit_scale(m);
         if (tid < KR) {
-            uint32_t d[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) d[j] = digits_of((int)rintf(fminf(fmaxf(x[j] * inv, -DIGIT_MAX), DIGIT_MAX)));
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
                 i32x4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = digit_bytes(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3], n);
-                qd[n][cc >> 2][(cc & 3) * 16 + rr] = w;
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t dg[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dg[e] = digits_of(clamp(x[j][e] * inv));
+                    w[j] = col.bytes(dg, n);
+                }
+                qs[n][cc >> 2][(cc & 3) * 16 + rr] = w;
             }
         }
-        // score = q . k / sqrt(HD) in units of ln 2; a row that is not finite gives NaN
-        qscale = mine >= INF_BITS ? __uint_as_float(0x7fc00000u)
-                                  : fmaxf(__uint_as_float(mine), 0x1p-100f) / DIGIT_MAX * (1.44269504088896340736f / __builtin_sqrtf((float)HD));
+        qscale = score_scale(mine);
         __syncthreads();
     }
 
+    const int pos = col.row < rows ? len - n_q + (row0 + col.row) / a.group : -1;
+    const int from = a.window ? pos - a.window + 1 : 0;
     float m_run = -INFINITY, l_run = 0.0f;
     f32x4 o[VD];
 #pragma unroll
     for (int d = 0; d < VD; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const size_t head = ((size_t)b.seq[i] * c.nkv + h) * c.nb;
-    for (int blk = blk0 + wave; blk < blk1; blk += 4) {
-        const i32x4* kp = (const i32x4*)(c.kc + (head + blk) * KV8_BLOCK * KR) + lane;
-        const i32x4* vp = (const i32x4*)(c.vc + (head + blk) * KV8_BLOCK * HD) + lane;
-        const float f = qscale * c.ks[head + blk], vs = c.vs[head + blk];
-        i32x4 kk[4][KD], vv[VD];
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int d = 0; d < KD; ++d) kk[t][d] = kp[(t * KD + d) * 64];
-#pragma unroll
-        for (int d = 0; d < VD; ++d) vv[d] = vp[d * 64];
+    for (; blk < blk1; blk += 4) {
+        const float f = qscale * ks;
         float s[16], mb = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            i32x4 acc[3];
+            i32x4 acc[DIG];
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
+            for (int n = 0; n < DIG; ++n) {
                 acc[n] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int d = 0; d < KD; ++d) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[t][d], qd[n][d][lane], acc[n], 0, 0, 0);
+                for (int d = 0; d < KD; ++d) {
+                    if constexpr (ROWS == 4) acc[n] = mfma(kk[t][d], qr[d], acc[n]);
+                    else acc[n] = mfma(kk[t][d], qs[n][d][lane], acc[n]);
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // each sum is below 2^24; the middle one is added to the low one first
-                const float v = fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j])) * f;
-                const int p = blk * KV8_BLOCK + 16 * t + 4 * g + j;
-                const bool in = p <= pos && p >= from;
-                s[4 * t + j] = in ? v : -INFINITY;
-                mb = fmaxf(mb, s[4 * t + j]);
+            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.value(acc, j) * f;
+        }
+        if (LATE_V) load_v(blk);
+        if (!LATE_K && blk + 4 < blk1) load_k(blk + 4);
+        // not every row sees all of the block
+        if (blk * KV8_BLOCK + KV8_BLOCK - 1 > p0 || (a.window && blk * KV8_BLOCK < p1 - a.window + 1)) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int p = blk * KV8_BLOCK + 16 * (j / 4) + 4 * g + j % 4;
+                s[j] = p <= pos && p >= from ? s[j] : -INFINITY;
             }
         }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mb = fmaxf(mb, s[j]);
         mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
         mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
-        // probabilities relative to the block's own maximum
+        // Probabilities relative to the block's own maximum.  A row that sees
+        // nothing of the block has -inf for all its scores, and none of them
+        // may take part whatever the block's scales are; one whose scores are
+        // all NaN has the same maximum, and its sum becomes NaN.
+        const float top = mb == -INFINITY ? 0.0f : mb;
         float lb = 0.0f;
         uint32_t pd[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const int p = blk * KV8_BLOCK + 16 * (j / 4) + 4 * g + j % 4;
-            const float e = p <= pos && p >= from ? exp2_fast(s[j] - mb) : 0.0f;
+            const float e = exp2_fast(s[j] - top);
             lb += e;
-            pd[j] = digits_of((int)rintf(e * DIGIT_MAX));
+            pd[j] = digits_of(e * DIGIT_MAX);
         }
         const float m_new = fmaxf(m_run, mb);
         const float alpha = m_run == m_new ? 1.0f : exp2_fast(m_run - m_new);
         const float beta = mb == -INFINITY ? 0.0f : exp2_fast(mb - m_new);
         m_run = m_new;
-        l_run = l_run * alpha + (mb == -INFINITY ? lb : lb * beta);  // lb is NaN where every score is
-        // a row that sees nothing of the block takes nothing from it, whatever its scale is
+        l_run = l_run * alpha + (mb == -INFINITY ? lb : lb * beta);
         const float w = mb == -INFINITY ? 0.0f : beta * vs * (1.0f / DIGIT_MAX);
-        i32x4 pb[3];
+        i32x4 pb[DIG];
 #pragma unroll
-        for (int n = 0; n < 3; ++n)
+        for (int n = 0; n < DIG; ++n)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) pb[n][t] = digit_bytes(pd[4 * t], pd[4 * t + 1], pd[4 * t + 2], pd[4 * t + 3], n);
+            for (int t = 0; t < 4; ++t) pb[n][t] = col.bytes(pd + 4 * t, n);
+        if (LATE_K && blk + 4 < blk1) load_k(blk + 4);
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < VD; ++d) o[d] *= alpha;
+        }
 #pragma unroll
         for (int d = 0; d < VD; ++d) {
-            i32x4 acc[3];
+            i32x4 acc[DIG];
 #pragma unroll
-            for (int n = 0; n < 3; ++n) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vv[d], pb[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
+            for (int n = 0; n < DIG; ++n) acc[n] = mfma(vv[d], pb[n], i32x4{0, 0, 0, 0});
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float v = fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j]));
-                o[d][j] = fmaf(v, w, o[d][j] * alpha);
-            }
+            for (int j = 0; j < 4; ++j) o[d][j] = fmaf(col.partial(acc, j), w, o[d][j]);
         }
+        if (!LATE_V && blk + 4 < blk1) load_v(blk + 4);
     }
     // join the waves
     l_run += __shfl_xor(l_run, 16, 64);
     l_run += __shfl_xor(l_run, 32, 64);
     if (g == 0) {
-        st_m[wave][r] = m_run;
-        st_l[wave][r] = l_run;
+        st_m[wave][col.row] = m_run;
+        st_l[wave][col.row] = l_run;
+    }
+    if constexpr (ROWS == 4) {
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[d][j] = col.join(o[d][j]);
+            if (d % 4 == col.digit) *(f32x4*)&ob[wave][col.row][16 * d + 4 * g] = o[d];  // a quarter each of the row's four lanes
+        }
     }
     __syncthreads();
+    auto weight = [&](int w, int r, float M) { return st_m[w][r] == -INFINITY ? 0.0f : exp2_fast(st_m[w][r] - M); };
+    auto put = [&](int r, int q4, f32x4 v, float M, float L) {  // dims 4 q4 .. of the tile's row r
+        const size_t slot = slot_of(r);
+        if (a.ns > 1) {
+            const size_t at = slot * a.ns + chunk;
+            if (q4 == 0) {
+                a.part[at] = M;
+                a.part[a.rows * a.ns + at] = L;
+            }
+            ((f32x4*)(a.part + 2 * a.rows * a.ns + at * HD))[q4] = v;
+        } else {
+            ((f32x4*)(a.out + slot * HD))[q4] = v * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
+        }
+    };
+    const int jr = ROWS == 4 ? tid / (HD / 4) : col.row;  // row that this thread joins
+    if (ROWS == 4 && jr >= rows) return;
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, st_m[w][r]);
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, st_m[w][jr]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) L += st_l[w][r] * (st_m[w][r] == -INFINITY ? 0.0f : exp2_fast(st_m[w][r] - M));
-    const float mine = m_run == -INFINITY ? 0.0f : exp2_fast(m_run - M);
+    for (int w = 0; w < 4; ++w) L += st_l[w][jr] * weight(w, jr, M);
+    if constexpr (ROWS == 4) {
+        const int q4 = tid % (HD / 4);
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int d = 0; d < VD; ++d) o[d] *= mine;
-#pragma unroll
-    for (int half = 2; half > 0; half >>= 1) {
-        if (wave >= half && wave < 2 * half)
-#pragma unroll
-            for (int d = 0; d < VD; ++d) *(f32x4*)&ob[wave - half][r][16 * d + 4 * g] = o[d];
-        __syncthreads();
-        if (wave < half)
-#pragma unroll
-            for (int d = 0; d < VD; ++d) o[d] += *(const f32x4*)&ob[wave][r][16 * d + 4 * g];
-        __syncthreads();
-    }
-    if (wave != 0 || r >= rows) return;
-    if (a.ns > 1) {
-        const size_t at = slot * a.ns + chunk;
-        if (g == 0) {
-            a.part[at] = M;
-            a.part[a.rows * a.ns + at] = L;
-        }
-        f32x4* dst = (f32x4*)(a.part + 2 * a.rows * a.ns + at * HD);
-#pragma unroll
-        for (int d = 0; d < VD; ++d) dst[4 * d + g] = o[d];
+        for (int w = 0; w < 4; ++w) v += *(const f32x4*)&ob[w][jr][4 * q4] * weight(w, jr, M);
+        put(jr, q4, v, M, L);
     } else {
-        const float inv = M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L;
-        f32x4* dst = (f32x4*)(a.out + slot * HD);
+        const float mine = weight(wave, jr, M);
 #pragma unroll
-        for (int d = 0; d < VD; ++d) dst[4 * d + g] = o[d] * inv;
+        for (int d = 0; d < VD; ++d) o[d] *= mine;
+#pragma unroll
+        for (int half = 2; half > 0; half >>= 1) {
+            if (wave >= half && wave < 2 * half)
+#pragma unroll
+                for (int d = 0; d < VD; ++d) *(f32x4*)&ob[wave - half][jr][16 * d + 4 * g] = o[d];
+            __syncthreads();
+            if (wave < half)
+#pragma unroll
+                for (int d = 0; d < VD; ++d) o[d] += *(const f32x4*)&ob[wave][jr][16 * d + 4 * g];
+            __syncthreads();
+        }
+        if (wave != 0 || jr >= rows) return;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) put(jr, 4 * d + g, o[d], M, L);
     }
 }
 
-// Joins the chunk states of one output row.
+// Joins the chunk states of one output row: a workgroup takes 32 of its dims,
+// its threads the chunks side by side, their outputs on the way before the
+// weights are known.
 template <int HD>
 __global__ __launch_bounds__(NT) void k_kv8_combine(Att8 a) {
-    constexpr int LN = HD / 4, GR = NT / LN;  // float4 lanes, groups that share the chunks
+    constexpr int LN = 8, GR = NT / LN, U = 4;  // float4 lanes, groups that share the chunks, loads in flight
     __shared__ float red[8];
     __shared__ __align__(16) f32x4 sum[GR][LN];
-    const size_t slot = blockIdx.x;
+    const size_t slot = blockIdx.x / (HD / 32);
+    const int d4 = blockIdx.x % (HD / 32) * LN;
     const float* pm = a.part + slot * a.ns;
     const float* pl = a.part + (a.rows + slot) * a.ns;
-    const f32x4* po = (const f32x4*)(a.part + 2 * a.rows * a.ns + slot * a.ns * HD);
+    const f32x4* po = (const f32x4*)(a.part + 2 * a.rows * a.ns + slot * a.ns * HD) + d4;
     const int tid = threadIdx.x, ln = tid % LN, gr = tid / LN;
-    float m = -INFINITY;
-    for (int j = tid; j < a.ns; j += NT) m = fmaxf(m, pm[j]);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    // m and l of the thread's first chunk for the row's sums
+    const float m0 = tid < a.ns ? pm[tid] : -INFINITY, l0 = tid < a.ns ? pl[tid] : 0.0f;
+    f32x4 v[U];
+    float mv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int j = min(gr + u * GR, a.ns - 1);
+        v[u] = po[(size_t)j * (HD / 4) + ln];
+        mv[u] = pm[j];
+    }
+    m = m0;
+    for (int j = tid + NT; j < a.ns; j += NT) m = fmaxf(m, pm[j]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
     const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float l = 0.0f;
-    for (int j = tid; j < a.ns; j += NT) l += pl[j] * (pm[j] == -INFINITY ? 0.0f : exp2_fast(pm[j] - M));
+    auto weight = [&](float x) { return x == -INFINITY ? 0.0f : exp2_fast(x - M); };
+    l = l0 * weight(m0);
+    for (int j = tid + NT; j < a.ns; j += NT) l += pl[j] * weight(pm[j]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, 64);
     if ((tid & 63) == 0) red[4 + (tid >> 6)] = l;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int j = gr; j < a.ns; j += GR)
-        if (pm[j] != -INFINITY) acc += po[(size_t)j * LN + ln] * exp2_fast(pm[j] - M);  // a chunk that saw nothing wrote no output
+    // a chunk that saw nothing wrote no output
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (gr + u * GR < a.ns && mv[u] != -INFINITY) acc += v[u] * weight(mv[u]);
+    for (int j = gr + U * GR; j < a.ns; j += GR)
+        if (pm[j] != -INFINITY) acc += po[(size_t)j * (HD / 4) + ln] * weight(pm[j]);
     sum[gr][ln] = acc;
     __syncthreads();
-    if (tid < LN) {
+    if (tid < 32) {
+        const float* t = (const float*)sum;
         const float L = (red[4] + red[5]) + (red[6] + red[7]);
+        float r = 0.0f;
 #pragma unroll
-        for (int j = 1; j < GR; ++j) acc += sum[j][ln];
-        const float inv = M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L;
-        ((f32x4*)(a.out + slot * HD))[ln] = acc * inv;
+        for (int j = 0; j < GR; ++j) r += t[j * 32 + tid];
+        a.out[slot * HD + 4 * d4 + tid] = r * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
     }
 }
 
@@ -607,8 +748,10 @@ int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int block
 
 int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t s) {
     return with_hd(hd, [&](auto h) {
-        hipLaunchKernelGGL(k_kv8_attention<h.value>, dim3(a.ns * c.nkv * a.tiles, 1, n), dim3(NT), 0, s, c, b, a);
-        if (a.ns > 1) hipLaunchKernelGGL(k_kv8_combine<h.value>, dim3(a.rows), dim3(NT), 0, s, a);
+        const dim3 grid(a.ns * c.nkv * a.tiles, 1, n);
+        if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value, Narrow>), grid, dim3(NT), 0, s, c, b, a);
+        else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide>), grid, dim3(NT), 0, s, c, b, a);
+        if (a.ns > 1) hipLaunchKernelGGL(k_kv8_combine<h.value>, dim3(a.rows * (h.value / 32)), dim3(NT), 0, s, a);
     });
 }
 
