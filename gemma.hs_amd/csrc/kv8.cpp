@@ -12,6 +12,7 @@ namespace {
 
 constexpr int MAX_SEQ = 1 << 22;   // tokens a sequence
 constexpr int MAX_ROWS = 1 << 20;  // query rows a kv head and sequence
+constexpr int MAX_GROUP = 1024;    // heads a kv head: rows * group stays below 2^32 (Att8::group_inv)
 constexpr int MAX_GRID = 1 << 23;  // workgroups of 256 threads in a grid's x (2^32 threads at most)
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -255,6 +256,7 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
     if (n_heads <= 0 || n_heads % kv->nkv || window < 0)
         return set_error(GH_ERR_INVALID, "gh_kv8_attention: %d heads over %d kv heads, window %d", n_heads, kv->nkv, window);
     const int group = n_heads / kv->nkv;
+    if (group > MAX_GROUP) return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d heads a kv head", group);
     int64_t total = 0;
     for (int i = 0; i < n; ++i) {
         if (n_q[i] < 0) return set_error(GH_ERR_INVALID, "gh_kv8_attention: %d query tokens", n_q[i]);
@@ -295,12 +297,12 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
         a.chunk = (int)std::max<int64_t>(4, (work / 512 + 3) / 4 * 4);
         a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
         if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
-            return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows of %d kv heads in one call",
-                             rows, kv->nkv);
+            return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows in one call", rows);
         a.q = q;
         a.out = out;
         a.heads = n_heads;
         a.group = group;
+        a.group_inv = group == 1 ? 0 : (unsigned)(((uint64_t(1) << 32) + group - 1) / group);
         a.window = window;
         a.rows = (size_t)b.off[m] * n_heads;
         if (a.ns > 1) {

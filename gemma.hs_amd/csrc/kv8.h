@@ -62,7 +62,8 @@ struct Att8 {
     float* out;
     float* part;  // chunk states: m [rows][ns], l [rows][ns], o [rows][ns][hd]; rows = heads * query tokens
     size_t rows;
-    int heads, group;  // query heads, per kv head
+    int heads, group;    // query heads, per kv head
+    unsigned group_inv;  // ceil(2^32 / group): the upper half of row * group_inv is row / group (0 for group 1)
     int window;
     int tile;   // rows a tile
     int tiles;  // row tiles of the longest entry

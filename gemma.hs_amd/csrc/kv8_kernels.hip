@@ -313,20 +313,32 @@ __global__ __launch_bounds__(NT) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k,
 // (2^-24 a: what rounding a to f32 costs).  Three products give the integer
 // dot product; no code is ever converted.
 constexpr float DIGIT_MAX = 8355711.0f;
-// digits of v, |v| <= DIGIT_MAX, as the three low bytes: adding 128 (65536 +
-// 256 + 1) makes every digit an unsigned byte, 128 too large
-__device__ __forceinline__ uint32_t digits_of(float v) { return ((uint32_t)((int)rintf(v) + 0x808080)) ^ 0x808080u; }
+// Digits of v, |v| <= DIGIT_MAX, as the three low bytes, 128 too large: adding
+// 128 (65536 + 256 + 1) makes every digit an unsigned byte.
+__device__ __forceinline__ uint32_t digits_of(float v) { return (uint32_t)((int)rintf(v) + 0x808080); }
+// The same for DIGIT_MAX p with 0 <= p <= 1, the two low digits 128 too large:
+// an f32 between 2^23 and 2^24 has its integer in its low bits, and the sum
+// below stays in front of 2^24.
+__device__ __forceinline__ uint32_t digits_of_share(float p) { return __float_as_uint(fmaf(p, DIGIT_MAX, 0x1p23f + 0x8080)); }
+constexpr uint32_t DIGIT_BIAS = 0x80808080u;  // what an exclusive or takes off four digits that are 128 too large
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
 constexpr int DPP_ROW_ROR4 = 0x124, DPP_ROW_ROR8 = 0x128;
 
 __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+// byte n of four words
+__device__ __forceinline__ uint32_t byte_of(const uint32_t* d, int n) {
+    const uint32_t lo = __builtin_amdgcn_perm(d[1], d[0], n == 0 ? 0x0c0c0400u : n == 1 ? 0x0c0c0501u : 0x0c0c0602u);
+    const uint32_t hi = __builtin_amdgcn_perm(d[3], d[2], n == 0 ? 0x04000c0cu : n == 1 ? 0x05010c0cu : 0x06020c0cu);
+    return lo | hi;
 }
 
 // The 16 columns of a product: 16 query rows, a product for each digit
@@ -335,74 +347,94 @@ __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
 // where a kv head has few query rows: a third of the products, and of the
 // conversions of their results.
 struct Wide {
-    static constexpr int ROWS = 16, DIG = 3;
+    static constexpr int ROWS = 16, DIG = 3, WAVES = 4;
     int row;
     __device__ __forceinline__ explicit Wide(int col) : row(col) {}
-    // digit n of four packed values as four bytes
-    __device__ __forceinline__ int bytes(const uint32_t* d, int n) const {
-        const uint32_t lo = __builtin_amdgcn_perm(d[1], d[0], n == 0 ? 0x0c0c0400u : n == 1 ? 0x0c0c0501u : 0x0c0c0602u);
-        const uint32_t hi = __builtin_amdgcn_perm(d[3], d[2], n == 0 ? 0x04000c0cu : n == 1 ? 0x05010c0cu : 0x06020c0cu);
-        return (int)(lo | hi);
+    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return *p; }  // other tiles read the same codes
+    // digit n of four probabilities
+    __device__ __forceinline__ int share(const uint32_t* d, int n) const {
+        return (int)(n < 2 ? byte_of(d, n) ^ DIGIT_BIAS : byte_of(d, n));
     }
-    // a product's values: each sum is below 2^24
-    __device__ __forceinline__ float value(const i32x4* acc, int j) const {
+    // column of digit n of a query row in the digit's operand
+    __device__ __forceinline__ static int place(int r, int) { return r; }
+    __device__ __forceinline__ static int operand(int n) { return n; }
+    // a product's value times w: each sum is below 2^24
+    __device__ __forceinline__ float scaled(float w) const { return w; }
+    __device__ __forceinline__ float sum(const i32x4* acc, int j) const {
         return fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j]));
     }
-    __device__ __forceinline__ float partial(const i32x4* acc, int j) const { return value(acc, j); }
     __device__ __forceinline__ float join(float v) const { return v; }
 };
 struct Narrow {
-    static constexpr int ROWS = 4, DIG = 1;
+    static constexpr int ROWS = 4, DIG = 1, WAVES = 8;
     int row, digit;
-    uint32_t lo, hi;  // byte selectors of the lane's digit
+    uint32_t lo, hi, bias;  // byte selectors of the lane's digit, and what its bytes are too large
     float weight;
+    // each code is read once a call
+    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return __builtin_nontemporal_load(p); }
     __device__ __forceinline__ explicit Narrow(int col) : row(col & 3), digit(col >> 2) {
         lo = digit == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * digit;
         hi = digit == 3 ? 0x0c0c0c0cu : 0x04000c0cu + 0x01010000u * digit;
+        bias = digit < 2 ? DIGIT_BIAS : 0u;
         weight = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
     }
-    __device__ __forceinline__ int bytes(const uint32_t* d, int) const {
-        return (int)(__builtin_amdgcn_perm(d[1], d[0], lo) | __builtin_amdgcn_perm(d[3], d[2], hi));
+    __device__ __forceinline__ int share(const uint32_t* d, int) const {
+        return (int)((__builtin_amdgcn_perm(d[1], d[0], lo) | __builtin_amdgcn_perm(d[3], d[2], hi)) ^ bias);
     }
+    __device__ __forceinline__ static int place(int r, int n) { return 4 * n + r; }
+    __device__ __forceinline__ static int operand(int) { return 0; }
     // the lane's digit alone; join() adds the row's other two
-    __device__ __forceinline__ float partial(const i32x4* acc, int j) const { return (float)acc[0][j] * weight; }
+    __device__ __forceinline__ float scaled(float w) const { return w * weight; }
+    __device__ __forceinline__ float sum(const i32x4* acc, int j) const { return (float)acc[0][j]; }
     __device__ __forceinline__ float join(float v) const {
         v += dpp<DPP_ROW_ROR8>(v);
         return v + dpp<DPP_ROW_ROR4>(v);
     }
-    __device__ __forceinline__ float value(const i32x4* acc, int j) const { return join(partial(acc, j)); }
 };
 
 // One workgroup: the columns' query rows of one kv head x one chunk of key
-// blocks, the blocks dealt to its 4 waves; each wave keeps its own running
+// blocks, the blocks dealt to its waves; each wave keeps its own running
 // maximum, sum and output, joined through LDS at the end.
 //   S^T = K Q^T   operand A: codes of 16 tokens, B: digits of the query rows;
 //                 lane (g, col) gets tokens 16 t + 4 g + i of its row
 //   O^T = V^T P^T operand A: codes of 16 dims, B: digits of the lane's own
 //                 16 probabilities (the layout of V has their order)
 // The codes of the next block are on their way while the present one is
-// worked on: K's from its products on, V's from the end of the block on.
+// worked on, as far as the registers reach.
 template <int HD, class Cols>
-__global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
-    constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Cols::ROWS, DIG = Cols::DIG;
+__global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
+    constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Cols::ROWS, DIG = Cols::DIG, WAVES = Cols::WAVES;
     constexpr bool LATE_K = HD == 256, LATE_V = HD == 256 && ROWS == 16;
-    __shared__ float st_m[4][ROWS], st_l[4][ROWS];
-    __shared__ __align__(16) float ob[ROWS == 4 ? 4 : 2][ROWS][HD + 4];
-    const int i = blockIdx.z, chunk = blockIdx.x % a.ns, h = blockIdx.x / a.ns % c.nkv;
-    const int row0 = blockIdx.x / a.ns / c.nkv * ROWS;
+    __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
+    __shared__ uint32_t qmax[ROWS];
+    __shared__ i32x4 qs[DIG][KD][64];
+    __shared__ __align__(16) float ob[ROWS == 4 ? WAVES : 2][ROWS][HD + 4];
+    // Narrow: one tile, grid (chunks, kv heads).  Wide: grid x over the kv
+    // heads, then the chunks, then the tiles, the longest (last) first.
+    const int i = blockIdx.z;
+    int h = blockIdx.y, chunk = blockIdx.x, tile = 0;
+    if (ROWS > 4) {
+        const unsigned x = blockIdx.x / (unsigned)c.nkv;
+        h = blockIdx.x - x * c.nkv;
+        const unsigned t = a.ns > 1 ? x / (unsigned)a.ns : x;
+        chunk = x - t * a.ns;
+        tile = a.tiles - 1 - t;
+    }
+    const int row0 = tile * ROWS;
     const int n_q = b.off[i + 1] - b.off[i], rows = min(n_q * a.group - row0, ROWS), len = b.pos[i];
     if (rows <= 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const Cols col(lane & 15);
+    // query token of the tile's row r, and the row's place in q and out
+    auto token_of = [&](int r) { return (int)__umulhi((unsigned)(row0 + r), a.group_inv) + (a.group == 1 ? row0 + r : 0); };
+    auto slot_of = [&](int r) {
+        const int t = token_of(r);
+        return ((size_t)b.off[i] + t) * a.heads + (h * a.group + row0 + r - t * a.group);
+    };
     // positions of the tile's first and last row, and the blocks they see
-    const int p0 = len - n_q + row0 / a.group, p1 = len - n_q + (row0 + rows - 1) / a.group;
+    const int p0 = len - n_q + token_of(0), p1 = len - n_q + token_of(rows - 1);
     const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
     const int blk0 = begin + chunk * a.chunk, blk1 = min(blk0 + a.chunk, end);
-    // output row of the tile's row r
-    auto slot_of = [&](int r) {
-        const int my = row0 + r;
-        return ((size_t)b.off[i] + my / a.group) * a.heads + h * a.group + my % a.group;
-    };
     if (blk0 >= blk1) {  // nothing to see in this chunk
         if (a.ns > 1) {
             if (tid < rows) {
@@ -410,7 +442,7 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
                 a.part[(a.rows + slot_of(tid)) * a.ns + chunk] = 0.0f;
             }
         } else {
-            for (int e = tid; e < rows * HD; e += NT) a.out[slot_of(e / HD) * HD + e % HD] = 0.0f;
+            for (int e = tid; e < rows * HD; e += 64 * WAVES) a.out[slot_of(e / HD) * HD + e % HD] = 0.0f;
         }
         return;
     }
@@ -422,13 +454,13 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int d = 0; d < KD; ++d) kk[t][d] = p[(t * KD + d) * 64];
+            for (int d = 0; d < KD; ++d) kk[t][d] = Cols::load(p + (t * KD + d) * 64);
         ks = c.ks[head + blk];
     };
     auto load_v = [&](int blk) {
         const i32x4* p = (const i32x4*)(c.vc + (head + blk) * KV8_BLOCK * HD) + lane;
 #pragma unroll
-        for (int d = 0; d < VD; ++d) vv[d] = p[d * 64];
+        for (int d = 0; d < VD; ++d) vv[d] = Cols::load(p + d * 64);
         vs = c.vs[head + blk];
     };
     int blk = blk0 + wave;
@@ -437,90 +469,45 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
         if (!LATE_V) load_v(blk);
     }
 
-    // digits of the query rows
-    float qscale;
-    __shared__ i32x4 qs[ROWS == 4 ? 1 : 3][ROWS == 4 ? 1 : KD][ROWS == 4 ? 1 : 64];
-    i32x4 qr[ROWS == 4 ? KD : 1];
-    // score = q . k / sqrt(HD) in units of ln 2; a row that is not finite gives NaN
-    auto score_scale = [](uint32_t m) {
-        return m >= INF_BITS ? __uint_as_float(0x7fc00000u)
-                             : fmaxf(__uint_as_float(m), 0x1p-100f) / DIGIT_MAX * (1.44269504088896340736f / __builtin_sqrtf((float)HD));
-    };
-    // rows that are nearly zero: their digits vanish
-    auto digit_scale = [](uint32_t m) { return DIGIT_MAX / fmaxf(__uint_as_float(m), 0x1p-100f); };
-    auto clamp = [](float v) { return fminf(fmaxf(v, -DIGIT_MAX), DIGIT_MAX); };
-    if constexpr (ROWS == 4) {  // every lane its own, in registers
-        f32x4 x[KD][4];
-        uint32_t m = 0;
-        const f32x4* p = (const f32x4*)(a.q + slot_of(min(col.row, rows - 1)) * HD);
+    // digits of the query rows, a wave a row, a lane 4 dims
+#pragma unroll 1
+    for (int r = wave; r < ROWS; r += WAVES) {
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < rows && 4 * lane < HD) x = ((const f32x4*)(a.q + slot_of(r) * HD))[lane];
+        uint32_t m = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
 #pragma unroll
-        for (int d = 0; d < KD; ++d)
+        for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+        // a row that is nearly zero: its digits vanish
+        const float inv = DIGIT_MAX / fmaxf(__uint_as_float(m), 0x1p-100f);
+        uint32_t dg[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[d][j] = 64 * d + 16 * g < HD ? p[16 * d + 4 * g + j] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int e = 0; e < 4; ++e) dg[e] = digits_of(fminf(fmaxf(x[e] * inv, -DIGIT_MAX), DIGIT_MAX));
+        if (4 * lane < KR) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[d][j][e]));
-            }
-        m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-        const float inv = digit_scale(m);
-#pragma unroll
-        for (int d = 0; d < KD; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t dg[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dg[e] = digits_of(clamp(x[d][j][e] * inv));
-                qr[d][j] = col.bytes(dg, 0);
-            }
-        qscale = score_scale(m);
-    } else {  // a thread 16 dims of one row, through LDS
-        __shared__ uint32_t qmax[KR / 16][16];
-        f32x4 x[4];
-        const int rr = tid & 15, cc = tid >> 4;
-        uint32_t am = 0;
-        const bool in = tid < KR && rr < rows && cc < HD / 16;
-        const f32x4* p = (const f32x4*)(a.q + slot_of(min(rr, rows - 1)) * HD) + 4 * cc;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x[j] = in ? p[j] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) am = max(am, abs_bits(x[j][e]));
+            for (int n = 0; n < (ROWS == 4 ? 4 : 3); ++n)
+                ((uint32_t*)&qs[Cols::operand(n)][lane >> 4][(lane >> 2 & 3) * 16 + Cols::place(r, n)])[lane & 3] =
+                    n < 3 ? byte_of(dg, n) ^ DIGIT_BIAS : 0u;
         }
-        if (tid < KR) qmax[cc][rr] = am;
-        __syncthreads();
-        uint32_t m = 0, mine = 0;
-#pragma unroll
-        for (int j = 0; j < KR / 16; ++j) {
-            m = max(m, qmax[j][rr]);
-            mine = max(mine, qmax[j][col.row]);
-        }
-        const float inv = digit_scale(m);
-        if (tid < KR) {
-#pragma unroll
-            for (int n = 0; n < 3; ++n) {
-                i32x4 w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t dg[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dg[e] = digits_of(clamp(x[j][e] * inv));
-                    w[j] = col.bytes(dg, n);
-                }
-                qs[n][cc >> 2][(cc & 3) * 16 + rr] = w;
-            }
-        }
-        qscale = score_scale(mine);
-        __syncthreads();
+        if (lane == 0) qmax[r] = m;
     }
-
-    const int pos = col.row < rows ? len - n_q + (row0 + col.row) / a.group : -1;
+    __syncthreads();
+    // score = q . k / sqrt(HD) in units of ln 2; a row that is not finite gives NaN
+    float qscale;
+    {
+        const uint32_t m = qmax[col.row];
+        qscale = m >= INF_BITS ? __uint_as_float(0x7fc00000u)
+                               : fmaxf(__uint_as_float(m), 0x1p-100f) * (1.44269504088896340736f / DIGIT_MAX / (HD == 32 ? 5.65685424949238f : HD == 64 ? 8.0f : HD == 128 ? 11.3137084989848f : 16.0f));
+        qscale = col.scaled(qscale);
+    }
+    const int pos = col.row < rows ? len - n_q + token_of(col.row) : -1;
     const int from = a.window ? pos - a.window + 1 : 0;
     float m_run = -INFINITY, l_run = 0.0f;
     f32x4 o[VD];
 #pragma unroll
     for (int d = 0; d < VD; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (; blk < blk1; blk += 4) {
+    for (; blk < blk1; blk += WAVES) {
+        int at = lane;
+        asm volatile("" : "+v"(at));  // q's digits are read again for each block: no registers to keep them in
         const float f = qscale * ks;
         float s[16], mb = -INFINITY;
 #pragma unroll
@@ -531,15 +518,14 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
                 acc[n] = i32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < KD; ++d) {
-                    if constexpr (ROWS == 4) acc[n] = mfma(kk[t][d], qr[d], acc[n]);
-                    else acc[n] = mfma(kk[t][d], qs[n][d][lane], acc[n]);
+                    acc[n] = mfma(kk[t][d], qs[n][d][at], acc[n]);
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.value(acc, j) * f;
+            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.join(col.sum(acc, j) * f);
         }
         if (LATE_V) load_v(blk);
-        if (!LATE_K && blk + 4 < blk1) load_k(blk + 4);
+        if (!LATE_K && blk + WAVES < blk1) load_k(blk + WAVES);
         // not every row sees all of the block
         if (blk * KV8_BLOCK + KV8_BLOCK - 1 > p0 || (a.window && blk * KV8_BLOCK < p1 - a.window + 1)) {
 #pragma unroll
@@ -563,20 +549,21 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
         for (int j = 0; j < 16; ++j) {
             const float e = exp2_fast(s[j] - top);
             lb += e;
-            pd[j] = digits_of(e * DIGIT_MAX);
+            pd[j] = digits_of_share(e);
         }
         const float m_new = fmaxf(m_run, mb);
         const float alpha = m_run == m_new ? 1.0f : exp2_fast(m_run - m_new);
         const float beta = mb == -INFINITY ? 0.0f : exp2_fast(mb - m_new);
         m_run = m_new;
         l_run = l_run * alpha + (mb == -INFINITY ? lb : lb * beta);
-        const float w = mb == -INFINITY ? 0.0f : beta * vs * (1.0f / DIGIT_MAX);
+        const float w = mb == -INFINITY ? 0.0f : col.scaled(beta * vs * (1.0f / DIGIT_MAX));
         i32x4 pb[DIG];
 #pragma unroll
         for (int n = 0; n < DIG; ++n)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) pb[n][t] = col.bytes(pd + 4 * t, n);
-        if (LATE_K && blk + 4 < blk1) load_k(blk + 4);
+            for (int t = 0; t < 4; ++t) pb[n][t] = col.share(pd + 4 * t, n);
+        __builtin_amdgcn_sched_barrier(0);  // scores and probabilities leave their registers here
+        if (LATE_K && blk + WAVES < blk1) load_k(blk + WAVES);
         if (__any(alpha != 1.0f)) {
 #pragma unroll
             for (int d = 0; d < VD; ++d) o[d] *= alpha;
@@ -587,9 +574,9 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
 #pragma unroll
             for (int n = 0; n < DIG; ++n) acc[n] = mfma(vv[d], pb[n], i32x4{0, 0, 0, 0});
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[d][j] = fmaf(col.partial(acc, j), w, o[d][j]);
+            for (int j = 0; j < 4; ++j) o[d][j] = fmaf(col.sum(acc, j), w, o[d][j]);
         }
-        if (!LATE_V && blk + 4 < blk1) load_v(blk + 4);
+        if (!LATE_V && blk + WAVES < blk1) load_v(blk + WAVES);
     }
     // join the waves
     l_run += __shfl_xor(l_run, 16, 64);
@@ -599,11 +586,21 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
         st_l[wave][col.row] = l_run;
     }
     if constexpr (ROWS == 4) {
+        // the row's four lanes add their digits' parts; each writes a quarter (all of it where there are fewer)
+        constexpr int STEP = VD < 4 ? 1 : 4;
 #pragma unroll
-        for (int d = 0; d < VD; ++d) {
+        for (int d = 0; d < VD; d += STEP) {
+            f32x4 v[STEP];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[d][j] = col.join(o[d][j]);
-            if (d % 4 == col.digit) *(f32x4*)&ob[wave][col.row][16 * d + 4 * g] = o[d];  // a quarter each of the row's four lanes
+            for (int e = 0; e < STEP; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[e][j] = col.join(o[d + e][j]);
+            f32x4 mine = v[0];
+            if constexpr (STEP == 4) {
+                const f32x4 x = col.digit & 1 ? v[1] : v[0], y = col.digit & 1 ? v[3] : v[2];
+                mine = col.digit & 2 ? y : x;
+            }
+            *(f32x4*)&ob[wave][col.row][16 * (d + (STEP == 4 ? col.digit : 0)) + 4 * g] = mine;
         }
     }
     __syncthreads();
@@ -625,21 +622,25 @@ __global__ __launch_bounds__(NT, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, A
     if (ROWS == 4 && jr >= rows) return;
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, st_m[w][jr]);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) L += st_l[w][jr] * weight(w, jr, M);
+    for (int w = 0; w < WAVES; ++w) M = fmaxf(M, st_m[w][jr]);
     if constexpr (ROWS == 4) {
         const int q4 = tid % (HD / 4);
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v += *(const f32x4*)&ob[w][jr][4 * q4] * weight(w, jr, M);
+        for (int w = 0; w < WAVES; ++w) {
+            const float x = weight(w, jr, M);
+            L += st_l[w][jr] * x;
+            v += *(const f32x4*)&ob[w][jr][4 * q4] * x;
+        }
         put(jr, q4, v, M, L);
     } else {
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) L += st_l[w][jr] * weight(w, jr, M);
         const float mine = weight(wave, jr, M);
 #pragma unroll
         for (int d = 0; d < VD; ++d) o[d] *= mine;
-#pragma unroll
-        for (int half = 2; half > 0; half >>= 1) {
+#pragma unroll 1
+        for (int half = WAVES / 2; half > 0; half >>= 1) {
             if (wave >= half && wave < 2 * half)
 #pragma unroll
                 for (int d = 0; d < VD; ++d) *(f32x4*)&ob[wave - half][jr][16 * d + 4 * g] = o[d];
@@ -748,9 +749,8 @@ int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int block
 
 int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t s) {
     return with_hd(hd, [&](auto h) {
-        const dim3 grid(a.ns * c.nkv * a.tiles, 1, n);
-        if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value, Narrow>), grid, dim3(NT), 0, s, c, b, a);
-        else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide>), grid, dim3(NT), 0, s, c, b, a);
+        if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value, Narrow>), dim3(a.ns, c.nkv, n), dim3(64 * Narrow::WAVES), 0, s, c, b, a);
+        else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide::WAVES), 0, s, c, b, a);
         if (a.ns > 1) hipLaunchKernelGGL(k_kv8_combine<h.value>, dim3(a.rows * (h.value / 32)), dim3(NT), 0, s, a);
     });
 }
