@@ -18,14 +18,18 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 constexpr uint32_t INF_BITS = 0x7f800000u;
 
-// Max over the 256 threads (two barriers; `slot`: 4 words of LDS).
+// Max over the workgroup (one barrier before, one after; `slot`: 16 words of LDS).
+template <int THREADS>
 __device__ __forceinline__ uint32_t block_max_u32(uint32_t v, uint32_t* slot) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
     __syncthreads();
-    return max(max(slot[0], slot[1]), max(slot[2], slot[3]));
+    v = slot[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) v = max(v, slot[w]);
+    return v;
 }
 
 // ------------------------------------------------------------------
@@ -42,156 +46,159 @@ __device__ __forceinline__ float scale_of(uint32_t a) {
 // most, and only near the middle between two codes; x - c s fits into 24
 // bits there (a multiple of the smaller ulp, no larger than s / 2 and a bit),
 // so one fma gives it without rounding and its comparison with s / 2 decides.
+// A NaN scale gives 0.
 __device__ __forceinline__ int code_of(float x, float s, float inv) {
     const float c = rintf(x * inv), r = fmaf(-c, s, x), h = 0.5f * s;
     int k = (int)c;
     if (fabsf(r) > h || (fabsf(r) == h && (k & 1))) k += r > 0.0f ? 1 : -1;
-    return k;
+    return s == s ? k : 0;
 }
 
-// A thread's items of a block: 16 values that share 16 bytes of codes.  K:
-// 16 dims of one row; V: 16 rows of one dim (the layout in kv8.h).
+// A block as one workgroup takes it, 16 values a thread.  K: 4 dims of rows
+// row, row + 16, ..., whole rows a load instruction; V: 16 rows of one dim,
+// whose codes are 16 consecutive bytes (the layout in kv8.h).
 template <int HD, bool V>
 struct Item {
-    static constexpr int N = 64 * HD / 16;              // items of a block
-    static constexpr int PER = (N + NT - 1) / NT;       // per thread
-    int at;  // byte offset of the item's codes in the block
-    int row, col;  // K: row, first dim; V: first row (g), dim
+    static constexpr int N = 4 * HD;  // the workgroup's threads
+    int row, col;  // first row, first dim
     __device__ __forceinline__ explicit Item(int e) {
-        if (V) {
-            const int d = e % HD, g = e / HD;
-            row = 4 * g;
-            col = d;
-            at = ((d / 16) * 64 + g * 16 + d % 16) * 16;
-        } else {
-            constexpr int KC = HD / 16, KD = HD < 64 ? 1 : HD / 64;
-            const int rr = e % 16, c = e / 16 % KC, t = e / (16 * KC);
-            row = 16 * t + rr;
-            col = 16 * c;
-            at = ((t * KD + c / 4) * 64 + (c % 4) * 16 + rr) * 16;
-        }
+        row = V ? e / HD * 4 : e / (HD / 4);
+        col = V ? e % HD : e % (HD / 4) * 4;
+    }
+    // byte offset of a value's code
+    __device__ __forceinline__ static int place(int r, int d) {
+        if (V) return ((d / 16) * 64 + (r / 4 % 4) * 16 + d % 16) * 16 + r / 16 * 4 + r % 4;
+        constexpr int KD = HD < 64 ? 1 : HD / 64;
+        return ((r / 16 * KD + d / 64) * 64 + (d / 16 % 4) * 16 + r % 16) * 16 + d % 16;
     }
     // row of value j
-    __device__ __forceinline__ int row_of(int j) const { return V ? row + 16 * (j / 4) + j % 4 : row; }
+    __device__ __forceinline__ int row_of(int j) const { return row + 16 * (j / 4) + (V ? j % 4 : 0); }
 };
 
+// The item's values of the rows below r1: those below r0 from the f32 rows
+// kept of the block, the others from src (row 0 of the block, `ld` floats a
+// row); 0 behind r1.  Rows out of reach are replaced by the last one for the
+// load, so that no load waits for a branch.
 template <int HD, bool V>
-using Items = float[Item<HD, V>::PER][16];
-
-// Values of the item's rows in [lo, hi) from src (row 0 of the block, `ld` floats a row).
-template <int HD, bool V>
-__device__ __forceinline__ void load_item(const Item<HD, V>& it, const float* src, size_t ld, int lo, int hi, float (&x)[16]) {
+__device__ __forceinline__ void load_item(const Item<HD, V>& it, const float* tail, const float* src, size_t ld, int r0, int r1,
+                                          float (&x)[16]) {
+    auto at = [&](int j) {
+        const int r = min(it.row_of(j), r1 - 1);
+        return r < r0 ? tail + r * HD + it.col : src + (ptrdiff_t)r * (ptrdiff_t)ld + it.col;
+    };
     if (V) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int r = it.row_of(j);
-            if (r >= lo && r < hi) x[j] = src[(size_t)r * ld + it.col];
-        }
-    } else if (it.row >= lo && it.row < hi) {
-        const f32x4* p = (const f32x4*)(src + (size_t)it.row * ld + it.col);
+        for (int j = 0; j < 16; ++j) x[j] = __builtin_nontemporal_load(at(j));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const f32x4 v = p[j];
-            x[4 * j] = v.x;
-            x[4 * j + 1] = v.y;
-            x[4 * j + 2] = v.z;
-            x[4 * j + 3] = v.w;
-        }
+        for (int j = 0; j < 16; ++j) x[j] = it.row_of(j) < r1 ? x[j] : 0.0f;
+    } else {
+        f32x4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __builtin_nontemporal_load((const f32x4*)at(4 * j));
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = it.row_of(j) < r1 ? v[j / 4][j % 4] : 0.0f;
+    }
+}
+
+// The item's values of rows [lo, hi) to dst (row 0, `ld` floats a row).
+template <int HD, bool V>
+__device__ __forceinline__ void store_item(const Item<HD, V>& it, float* dst, size_t ld, int lo, int hi, const float (&x)[16]) {
+    auto at = [&](int j) { return dst + (ptrdiff_t)it.row_of(j) * (ptrdiff_t)ld + it.col; };
+#pragma unroll
+    for (int j = 0; j < 16; j += V ? 1 : 4) {
+        const int r = it.row_of(j);
+        if (r < lo || r >= hi) continue;
+        if (V) *at(j) = x[j];
+        else *(f32x4*)at(j) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
     }
 }
 
 template <int HD, bool V>
-__device__ __forceinline__ void store_rows(const Item<HD, V>& it, float* dst, int lo, int hi, const float (&x)[16]) {
-    if (V) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int r = it.row_of(j);
-            if (r >= lo && r < hi) dst[r * HD + it.col] = x[j];
-        }
-    } else if (it.row >= lo && it.row < hi) {
-        f32x4* p = (f32x4*)(dst + it.row * HD + it.col);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = f32x4{x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
-    }
-}
-
-// Codes of the item's rows in [lo, hi); the rows in front of lo stay as they are.
-template <int HD, bool V>
-__device__ __forceinline__ void store_codes(const Item<HD, V>& it, int8_t* block, int lo, int hi, float s, const float (&x)[16]) {
+__device__ __forceinline__ void store_codes(const Item<HD, V>& it, int8_t* block, float s, const float (&x)[16]) {
     const float inv = 1.0f / s;
-    const bool ok = s == s;
     union {
         int8_t b[16];
+        int i[4];
         i32x4 w;
     } u;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) u.b[j] = ok ? (int8_t)code_of(x[j], s, inv) : 0;
-    if (V && lo > 0) {
+    for (int j = 0; j < 16; ++j) u.b[j] = (int8_t)code_of(x[j], s, inv);
+    int8_t* at = block + Item<HD, V>::place(it.row, it.col);
+    if (V) *(i32x4*)at = u.w;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int r = it.row_of(j);
-            if (r >= lo && r < hi) block[it.at + j] = u.b[j];
-        }
-    } else if (V || (it.row >= lo && it.row < hi)) {
-        *(i32x4*)(block + it.at) = u.w;
-    }
+    for (int j = 0; !V && j < 4; ++j) *(int*)(block + Item<HD, V>::place(it.row_of(4 * j), it.col)) = u.i[j];
 }
 
+// f32 values of the codes: one product each, rounded once
 template <int HD, bool V>
-__device__ __forceinline__ void zero_items(Items<HD, V>& x) {
+__device__ __forceinline__ void read_item(const Item<HD, V>& it, const int8_t* block, float s, float (&x)[16]) {
+    union {
+        int8_t b[16];
+        int i[4];
+        i32x4 w;
+    } u;
+    if (V) u.w = __builtin_nontemporal_load((const i32x4*)(block + Item<HD, V>::place(it.row, it.col)));
 #pragma unroll
-    for (int i = 0; i < Item<HD, V>::PER; ++i)
+    for (int j = 0; !V && j < 4; ++j)
+        u.i[j] = __builtin_nontemporal_load((const int*)(block + Item<HD, V>::place(it.row_of(4 * j), it.col)));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[i][j] = 0.0f;
+    for (int j = 0; j < 16; ++j) x[j] = (float)u.b[j] * s;
 }
 
-template <int HD, bool V>
-__device__ __forceinline__ uint32_t amax_items(const Items<HD, V>& x, uint32_t* slot) {
+__device__ __forceinline__ uint32_t amax(const float (&x)[16]) {
     uint32_t a = 0;
 #pragma unroll
-    for (int i = 0; i < Item<HD, V>::PER; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) a = max(a, abs_bits(x[i][j]));
-    return block_max_u32(a, slot);
-}
-
-// f(item, its values) for each of the thread's items
-template <int HD, bool V, class F>
-__device__ __forceinline__ void each_item(Items<HD, V>& x, F&& f) {
-#pragma unroll
-    for (int i = 0; i < Item<HD, V>::PER; ++i) {
-        const int e = i * NT + threadIdx.x;
-        if (Item<HD, V>::N % NT == 0 || e < Item<HD, V>::N) f(Item<HD, V>(e), x[i]);
-    }
+    for (int j = 0; j < 16; ++j) a = max(a, abs_bits(x[j]));
+    return a;
 }
 
 // Rows [r0, r1) of a block come from src (its row 0), the first r0 are there
-// already: codes and f32 rows.
+// already: codes, scale, and with `keep` the f32 rows of the new ones.
 template <int HD, bool V>
 __device__ __forceinline__ void append_block(int8_t* block, float* scale, float* tail, const float* src, size_t ld, int r0,
-                                             int r1, bool keep_rows, uint32_t* slot) {
-    Items<HD, V> x;
-    zero_items<HD, V>(x);
-    const float old = r0 > 0 ? *scale : 0.0f;
-    each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { load_item<HD, V>(it, src, ld, r0, r1, v); });
-    float s = scale_of(amax_items<HD, V>(x, slot));  // its barriers: every thread has read the old scale
-    if (r0 > 0 && !(s == s && old == old)) s = __uint_as_float(0x7fc00000u);
-    else if (r0 > 0) s = fmaxf(s, old);
-    const int lo = r0 > 0 && !(s > old) ? r0 : 0;  // a larger scale: the rows before again, from their f32 values
-    if (lo < r0)
-        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { load_item<HD, V>(it, tail, HD, 0, r0, v); });
-    each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) {
-        store_codes<HD, V>(it, block, lo, r1, s, v);
-        if (keep_rows) store_rows<HD, V>(it, tail, r0, r1, v);
-    });
-    if (threadIdx.x == 0) *scale = s;
+                                             int r1, bool keep, uint32_t* slot) {
+    constexpr int N = Item<HD, V>::N;
+    const int tid = threadIdx.x;
+    float s = 0.0f;
+    if (r0 > 0) {
+        // A few rows behind others: if they do not raise the scale, theirs
+        // are the only codes to write.
+        const float old = *scale;
+        uint32_t a = 0;
+        const int e1 = (r1 - r0) * HD;
+        for (int e = tid; e < e1; e += N) a = max(a, abs_bits(src[(ptrdiff_t)(r0 + e / HD) * (ptrdiff_t)ld + e % HD]));
+        s = scale_of(block_max_u32<N>(a, slot));  // its barriers: every thread has read the old scale
+        if (old != old || s != s) s = __uint_as_float(0x7fc00000u);
+        else s = fmaxf(s, old);
+        if (tid == 0) *scale = s;
+        const bool same = !(s > old);
+        if (same || keep) {
+            const float inv = 1.0f / s;
+            for (int e = tid; e < e1; e += N) {
+                const int r = r0 + e / HD, d = e % HD;
+                const float x = src[(ptrdiff_t)r * (ptrdiff_t)ld + d];
+                if (same) block[Item<HD, V>::place(r, d)] = (int8_t)code_of(x, s, inv);
+                if (keep) tail[r * HD + d] = x;
+            }
+        }
+        if (same) return;
+    }
+    const Item<HD, V> it(tid);
+    float x[16];
+    load_item<HD, V>(it, tail, src, ld, r0, r1, x);
+    if (r0 == 0) {
+        s = scale_of(block_max_u32<N>(amax(x), slot));
+        if (tid == 0) *scale = s;
+        if (keep) store_item<HD, V>(it, tail, HD, 0, r1, x);
+    }
+    store_codes<HD, V>(it, block, s, x);
 }
 
 // One workgroup per block that the new tokens touch, kv head and K or V.
 // Reads 4 bytes an element and writes 1: bound by memory.
 template <int HD>
-__global__ __launch_bounds__(NT) void k_kv8_append(Kv8Dev c, Kv8Batch b, const float* k, const float* v) {
-    __shared__ uint32_t slot[4];
+__global__ __launch_bounds__(4 * HD, 8) void k_kv8_append(Kv8Dev c, Kv8Batch b, const float* k, const float* v) {
+    __shared__ uint32_t slot[16];
     const int i = blockIdx.z, h = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
     const int pos = b.pos[i], cnt = b.off[i + 1] - b.off[i], end = pos + cnt;
@@ -216,46 +223,31 @@ __global__ __launch_bounds__(NT) void k_kv8_append(Kv8Dev c, Kv8Batch b, const f
     if (shared_tail && blk == first && left) {
         __syncthreads();
         const float* from = in + ((size_t)b.off[i] + cnt - left) * ld + h * HD;
-        for (int e = threadIdx.x; e < left * (HD / 4); e += NT)
+        for (int e = threadIdx.x; e < left * (HD / 4); e += 4 * HD)
             ((f32x4*)tail)[e] = *(const f32x4*)(from + (size_t)(e / (HD / 4)) * ld + e % (HD / 4) * 4);
     }
-}
-
-// f32 value of a code: one product, rounded once
-template <int HD, bool V>
-__device__ __forceinline__ void read_item(const Item<HD, V>& it, const int8_t* block, float s, float (&x)[16]) {
-    union {
-        int8_t b[16];
-        i32x4 w;
-    } u;
-    u.w = *(const i32x4*)(block + it.at);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = (float)u.b[j] * s;
 }
 
 // A block that keeps its first r1 rows.  same: it was the last one already,
 // its f32 rows are there and are quantised anew; else its values become them.
 template <int HD, bool V>
 __device__ __forceinline__ void truncate_block(int8_t* block, float* scale, float* tail, int r1, bool same, uint32_t* slot) {
-    Items<HD, V> x;
-    zero_items<HD, V>(x);
+    const Item<HD, V> it(threadIdx.x);
+    float x[16];
     if (same) {
-        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { load_item<HD, V>(it, tail, HD, 0, r1, v); });
-        const float s = scale_of(amax_items<HD, V>(x, slot));
-        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) { store_codes<HD, V>(it, block, 0, r1, s, v); });
+        load_item<HD, V>(it, tail, tail, 0, r1, r1, x);
+        const float s = scale_of(block_max_u32<Item<HD, V>::N>(amax(x), slot));
         if (threadIdx.x == 0) *scale = s;
+        store_codes<HD, V>(it, block, s, x);
     } else {
-        const float s = *scale;
-        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&v)[16]) {
-            read_item<HD, V>(it, block, s, v);
-            store_rows<HD, V>(it, tail, 0, r1, v);
-        });
+        read_item<HD, V>(it, block, *scale, x);
+        store_item<HD, V>(it, tail, HD, 0, r1, x);
     }
 }
 
 template <int HD>
-__global__ __launch_bounds__(NT) void k_kv8_truncate(Kv8Dev c, Kv8Batch b) {
-    __shared__ uint32_t slot[4];
+__global__ __launch_bounds__(4 * HD, 8) void k_kv8_truncate(Kv8Dev c, Kv8Batch b) {
+    __shared__ uint32_t slot[16];
     const int i = blockIdx.z, h = blockIdx.y >> 1;
     const int blk = b.off[i] / KV8_BLOCK, r1 = b.off[i] % KV8_BLOCK;
     const bool same = blk == b.pos[i] / KV8_BLOCK;
@@ -268,7 +260,7 @@ __global__ __launch_bounds__(NT) void k_kv8_truncate(Kv8Dev c, Kv8Batch b) {
 }
 
 template <int HD>
-__global__ __launch_bounds__(NT) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k, float* v) {
+__global__ __launch_bounds__(4 * HD, 8) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k, float* v) {
     const int i = blockIdx.z, h = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
     float* out = is_v ? v : k;
@@ -278,28 +270,16 @@ __global__ __launch_bounds__(NT) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k,
     const int r0 = max(pos - blk * KV8_BLOCK, 0), r1 = min(end - blk * KV8_BLOCK, KV8_BLOCK);
     const size_t ld = (size_t)c.nkv * HD, at = ((size_t)b.seq[i] * c.nkv + h) * c.nb + blk;
     float* dst = out + ((ptrdiff_t)b.off[i] + (blk * KV8_BLOCK - pos)) * (ptrdiff_t)ld + h * HD;  // row 0 of the block
-    auto go = [&](auto vv) {
-        constexpr bool V = decltype(vv)::value;
-        const int8_t* block = V ? c.vc + at * KV8_BLOCK * HD : c.kc + at * KV8_BLOCK * kv8_k_row(HD);
-        const float s = V ? c.vs[at] : c.ks[at];
-        Items<HD, V> x;
-        each_item<HD, V>(x, [&](const Item<HD, V>& it, float(&val)[16]) {
-            read_item<HD, V>(it, block, s, val);
-            if (V) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int r = it.row_of(j);
-                    if (r >= r0 && r < r1) dst[(ptrdiff_t)r * (ptrdiff_t)ld + it.col] = val[j];
-                }
-            } else if (it.row >= r0 && it.row < r1) {
-                f32x4* p = (f32x4*)(dst + (ptrdiff_t)it.row * (ptrdiff_t)ld + it.col);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = f32x4{val[4 * j], val[4 * j + 1], val[4 * j + 2], val[4 * j + 3]};
-            }
-        });
-    };
-    if (is_v) go(std::true_type{});
-    else go(std::false_type{});
+    float x[16];
+    if (is_v) {
+        const Item<HD, true> it(threadIdx.x);
+        read_item<HD, true>(it, c.vc + at * KV8_BLOCK * HD, c.vs[at], x);
+        store_item<HD, true>(it, dst, ld, r0, r1, x);
+    } else {
+        const Item<HD, false> it(threadIdx.x);
+        read_item<HD, false>(it, c.kc + at * KV8_BLOCK * kv8_k_row(HD), c.ks[at], x);
+        store_item<HD, false>(it, dst, ld, r0, r1, x);
+    }
 }
 
 // ------------------------------------------------------------------
@@ -731,19 +711,19 @@ int with_hd(int hd, F&& f) {
 int launch_kv8_append(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, const float* k, const float* v,
                       hipStream_t s) {
     return with_hd(hd, [&](auto h) {
-        hipLaunchKernelGGL(k_kv8_append<h.value>, dim3(blocks, 2 * c.nkv, n), dim3(NT), 0, s, c, b, k, v);
+        hipLaunchKernelGGL(k_kv8_append<h.value>, dim3(blocks, 2 * c.nkv, n), dim3(4 * h.value), 0, s, c, b, k, v);
     });
 }
 
 int launch_kv8_truncate(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, hipStream_t s) {
     return with_hd(hd, [&](auto h) {
-        hipLaunchKernelGGL(k_kv8_truncate<h.value>, dim3(1, 2 * c.nkv, n), dim3(NT), 0, s, c, b);
+        hipLaunchKernelGGL(k_kv8_truncate<h.value>, dim3(1, 2 * c.nkv, n), dim3(4 * h.value), 0, s, c, b);
     });
 }
 
 int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, float* k, float* v, hipStream_t s) {
     return with_hd(hd, [&](auto h) {
-        hipLaunchKernelGGL(k_kv8_read<h.value>, dim3(blocks, 2 * c.nkv, n), dim3(NT), 0, s, c, b, k, v);
+        hipLaunchKernelGGL(k_kv8_read<h.value>, dim3(blocks, 2 * c.nkv, n), dim3(4 * h.value), 0, s, c, b, k, v);
     });
 }
 

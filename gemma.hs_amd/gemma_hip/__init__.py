@@ -211,7 +211,7 @@ def _dev(ctx, a):
 
 class _OnDevice:
     """Device addresses of a call's arguments: a DeviceBuffer's, an address as
-    it is, or an upload of a numpy array of the given shape (f32) that lives
+    it is, or an upload of a numpy array of `count` f32 values that lives
     until the block ends."""
 
     def __init__(self, ctx: Context):
@@ -229,21 +229,29 @@ class _OnDevice:
         self.held.append(b)
         return b
 
-    def __call__(self, a, shape=None):
-        if a is None or isinstance(a, C.c_void_p):
+    def __call__(self, a, count=None, itemsize=4):
+        if a is None or isinstance(a, (int, C.c_void_p)):
             return a
-        if isinstance(a, int):
-            return C.c_void_p(a)
         if isinstance(a, DeviceBuffer):
-            if shape is not None and a.nbytes < 4 * int(np.prod(shape, dtype=np.int64)):
-                raise ValueError(f"a buffer of {a.nbytes} bytes is too small for f32 {tuple(shape)}")
+            if count is not None and a.nbytes < itemsize * count:
+                raise ValueError(f"a buffer of {a.nbytes} bytes does not hold {count} values")
             return a.ptr
         a = np.ascontiguousarray(a, dtype=np.float32)
-        if shape is not None and a.size != int(np.prod(shape, dtype=np.int64)):
-            raise ValueError(f"an array of {a.size} values does not hold {tuple(shape)}")
+        if count is not None and a.size != count:
+            raise ValueError(f"an array of {a.size} values where {count} are wanted")
         b = self.new(a.nbytes)
         b.upload(a)
         return b.ptr
+
+
+def _ints(*arrays):
+    """The arrays as contiguous int32 vectors of one length."""
+    out = [np.ascontiguousarray(a, dtype=np.int32) for a in arrays]
+    n = out[0].size
+    for a in out:
+        if a.ndim != 1 or a.size != n:
+            raise ValueError("one entry for each sequence")
+    return out
 
 
 def rmsnorm(ctx: Context, x, w, eps: float = 1e-6, zero_centered: bool = True) -> np.ndarray:
@@ -327,15 +335,15 @@ def sample_rows(ctx: Context, logits, vocab: int, rules: np.ndarray, out=None):
     rules = np.ascontiguousarray(rules)
     if rules.dtype != SAMPLING or rules.ndim != 1:
         raise ValueError("rules must be a one-dimensional array of gemma_hip.SAMPLING")
-    n = len(rules)
+    n = rules.size
+    if type(logits) is int and type(out) is int:
+        check(lib().gh_sample_rows(ctx.h, logits, n, vocab, rules.ctypes.data, out))
+        return out
     with _OnDevice(ctx) as dev:
-        lp = dev(logits, (n, vocab))
-        if out is not None:
-            check(lib().gh_sample_rows(ctx.h, lp, n, int(vocab), _ptr(rules), dev(out)))
-            return out
-        tb = dev.new(4 * n)
-        check(lib().gh_sample_rows(ctx.h, lp, n, int(vocab), _ptr(rules), tb.ptr))
-        return tb.numpy(np.int32, n)
+        lp = dev(logits, n * vocab)
+        tb = dev.new(4 * n) if out is None else None
+        check(lib().gh_sample_rows(ctx.h, lp, n, vocab, rules.ctypes.data, tb.ptr if tb else dev(out, n)))
+        return tb.numpy(np.int32, n) if tb else out
 
 
 def gelu_mul(ctx: Context, g, u) -> np.ndarray:
@@ -589,64 +597,73 @@ class KVCache8:
         self.ctx, self.h = ctx, h
         self.n_seq, self.max_seq, self.n_kv_heads, self.head_dim = n_seq, max_seq, n_kv_heads, head_dim
 
-    @staticmethod
-    def _ints(*arrays):
-        out = [np.ascontiguousarray(a, dtype=np.int32) for a in arrays]
-        if any(a.ndim != 1 or a.size != out[0].size for a in out):
-            raise ValueError("one entry for each sequence")
-        return out
-
     def cacheLength(self, seq: int = 0) -> int:
         n = C.c_int32()
         check(lib().gh_kv8_length(self.h, int(seq), C.byref(n)))
         return n.value
 
+    def _count(self, tokens, heads: int) -> int:
+        return int(tokens.sum(dtype=np.int64)) * heads * self.head_dim
+
     def append(self, seqs, n_tok, k, v) -> None:
         """Append n_tok[i] tokens to sequence seqs[i]; k, v [sum n_tok, n_kv_heads, head_dim]."""
-        seqs, n_tok = self._ints(seqs, n_tok)
-        shape = (int(n_tok.sum(dtype=np.int64)), self.n_kv_heads, self.head_dim)
+        seqs, n_tok = _ints(seqs, n_tok)
+        if type(k) is int and type(v) is int:
+            check(lib().gh_kv8_append(self.h, seqs.size, seqs.ctypes.data, n_tok.ctypes.data, k, v))
+            return
+        count = self._count(n_tok, self.n_kv_heads)
         with _OnDevice(self.ctx) as dev:
-            check(lib().gh_kv8_append(self.h, seqs.size, _ptr(seqs), _ptr(n_tok), dev(k, shape), dev(v, shape)))
+            check(lib().gh_kv8_append(self.h, seqs.size, seqs.ctypes.data, n_tok.ctypes.data, dev(k, count), dev(v, count)))
 
     def truncate(self, seqs, lens) -> None:
         """Rewind sequence seqs[i] to its first lens[i] tokens."""
-        seqs, lens = self._ints(seqs, lens)
-        check(lib().gh_kv8_truncate(self.h, seqs.size, _ptr(seqs), _ptr(lens)))
+        seqs, lens = _ints(seqs, lens)
+        check(lib().gh_kv8_truncate(self.h, seqs.size, seqs.ctypes.data, lens.ctypes.data))
 
     def read(self, seqs, begins, ends, k_out=None, v_out=None):
         """The f32 values of tokens [begins[i], ends[i]) of sequence seqs[i]:
         into k_out and v_out (either may be None), or, with neither, as a pair
         of numpy arrays [sum, n_kv_heads, head_dim]."""
-        seqs, begins, ends = self._ints(seqs, begins, ends)
-        total = int((ends.astype(np.int64) - begins).sum())
-        shape = (max(total, 0), self.n_kv_heads, self.head_dim)
+        seqs, begins, ends = _ints(seqs, begins, ends)
+
+        def call(kp, vp):
+            check(lib().gh_kv8_read(self.h, seqs.size, seqs.ctypes.data, begins.ctypes.data, ends.ctypes.data, kp, vp))
+
+        if type(k_out) is int and type(v_out) is int:
+            call(k_out, v_out)
+            return k_out, v_out
+        count = max(0, self._count(ends.astype(np.int64) - begins, self.n_kv_heads))
         with _OnDevice(self.ctx) as dev:
             if k_out is not None or v_out is not None:
-                check(lib().gh_kv8_read(self.h, seqs.size, _ptr(seqs), _ptr(begins), _ptr(ends), dev(k_out, shape),
-                                        dev(v_out, shape)))
+                call(dev(k_out, count), dev(v_out, count))
                 return k_out, v_out
-            n = int(np.prod(shape, dtype=np.int64))
-            kb, vb = dev.new(4 * n), dev.new(4 * n)
-            check(lib().gh_kv8_read(self.h, seqs.size, _ptr(seqs), _ptr(begins), _ptr(ends), kb.ptr, vb.ptr))
-            return kb.numpy(count=n).reshape(shape), vb.numpy(count=n).reshape(shape)
+            kb, vb = dev.new(4 * count), dev.new(4 * count)
+            call(kb.ptr, vb.ptr)
+            shape = (-1, self.n_kv_heads, self.head_dim)
+            return kb.numpy(count=count).reshape(shape), vb.numpy(count=count).reshape(shape)
 
     def attention(self, seqs, n_q, q, n_heads: int, window: int = 0, out=None):
         """Attention of the last n_q[i] tokens of sequence seqs[i] (their K
         and V appended before) over it; q, result [sum n_q, n_heads, head_dim].
         A query sees its own position and those before, with window > 0 only
         the last `window` of them."""
-        seqs, n_q = self._ints(seqs, n_q)
-        shape = (int(n_q.sum(dtype=np.int64)), int(n_heads), self.head_dim)
+        seqs, n_q = _ints(seqs, n_q)
+
+        def call(qp, op):
+            check(lib().gh_kv8_attention(self.h, seqs.size, seqs.ctypes.data, n_q.ctypes.data, qp, n_heads, window, op))
+
+        if type(q) is int and type(out) is int:
+            call(q, out)
+            return out
+        count = self._count(n_q, int(n_heads))
         with _OnDevice(self.ctx) as dev:
-            qp = dev(q, shape)
+            qp = dev(q, count)
             if out is not None:
-                check(lib().gh_kv8_attention(self.h, seqs.size, _ptr(seqs), _ptr(n_q), qp, int(n_heads), int(window),
-                                             dev(out, shape)))
+                call(qp, dev(out, count))
                 return out
-            n = int(np.prod(shape, dtype=np.int64))
-            ob = dev.new(4 * n)
-            check(lib().gh_kv8_attention(self.h, seqs.size, _ptr(seqs), _ptr(n_q), qp, int(n_heads), int(window), ob.ptr))
-            return ob.numpy(count=n).reshape(shape)
+            ob = dev.new(4 * max(0, count))
+            call(qp, ob.ptr)
+            return ob.numpy(count=count).reshape(-1, int(n_heads), self.head_dim)
 
     def close(self) -> None:
         if self.h:
