@@ -75,28 +75,26 @@ struct Item {
     __device__ __forceinline__ int row_of(int j) const { return row + 16 * (j / 4) + (V ? j % 4 : 0); }
 };
 
-// The item's values of the rows below r1: those below r0 from the f32 rows
-// kept of the block, the others from src (row 0 of the block, `ld` floats a
-// row); 0 behind r1.  Rows out of reach are replaced by the last one for the
-// load, so that no load waits for a branch.
+// The item's values of rows [lo, hi) from src (row 0, `ld` floats a row: a
+// block is below 2^31 bytes); the others as they are.  A row out of reach is
+// replaced by one within for the load, so that no load waits for a branch.
 template <int HD, bool V>
-__device__ __forceinline__ void load_item(const Item<HD, V>& it, const float* tail, const float* src, size_t ld, int r0, int r1,
-                                          float (&x)[16]) {
-    auto at = [&](int j) {
-        const int r = min(it.row_of(j), r1 - 1);
-        return r < r0 ? tail + r * HD + it.col : src + (ptrdiff_t)r * (ptrdiff_t)ld + it.col;
-    };
+__device__ __forceinline__ void load_item(const Item<HD, V>& it, const float* src, uint32_t ld, int lo, int hi, float (&x)[16]) {
+    const char* base = (const char*)(src + (ptrdiff_t)lo * (ptrdiff_t)ld);
+    auto at = [&](int j) { return base + 4 * ((uint32_t)(min(max(it.row_of(j), lo), hi - 1) - lo) * ld + it.col); };
+    auto in = [&](int j) { return it.row_of(j) >= lo && it.row_of(j) < hi; };
     if (V) {
+        float v[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = __builtin_nontemporal_load(at(j));
+        for (int j = 0; j < 16; ++j) v[j] = __builtin_nontemporal_load((const float*)at(j));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = it.row_of(j) < r1 ? x[j] : 0.0f;
+        for (int j = 0; j < 16; ++j) x[j] = in(j) ? v[j] : x[j];
     } else {
         f32x4 v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = __builtin_nontemporal_load((const f32x4*)at(4 * j));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = it.row_of(j) < r1 ? v[j / 4][j % 4] : 0.0f;
+        for (int j = 0; j < 16; ++j) x[j] = in(j) ? v[j / 4][j % 4] : x[j];
     }
 }
 
@@ -108,25 +106,46 @@ __device__ __forceinline__ void store_item(const Item<HD, V>& it, float* dst, si
     for (int j = 0; j < 16; j += V ? 1 : 4) {
         const int r = it.row_of(j);
         if (r < lo || r >= hi) continue;
-        if (V) *at(j) = x[j];
-        else *(f32x4*)at(j) = f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]};
+        if (V) __builtin_nontemporal_store(x[j], at(j));
+        else __builtin_nontemporal_store(f32x4{x[j], x[j + 1], x[j + 2], x[j + 3]}, (f32x4*)at(j));
     }
+}
+
+// The 16 codes as bytes.  x * inv + 1.5 2^23 has the code in its low byte, and
+// the only error before its rounding is inv's, below 127 2^-24: unless a
+// quotient lies within 2^-16 of the middle between two codes (a wave in
+// thirty), that is the answer.
+__device__ __forceinline__ i32x4 codes_of(const float (&x)[16], float s) {
+    constexpr float MAGIC = 0x1.8p23f;
+    const float inv = 1.0f / s;
+    uint32_t v[16];
+    float off = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float t = fmaf(x[j], inv, MAGIC);
+        off = fmaxf(off, fabsf(fmaf(x[j], inv, MAGIC - t)));
+        v[j] = __float_as_uint(t);
+    }
+    if (__any(off > 0.5f - 0x1p-16f)) {
+#pragma unroll 1
+        for (int j = 0; j < 16; ++j) v[j] = (uint32_t)code_of(x[j], s, inv);
+    }
+    i32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = __builtin_amdgcn_perm(v[4 * j + 1], v[4 * j], 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(v[4 * j + 3], v[4 * j + 2], 0x04000c0cu);
+        w[j] = (int)(lo | hi);
+    }
+    return w;
 }
 
 template <int HD, bool V>
 __device__ __forceinline__ void store_codes(const Item<HD, V>& it, int8_t* block, float s, const float (&x)[16]) {
-    const float inv = 1.0f / s;
-    union {
-        int8_t b[16];
-        int i[4];
-        i32x4 w;
-    } u;
+    const i32x4 w = codes_of(x, s);
+    if (V) *(i32x4*)(block + Item<HD, V>::place(it.row, it.col)) = w;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) u.b[j] = (int8_t)code_of(x[j], s, inv);
-    int8_t* at = block + Item<HD, V>::place(it.row, it.col);
-    if (V) *(i32x4*)at = u.w;
-#pragma unroll
-    for (int j = 0; !V && j < 4; ++j) *(int*)(block + Item<HD, V>::place(it.row_of(4 * j), it.col)) = u.i[j];
+    for (int j = 0; !V && j < 4; ++j) *(int*)(block + Item<HD, V>::place(it.row_of(4 * j), it.col)) = w[j];
 }
 
 // f32 values of the codes: one product each, rounded once
@@ -137,10 +156,10 @@ __device__ __forceinline__ void read_item(const Item<HD, V>& it, const int8_t* b
         int i[4];
         i32x4 w;
     } u;
-    if (V) u.w = __builtin_nontemporal_load((const i32x4*)(block + Item<HD, V>::place(it.row, it.col)));
+    if (V) u.w = *(const i32x4*)(block + Item<HD, V>::place(it.row, it.col));
 #pragma unroll
     for (int j = 0; !V && j < 4; ++j)
-        u.i[j] = __builtin_nontemporal_load((const int*)(block + Item<HD, V>::place(it.row_of(4 * j), it.col)));
+        u.i[j] = *(const int*)(block + Item<HD, V>::place(it.row_of(4 * j), it.col));
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = (float)u.b[j] * s;
 }
@@ -184,9 +203,11 @@ __device__ __forceinline__ void append_block(int8_t* block, float* scale, float*
         if (same) return;
     }
     const Item<HD, V> it(tid);
-    float x[16];
-    load_item<HD, V>(it, tail, src, ld, r0, r1, x);
-    if (r0 == 0) {
+    float x[16] = {};
+    load_item<HD, V>(it, src, ld, r0, r1, x);
+    if (r0 > 0) {
+        load_item<HD, V>(it, tail, HD, 0, r0, x);
+    } else {
         s = scale_of(block_max_u32<N>(amax(x), slot));
         if (tid == 0) *scale = s;
         if (keep) store_item<HD, V>(it, tail, HD, 0, r1, x);
@@ -233,9 +254,9 @@ __global__ __launch_bounds__(4 * HD, 8) void k_kv8_append(Kv8Dev c, Kv8Batch b, 
 template <int HD, bool V>
 __device__ __forceinline__ void truncate_block(int8_t* block, float* scale, float* tail, int r1, bool same, uint32_t* slot) {
     const Item<HD, V> it(threadIdx.x);
-    float x[16];
+    float x[16] = {};
     if (same) {
-        load_item<HD, V>(it, tail, tail, 0, r1, r1, x);
+        load_item<HD, V>(it, tail, HD, 0, r1, x);
         const float s = scale_of(block_max_u32<Item<HD, V>::N>(amax(x), slot));
         if (threadIdx.x == 0) *scale = s;
         store_codes<HD, V>(it, block, s, x);
