@@ -17,19 +17,29 @@ constexpr int SMP_MAX_VOCAB = 1 << 24;
 inline int smp_bits(int n) {
     int b = 0;
     while ((int64_t(1) << b) < n) ++b;
-    return std::min(52, 62 - b);
+    return std::min(51, 62 - b);
 }
 
 // Steps between a row's largest and smallest logit, elements that the exact
 // search sorts, and workgroups a row at most.
 constexpr int SMP_BINS = 2048, SMP_LIST = 4096, SMP_CHUNKS = 64;
 
+// What the bins alone say of a row's searches.
+struct SmpCuts {
+    unsigned long long total;   // mass of all
+    unsigned long long upto_m;  // min_p: mass of the bins that it cannot reach behind
+    int lo[4], hi[4];           // bins whose elements decide: top_k, top_p, min_p, the draw (lo > hi: none)
+    int k, p, m;                // which of the rules cut anything off
+};
+
 // Device scratch of a row that several workgroups read.
 struct SmpRow {
-    unsigned long long mass[SMP_BINS], list[SMP_LIST], first[SMP_CHUNKS];
-    unsigned count[SMP_BINS];
+    unsigned long long mass[SMP_BINS], run_mass[SMP_BINS], list[SMP_LIST], first[SMP_CHUNKS];
+    unsigned count[SMP_BINS], run_count[SMP_BINS];
     float low[SMP_CHUNKS];
-    unsigned nan[SMP_CHUNKS], n_list, pad[15];
+    unsigned nan[SMP_CHUNKS];
+    SmpCuts cuts;
+    unsigned n_list, pad[5];
 };
 
 // Workgroups a row; 0: one, which runs every step (no scratch).

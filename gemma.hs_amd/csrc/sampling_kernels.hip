@@ -22,9 +22,6 @@ namespace gh {
 
 namespace {
 
-constexpr int NT = 1024;
-constexpr int NW = NT / 64;
-
 typedef unsigned long long u64;
 
 // Ascending in rank order: value descending, then index ascending.
@@ -37,16 +34,39 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 __device__ __forceinline__ u64 rank_key(float v, int i) { return ((u64)value_key(v) << 32) | (unsigned)i; }
 
-// A row's weights exp((l - max) / T), as integers of smp_bits fractional bits:
+// A row's weights exp((l - max) / T), as integers of `bits` fractional bits:
 // their sums do not depend on the order, and are exact to 2^-bits a weight.
 // In 64 bits because a draw compares sums over the whole vocabulary.
+// 2^y = 2^k 2^f with |f| <= 1/2 and the series of exp(f ln 2) up to f^12,
+// whose first term left out is below 2^-52.
 struct Weights {
     float top;
-    double inv_t, one;
-    __device__ __forceinline__ double real(float l) const {
-        return l == top ? 1.0 : exp(((double)l - (double)top) * inv_t);
+    double log2e_t;  // log2(e) / T
+    int bits;        // at most 51
+    __device__ __forceinline__ double scaled(float l, int e) const {
+        if (l == top) return ldexp(1.0, e);  // an infinite one among them
+        const double y = fmax(((double)l - (double)top) * log2e_t, -1000.0);
+        const double k = rint(y), f = (y - k) * 0.693147180559945309417;
+        double p = 1.0 / 479001600;
+        p = fma(p, f, 1.0 / 39916800);
+        p = fma(p, f, 1.0 / 3628800);
+        p = fma(p, f, 1.0 / 362880);
+        p = fma(p, f, 1.0 / 40320);
+        p = fma(p, f, 1.0 / 5040);
+        p = fma(p, f, 1.0 / 720);
+        p = fma(p, f, 1.0 / 120);
+        p = fma(p, f, 1.0 / 24);
+        p = fma(p, f, 1.0 / 6);
+        p = fma(p, f, 0.5);
+        p = fma(p, f, 1.0);
+        p = fma(p, f, 1.0);
+        return ldexp(p, (int)k + e);
     }
-    __device__ __forceinline__ u64 fixed(float l) const { return (u64)__double2ull_rn(real(l) * one); }
+    __device__ __forceinline__ double real(float l) const { return scaled(l, 0); }
+    // rounded by an addition: between 2^52 and 2^53 a double's low bits are the integer
+    __device__ __forceinline__ u64 fixed(float l) const {
+        return (u64)(__double_as_longlong(scaled(l, bits) + 0x1p52) - __double_as_longlong(0x1p52));
+    }
 };
 
 // What the bins are: equal steps of top - l up to `reach`, behind which every
@@ -68,41 +88,36 @@ __device__ __forceinline__ u64 shfl_up64(u64 v, int o) {
     return ((u64)hi << 32) | lo;
 }
 
-struct Range {
-    int lo, hi;
-    __device__ __forceinline__ bool has(int b) const { return b >= lo && b <= hi; }
-};
-
-struct Shared {
-    u64 mass[SMP_BINS];       // per bin, then running
-    unsigned count[SMP_BINS];
-    u64 list[SMP_LIST];
-    u64 red[NW];
-    unsigned red32[NW];
-    u64 key, base_mass;  // slow_row
-    unsigned base_count;
-    unsigned n_list;
-    int at;
-    u64 found;
+// LDS of a workgroup's reductions, of its bins, and of the list.
+struct Small {
+    u64 red[16];
+    unsigned red32[16];
+    float redf[16];
     int bin[8];
     u64 before[8], upto[8];
+    unsigned n_list;
+};
+struct BinSums {
+    u64 mass[SMP_BINS];  // per bin, then running
+    unsigned count[SMP_BINS];
 };
 
-template <class Op>
-__device__ u64 block_reduce(u64 v, Shared& sh, Op op) {
+template <int NT, class Op>
+__device__ __forceinline__ u64 block_reduce(u64 v, Small& sh, Op op) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = op(v, shfl_xor64(v, o));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = sh.red[threadIdx.x & (NW - 1)];
+    v = sh.red[0];
 #pragma unroll
-    for (int o = NW / 2; o > 0; o >>= 1) v = op(v, shfl_xor64(v, o));
+    for (int i = 1; i < NT / 64; ++i) v = op(v, sh.red[i]);
     return v;
 }
 
-// inclusive running sums over the threads; *total the last
-__device__ __forceinline__ void block_scan(u64& m, unsigned& c, Shared& sh) {
+// inclusive running sums over the threads
+template <int NT>
+__device__ __forceinline__ void block_scan(u64& m, unsigned& c, Small& sh) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -113,11 +128,9 @@ __device__ __forceinline__ void block_scan(u64& m, unsigned& c, Shared& sh) {
     __syncthreads();
     if (lane == 63) sh.red[w] = m, sh.red32[w] = c;
     __syncthreads();
-    u64 pm = 0;
-    unsigned pc = 0;
-    for (int i = 0; i < w; ++i) pm += sh.red[i], pc += sh.red32[i];
-    m += pm;
-    c += pc;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i)
+        if (i < w) m += sh.red[i], c += sh.red32[i];
 }
 
 // ------------------------------------------------------------------
@@ -125,81 +138,90 @@ __device__ __forceinline__ void block_scan(u64& m, unsigned& c, Shared& sh) {
 // ------------------------------------------------------------------
 struct Stat {
     u64 first;  // rank key of the first in rank order; ~0: nothing above -inf
-    float low;  // smallest value above -inf
+    float low;  // smallest value above -inf; +inf if there is none
     bool nan;
 };
 
 // f(index, logit) of the elements [i0, i1), several loads in flight a thread
-template <class F>
+template <int NT, class F>
 __device__ __forceinline__ void each_logit(const float* l, int i0, int i1, F&& f) {
-    constexpr int U = 8;
-    int i = i0 + threadIdx.x;
-    for (; i + (U - 1) * NT < i1; i += U * NT) {
+    constexpr int U = 4;
+    for (int i = i0 + threadIdx.x; i < i1; i += U * NT) {
         float v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = l[i + j * NT];
+        for (int j = 0; j < U; ++j) v[j] = l[min(i + j * NT, i1 - 1)];
 #pragma unroll
-        for (int j = 0; j < U; ++j) f(i + j * NT, v[j]);
+        for (int j = 0; j < U; ++j)
+            if (i + j * NT < i1) f(i + j * NT, v[j]);
     }
-    for (; i < i1; i += NT) f(i, l[i]);
 }
 
-__device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Shared& sh) {
-    u64 first = ~0ull;
-    float low = INFINITY;
-    unsigned nan = 0;
-    each_logit(l, i0, i1, [&](int i, float v) {
+template <int NT>
+__device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small& sh) {
+    float best = -INFINITY, low = INFINITY;
+    int at = -1;
+    bool nan = false;
+    each_logit<NT>(l, i0, i1, [&](int i, float v) {
         nan |= v != v;
-        if (v > -INFINITY) {
-            first = min(first, rank_key(v, i));
-            low = fminf(low, v);
-        }
+        if (v > best) best = v, at = i;  // a thread's indexes ascend: the first of equal ones stays
+        low = fminf(low, v > -INFINITY ? v : INFINITY);
     });
-    first = block_reduce(first, sh, [](u64 a, u64 b) { return a < b ? a : b; });
-    // smallest value = largest value key; the NaN flag in the bit above it
-    const u64 rest = block_reduce(((u64)nan << 32) | (low < INFINITY ? value_key(low) : 0u), sh, [](u64 a, u64 b) {
-        return ((a | b) & (1ull << 32)) | max((unsigned)a, (unsigned)b);
-    });
-    return {first, key_value((unsigned)rest), (rest >> 32) != 0};
+    u64 first = at >= 0 ? rank_key(best, at) : ~0ull;
+    unsigned bad = __any(nan);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        first = min(first, shfl_xor64(first, o));
+        low = fminf(low, __shfl_xor(low, o, 64));
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        sh.red[threadIdx.x >> 6] = first;
+        sh.redf[threadIdx.x >> 6] = low;
+        sh.red32[threadIdx.x >> 6] = bad;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+        first = min(first, sh.red[i]);
+        low = fminf(low, sh.redf[i]);
+        bad |= sh.red32[i];
+    }
+    return {first, low, bad != 0};
 }
 
-// One step behind the stats: true if the row's token is known (written).
-__device__ __forceinline__ bool settled(const Stat& s, const gh_sampling& rule, int32_t* token) {
-    const bool bad = s.nan || s.first == ~0ull;
-    if (!bad && rule.temperature > 0.0f) return false;
-    if (threadIdx.x == 0) *token = bad ? -1 : (int)(unsigned)s.first;
-    return true;
+// the row is drawn from: no NaN, something above -inf, and not greedy
+__device__ __forceinline__ bool drawn(const Stat& s, const gh_sampling& rule) {
+    return !s.nan && s.first != ~0ull && rule.temperature > 0.0f;
+}
+__device__ __forceinline__ int token_of_undrawn(const Stat& s) { return s.nan || s.first == ~0ull ? -1 : (int)(unsigned)s.first; }
+
+__device__ __forceinline__ Weights weights_of(const Stat& s, const gh_sampling& rule, int bits) {
+    return {key_value((unsigned)(s.first >> 32)), 1.44269504088896340736 / (double)rule.temperature, bits};
 }
 
-__device__ __forceinline__ Weights weights_of(const Stat& s, const gh_sampling& rule, double one) {
-    return {key_value((unsigned)(s.first >> 32)), 1.0 / (double)rule.temperature, one};
-}
-
-// `dead`: (top - l) / T from which on a weight rounds to zero
-__device__ __forceinline__ Bins bins_of(const Stat& s, const Weights& w, double dead) {
-    const double d = min((double)w.top - (double)s.low, dead / w.inv_t);
-    if (!(d > 0.0)) return {w.top, 0.0f, 0.0f};  // one value (an infinite one among them): one bin
+__device__ __forceinline__ Bins bins_of(const Stat& s, const Weights& w) {
+    // below 2^-(bits + 2) a weight rounds to zero
+    const double dead = (w.bits + 2) / w.log2e_t, span = (double)w.top - (double)s.low, d = span < dead ? span : dead;
+    if (!(d > 0.0)) return {w.top, 0.0f, 0.0f};  // one value: one bin
     return {w.top, (float)fmin((double)SMP_BINS / d, 3e38), (float)fmin(d * 1.000001, 3.4e38)};
 }
 
 // ------------------------------------------------------------------
 // step 2
 // ------------------------------------------------------------------
-__device__ __forceinline__ void clear_bins(Shared& sh) {
-    for (int b = threadIdx.x; b < SMP_BINS; b += NT) sh.mass[b] = 0, sh.count[b] = 0;
-    if (threadIdx.x == 0) sh.n_list = 0;
-    __syncthreads();
-}
-
+template <int NT>
 __device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const Weights& w, const Bins& bins, bool counts,
-                                           Shared& sh) {
-    each_logit(l, i0, i1, [&](int, float v) {
+                                           BinSums& h) {
+    for (int b = threadIdx.x; b < SMP_BINS; b += NT) h.mass[b] = 0, h.count[b] = 0;
+    __syncthreads();
+    each_logit<NT>(l, i0, i1, [&](int, float v) {
         if (!bins.in_reach(v)) return;
         const u64 m = w.fixed(v);
-        if (!m) return;
         const int b = bins.of(v);
-        atomicAdd(&sh.mass[b], m);
-        if (counts) atomicAdd(&sh.count[b], 1u);
+        if (m) {
+            atomicAdd(&h.mass[b], m);
+            if (counts) atomicAdd(&h.count[b], 1u);
+        }
     });
     __syncthreads();
 }
@@ -207,219 +229,308 @@ __device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const
 // ------------------------------------------------------------------
 // step 3: where the searches end, from the bins alone
 // ------------------------------------------------------------------
-struct Cuts {
-    bool k, p, m;        // which of the rules cut anything off
-    u64 total;           // mass of all
-    u64 upto_m;          // min_p: mass of the bins that it cannot reach behind
-    Range at[4];         // bins whose elements decide: top_k, top_p, min_p, the draw
-    __device__ __forceinline__ bool has(int b) const { return at[0].has(b) || at[1].has(b) || at[2].has(b) || at[3].has(b); }
-};
-
 // The bin in which a running sum first satisfies `reached`; slot i of sh.
-template <class P>
-__device__ __forceinline__ void find_bin(int i, Shared& sh, P&& reached) {
+template <int NT, class P>
+__device__ __forceinline__ void find_bin(int i, const BinSums& h, Small& sh, P&& reached) {
     for (int b = threadIdx.x; b < SMP_BINS; b += NT) {
-        const bool here = reached(sh.mass[b], sh.count[b]);
-        const bool there = b > 0 && reached(sh.mass[b - 1], sh.count[b - 1]);
+        const bool here = reached(h.mass[b], h.count[b]);
+        const bool there = b > 0 && reached(h.mass[b - 1], h.count[b - 1]);
         if (here && !there) {
             sh.bin[i] = b;
-            sh.before[i] = b > 0 ? sh.mass[b - 1] : 0;
-            sh.upto[i] = sh.mass[b];
+            sh.before[i] = b > 0 ? h.mass[b - 1] : 0;
+            sh.upto[i] = h.mass[b];
         }
     }
 }
 
-// sh.mass, sh.count: per bin; running afterwards.
-__device__ __forceinline__ Cuts find_cuts(const Weights& w, const Bins& bins, const gh_sampling& rule, Shared& sh) {
-    static_assert(SMP_BINS == 2 * NT, "two bins a thread");
-    const int tid = threadIdx.x;
+// h: per bin; running afterwards.
+template <int NT>
+__device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins, const gh_sampling& rule, BinSums& h, Small& sh) {
+    constexpr int PER = SMP_BINS / NT;
+    const int b0 = threadIdx.x * PER;
     {
-        const u64 m0 = sh.mass[2 * tid], m1 = sh.mass[2 * tid + 1];
-        const unsigned c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1];
-        u64 m = m0 + m1;
-        unsigned c = c0 + c1;
-        block_scan(m, c, sh);
-        sh.mass[2 * tid] = m - m1;
-        sh.mass[2 * tid + 1] = m;
-        sh.count[2 * tid] = c - c1;
-        sh.count[2 * tid + 1] = c;
+        u64 m[PER], sum = 0;
+        unsigned c[PER], csum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            m[j] = h.mass[b0 + j];
+            c[j] = h.count[b0 + j];
+            sum += m[j];
+            csum += c[j];
+        }
+        u64 run = sum;
+        unsigned crun = csum;
+        block_scan<NT>(run, crun, sh);
+        run -= sum;
+        crun -= csum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            run += m[j];
+            crun += c[j];
+            h.mass[b0 + j] = run;
+            h.count[b0 + j] = crun;
+        }
         __syncthreads();
     }
-    Cuts q;
-    q.total = sh.mass[SMP_BINS - 1];
+    SmpCuts q;
+    q.total = h.mass[SMP_BINS - 1];
     // what is behind the last element with a weight cannot be drawn: a top_k
     // that reaches there leaves all the mass
-    const unsigned alive = sh.count[SMP_BINS - 1];
-    q.k = rule.top_k > 0 && (unsigned)rule.top_k < alive;
+    q.k = rule.top_k > 0 && (unsigned)rule.top_k < h.count[SMP_BINS - 1];
     q.p = rule.top_p < 1.0f;
     q.m = rule.min_p > 0.0f;
-    const Range none{1, 0};
-    for (Range& r : q.at) r = none;
+    for (int i = 0; i < 4; ++i) q.lo[i] = 1, q.hi[i] = 0;
     u64 zlo = q.total, zhi = q.total;  // mass that top_k leaves
     if (q.k) {
         const unsigned k = rule.top_k;
-        find_bin(0, sh, [&](u64, unsigned c) { return c >= k; });
+        find_bin<NT>(0, h, sh, [&](u64, unsigned c) { return c >= k; });
         __syncthreads();
-        q.at[0] = {sh.bin[0], sh.bin[0]};
+        q.lo[0] = q.hi[0] = sh.bin[0];
         zlo = sh.before[0];
         zhi = sh.upto[0];
     }
     u64 lo = zlo, hi = zhi;  // mass that all three leave
     if (q.p) {
         const double tlo = (double)rule.top_p * (double)zlo, thi = (double)rule.top_p * (double)zhi;
-        find_bin(1, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= tlo; });
-        find_bin(2, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= thi; });
+        find_bin<NT>(1, h, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= tlo; });
+        find_bin<NT>(2, h, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= thi; });
         __syncthreads();
-        q.at[1] = {sh.bin[1], sh.bin[2]};
+        q.lo[1] = sh.bin[1];
+        q.hi[1] = sh.bin[2];
         lo = min(lo, sh.before[1]);
         hi = min(hi, sh.upto[2]);
     }
     q.upto_m = q.total;
     if (q.m) {
         // the logit at which a weight falls below min_p, a bin to either side for roundings
-        const double d = -log((double)rule.min_p) / w.inv_t * (double)bins.scale;
+        const double d = (double)-log2f(rule.min_p) / w.log2e_t * (double)bins.scale;
         q.m = d < SMP_BINS + 1;  // else every weight reaches it
         if (q.m) {
             const int b = (int)d;
-            q.at[2] = {max(b - 1, 0), min(b + 1, SMP_BINS - 1)};
-            q.upto_m = sh.mass[q.at[2].hi];
-            lo = min(lo, q.at[2].lo > 0 ? sh.mass[q.at[2].lo - 1] : 0);
+            q.lo[2] = max(b - 1, 0);
+            q.hi[2] = min(b + 1, SMP_BINS - 1);
+            q.upto_m = h.mass[q.hi[2]];
+            lo = min(lo, q.lo[2] > 0 ? h.mass[q.lo[2] - 1] : 0);
             hi = min(hi, q.upto_m);
         }
     }
     const double ulo = (double)rule.u * (double)lo, uhi = (double)rule.u * (double)hi;
-    find_bin(3, sh, [&](u64 m, unsigned) { return (double)m > ulo; });
-    find_bin(4, sh, [&](u64 m, unsigned) { return (double)m > uhi; });
+    find_bin<NT>(3, h, sh, [&](u64 m, unsigned) { return (double)m > ulo; });
+    find_bin<NT>(4, h, sh, [&](u64 m, unsigned) { return (double)m > uhi; });
     __syncthreads();
-    q.at[3] = {sh.bin[3], sh.bin[4]};
+    q.lo[3] = sh.bin[3];
+    q.hi[3] = sh.bin[4];
     return q;
 }
 
-__device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, const Cuts& cuts, u64* list,
+template <int NT>
+__device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, const SmpCuts& q, u64* list,
                                              unsigned* n) {
-    each_logit(l, i0, i1, [&](int i, float v) {
-        if (!bins.in_reach(v) || !cuts.has(bins.of(v))) return;
+    each_logit<NT>(l, i0, i1, [&](int i, float v) {
+        if (!bins.in_reach(v)) return;
+        const int b = bins.of(v);
+        bool in = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) in |= b >= q.lo[j] && b <= q.hi[j];
+        if (!in) return;
         const unsigned at = atomicAdd(n, 1u);
         if (at < SMP_LIST) list[at] = rank_key(v, i);
     });
-    __syncthreads();
 }
 
 // ------------------------------------------------------------------
-// step 4
+// step 4, 1024 threads
 // ------------------------------------------------------------------
-// ascending, in LDS; n <= SMP_LIST
-__device__ __forceinline__ void sort_list(Shared& sh, int n) {
+constexpr int PT = 1024;
+constexpr int PER = SMP_LIST / PT;
+
+struct PickShared {
+    u64 list[SMP_LIST];
+    u64 upto[PT];  // running mass of a thread's last element
+    u64 off_mass[SMP_LIST];
+    unsigned off_count[SMP_LIST];
+    u64 found[4];
+    u64 mass_at[4];
+    int at[4];
+};
+
+// ascending, in LDS; n <= SMP_LIST.  Steps between elements of one wave's 64
+// need no barrier: the wave's own order suffices.
+__device__ __forceinline__ void sort_list(u64* list, int n) {
     int size = 64;
     while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += NT) sh.list[i] = ~0ull;
+    for (int i = n + threadIdx.x; i < size; i += PT) list[i] = ~0ull;
     __syncthreads();
+    const int tid = threadIdx.x;
+    if (size <= PT) {  // one element a thread
+        u64 x = tid < size ? list[tid] : ~0ull;
+        for (int k = 2; k <= size; k *= 2) {
+            for (int j = k / 2; j > 0; j /= 2) {
+                u64 y;
+                if (j >= 64) {
+                    __syncthreads();
+                    if (tid < size) list[tid] = x;
+                    __syncthreads();
+                    y = tid < size ? list[tid ^ j] : ~0ull;
+                } else {
+                    y = shfl_xor64(x, j);
+                }
+                const bool up = (tid & k) == 0, lower = (tid & j) == 0;
+                x = (x < y) == (up == lower) ? x : y;
+            }
+        }
+        __syncthreads();
+        if (tid < size) list[tid] = x;
+        __syncthreads();
+        return;
+    }
     for (int k = 2; k <= size; k *= 2) {
         for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = threadIdx.x; t < size / 2; t += NT) {
+            for (int t = tid; t < size / 2; t += PT) {
                 const int a = 2 * t - (t & (j - 1)), b = a + j;  // a has a 0 where b has a 1
-                const u64 x = sh.list[a], y = sh.list[b];
-                if ((x > y) == ((a & k) == 0)) sh.list[a] = y, sh.list[b] = x;
+                const u64 x = list[a], y = list[b];
+                if ((x > y) == ((a & k) == 0)) list[a] = y, list[b] = x;
             }
             __syncthreads();
         }
     }
 }
 
-// The token, from the bins' running sums and the sorted list of the cuts' bins.
-__device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh_sampling& rule, const Cuts& cuts, int n,
-                                    Shared& sh) {
-    constexpr int PER = SMP_LIST / NT;
+// The token, from the bins' running sums (LDS or global) and the sorted list
+// of the cuts' bins.
+__device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh_sampling& rule, const SmpCuts& cuts,
+                                    const u64* mass, const unsigned* count, int n, PickShared& p, Small& sh) {
     const int tid = threadIdx.x;
     u64 upto[PER];       // running mass up to and with the element
     unsigned rank[PER];  // and its rank, from 1
     float val[PER];
+    u64 m[PER];
     {
-        u64 m[PER], s = 0;
+        u64 s = 0;
         int b[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = tid * PER + j;
-            val[j] = i < n ? key_value((unsigned)(sh.list[i] >> 32)) : 0.0f;
+            val[j] = i < n ? key_value((unsigned)(p.list[i] >> 32)) : 0.0f;
             m[j] = i < n ? w.fixed(val[j]) : 0;
-            b[j] = i < n ? bins.of(val[j]) : 0;
+            b[j] = i < n ? bins.of(val[j]) : -1;
             s += m[j];
         }
         u64 at = s;
-        unsigned dummy = 0;
-        block_scan(at, dummy, sh);
+        unsigned none = 0;
+        block_scan<PT>(at, none, sh);
         at -= s;  // of the list in front of this thread
-        // per bin: what its elements' running sums in the list lack
-        u64 om[PER];
-        unsigned oc[PER];
-        bool head[PER];
+        // What the elements' running sums in the list lack, of each bin of it:
+        // written by the bin's first element for those behind it (the bins
+        // are at most as many as the elements; p.off_* by the first's place).
+        int prev = tid * PER > 0 && tid * PER <= n ? bins.of(key_value((unsigned)(p.list[tid * PER - 1] >> 32))) : -1;
+        int head[PER];  // place of the first element of the bin, if it is one of this thread's, else -1
         u64 run = at;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = tid * PER + j;
-            head[j] = i < n && (i == 0 || bins.of(key_value((unsigned)(sh.list[i - 1] >> 32))) != b[j]);
-            om[j] = head[j] ? (b[j] > 0 ? sh.mass[b[j] - 1] : 0) - run : 0;
-            oc[j] = head[j] ? (b[j] > 0 ? sh.count[b[j] - 1] : 0) - i : 0;
+            const bool first = i < n && b[j] != prev;
+            head[j] = first ? i : -1;
+            if (first) {
+                p.off_mass[i] = (b[j] > 0 ? mass[b[j] - 1] : 0) - run;
+                p.off_count[i] = (b[j] > 0 ? count[b[j] - 1] : 0) - i;
+            }
             run += m[j];
+            prev = b[j];
+        }
+        // place of the first element of each element's bin: running maximum of the heads
+        int h = -1;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) h = max(h, head[j]);
+        int inc = h;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(inc, o, 64);
+            if ((tid & 63) >= o) inc = max(inc, y);
         }
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (head[j]) sh.mass[b[j]] = om[j], sh.count[b[j]] = oc[j];
+        if ((tid & 63) == 63) sh.red32[tid >> 6] = (unsigned)(inc + 1);
         __syncthreads();
+        int before = __shfl_up(inc, 1, 64);
+        if ((tid & 63) == 0) before = -1;
+#pragma unroll
+        for (int i = 0; i < PT / 64; ++i)
+            if (i < tid >> 6) before = max(before, (int)sh.red32[i] - 1);
         run = at;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = tid * PER + j;
+            if (head[j] >= 0) before = head[j];
             run += m[j];
-            upto[j] = i < n ? sh.mass[b[j]] + run : 0;
-            rank[j] = i < n ? sh.count[b[j]] + i + 1 : 0;
+            upto[j] = i < n ? p.off_mass[before] + run : 0;
+            rank[j] = i < n ? p.off_count[before] + i + 1 : 0;
         }
     }
-    // f(j) true: the first such element in rank order; sh.at its place, sh.found its running mass
-    auto first = [&](auto&& f) {
-        __syncthreads();
-        if (tid == 0) sh.at = n;
-        __syncthreads();
+    p.upto[tid] = upto[PER - 1];
+    if (tid < 4) p.at[tid] = n;
+    __syncthreads();
+    // `reached`, false and then true along the list: p.at[slot] the place of
+    // the first true, p.found[slot] its running mass
+    auto first = [&](int slot, auto&& reached) {
+        bool before = tid > 0 && tid * PER <= n && reached(-1);
 #pragma unroll
-        for (int j = PER - 1; j >= 0; --j)
-            if (tid * PER + j < n && f(j)) atomicMin(&sh.at, tid * PER + j);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (tid * PER + j == sh.at) sh.found = upto[j];
+        for (int j = 0; j < PER; ++j) {
+            const int i = tid * PER + j;
+            const bool here = i < n && reached(j);
+            if (here && !before) {
+                p.at[slot] = i;
+                p.found[slot] = upto[j];
+                p.mass_at[slot] = m[j];
+            }
+            before = here;
+        }
         __syncthreads();
     };
+    auto of = [&](int j) { return j < 0 ? p.upto[tid - 1] : upto[j]; };
     u64 left = cuts.total;
     if (cuts.k) {
-        first([&](int j) { return rank[j] == (unsigned)rule.top_k; });
-        left = sh.found;
+        // ranks of the elements without a weight may repeat; they are the last
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (tid * PER + j < n && rank[j] == (unsigned)rule.top_k && m[j]) p.found[0] = upto[j];
+        __syncthreads();
+        left = p.found[0];
     }
     u64 kept = left;
     if (cuts.p) {
         const double t = (double)rule.top_p * (double)left;
-        first([&](int j) { return (double)upto[j] >= t; });
-        kept = min(kept, sh.found);
+        first(1, [&](int j) { return (double)of(j) >= t; });
+        kept = min(kept, p.found[1]);
     }
     if (cuts.m) {
+        const double t = (double)rule.min_p;
+        first(2, [&](int j) {
+            return w.real(j < 0 ? key_value((unsigned)(p.list[tid * PER - 1] >> 32)) : val[j]) < t;
+        });
         kept = min(kept, cuts.upto_m);
-        first([&](int j) { return w.real(val[j]) < (double)rule.min_p; });
-        if (sh.at < n) kept = min(kept, sh.found - w.fixed(key_value((unsigned)(sh.list[sh.at] >> 32))));
+        if (p.at[2] < n) kept = min(kept, p.found[2] - p.mass_at[2]);
     }
     const double t = (double)rule.u * (double)kept;
-    first([&](int j) { return (double)upto[j] > t; });
-    return (int)(unsigned)sh.list[sh.at];
+    first(3, [&](int j) { return (double)of(j) > t; });
+    return (int)(unsigned)p.list[p.at[3]];
 }
 
 // ------------------------------------------------------------------
-// rows whose list is too long
+// rows whose list is too long, 1024 threads
 // ------------------------------------------------------------------
+struct SlowShared {
+    u64 mass[256];
+    unsigned count[256];
+    u64 key, base_mass;
+    unsigned base_count;
+};
+
 // The first element in rank order whose running count reaches `k` (k > 0), or
 // whose running mass reaches (strict: passes) `t`: digit by digit of its rank
 // key, from the counts and masses of the 256 values of each digit among the
 // elements that share the digits before.  The mass up to and with it goes to
 // sh.base_mass, its key to sh.key.
-__device__ void find(const float* l, int n, const Weights& w, unsigned k, double t, bool strict, Shared& sh) {
+__device__ void find(const float* l, int n, const Weights& w, unsigned k, double t, bool strict, SlowShared& sh) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) sh.key = sh.base_mass = 0, sh.base_count = 0;
@@ -428,7 +539,7 @@ __device__ void find(const float* l, int n, const Weights& w, unsigned k, double
         if (tid < 256) sh.mass[tid] = 0, sh.count[tid] = 0;
         __syncthreads();
         const u64 prefix = sh.key;
-        each_logit(l, 0, n, [&](int i, float v) {
+        each_logit<PT>(l, 0, n, [&](int i, float v) {
             const u64 key = rank_key(v, i);
             if (shift < 56 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
             const int d = (int)(key >> shift) & 255;
@@ -458,16 +569,16 @@ __device__ void find(const float* l, int n, const Weights& w, unsigned k, double
     __syncthreads();
 }
 
-__device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, const gh_sampling& rule, Shared& sh) {
+__device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, const gh_sampling& rule, SlowShared& sh, Small& red) {
     u64 total = 0, at_least = 0;
-    each_logit(l, 0, n, [&](int, float v) {
+    each_logit<PT>(l, 0, n, [&](int, float v) {
         const u64 m = w.fixed(v);
         total += m;
         if (w.real(v) >= (double)rule.min_p) at_least += m;
     });
     auto plus = [](u64 a, u64 b) { return a + b; };
-    total = block_reduce(total, sh, plus);
-    at_least = block_reduce(at_least, sh, plus);
+    total = block_reduce<PT>(total, red, plus);
+    at_least = block_reduce<PT>(at_least, red, plus);
     if (rule.top_k > 0 && rule.top_k < n) {
         find(l, n, w, rule.top_k, 0.0, false, sh);
         total = sh.base_mass;
@@ -485,40 +596,49 @@ __device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, co
 // kernels
 // ------------------------------------------------------------------
 // one workgroup a row
-__global__ __launch_bounds__(NT) void k_smp_row(const float* logits, int n, double one, double dead, SmpRules rules,
-                                                int32_t* tokens) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int bits, SmpRules rules, int32_t* tokens) {
+    __shared__ Small sh;
+    __shared__ BinSums h;
+    __shared__ union {
+        PickShared p;
+        SlowShared slow;
+    } u;
     const gh_sampling rule = rules.r[blockIdx.x];
     const float* l = logits + (size_t)blockIdx.x * n;
-    int32_t* token = tokens + blockIdx.x;
-    const Stat s = range_stat(l, 0, n, sh);
-    if (settled(s, rule, token)) return;
-    const Weights w = weights_of(s, rule, one);
-    const Bins bins = bins_of(s, w, dead);
-    clear_bins(sh);
-    range_hist(l, 0, n, w, bins, rule.top_k > 0, sh);
-    const Cuts cuts = find_cuts(w, bins, rule, sh);
-    range_gather(l, 0, n, bins, cuts, sh.list, &sh.n_list);
+    const Stat s = range_stat<PT>(l, 0, n, sh);
     int t;
-    const unsigned listed = sh.n_list;
-    if (listed <= SMP_LIST) {
-        sort_list(sh, listed);
-        t = pick(w, bins, rule, cuts, listed, sh);
+    if (!drawn(s, rule)) {
+        t = token_of_undrawn(s);
     } else {
-        t = slow_row(l, n, w, rule, sh);
+        const Weights w = weights_of(s, rule, bits);
+        const Bins bins = bins_of(s, w);
+        if (threadIdx.x == 0) sh.n_list = 0;
+        range_hist<PT>(l, 0, n, w, bins, rule.top_k > 0, h);
+        const SmpCuts cuts = find_cuts<PT>(w, bins, rule, h, sh);
+        range_gather<PT>(l, 0, n, bins, cuts, u.p.list, &sh.n_list);
+        __syncthreads();
+        const unsigned listed = sh.n_list;
+        if (listed <= SMP_LIST) {
+            sort_list(u.p.list, listed);
+            t = pick(w, bins, rule, cuts, h.mass, h.count, listed, u.p, sh);
+        } else {
+            t = slow_row(l, n, w, rule, u.slow, sh);
+        }
     }
-    if (threadIdx.x == 0) *token = t;
+    if (threadIdx.x == 0) tokens[blockIdx.x] = t;
 }
 
 __device__ __forceinline__ int chunk_begin(int n, int c, int chunks) { return (int)((int64_t)n * c / chunks); }
 
+constexpr int CT = 512;  // threads of a workgroup that reads a chunk of a row
+
 // a row's chunks: stats; the row's bins cleared
-__global__ __launch_bounds__(NT) void k_smp_stat(const float* logits, int n, SmpRow* rows) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, SmpRow* rows) {
+    __shared__ Small sh;
     const int c = blockIdx.x, chunks = gridDim.x;
     SmpRow& r = rows[blockIdx.y];
-    for (int b = c * NT + threadIdx.x; b < SMP_BINS; b += chunks * NT) r.mass[b] = 0, r.count[b] = 0;
-    const Stat s = range_stat(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), sh);
+    for (int b = c * CT + threadIdx.x; b < SMP_BINS; b += chunks * CT) r.mass[b] = 0, r.count[b] = 0;
+    const Stat s = range_stat<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), sh);
     if (threadIdx.x == 0) {
         r.first[c] = s.first;
         r.low[c] = s.low;
@@ -533,95 +653,94 @@ __device__ __forceinline__ Stat row_stat(const SmpRow& r, int chunks) {
     const bool in = lane < chunks;
     u64 first = in ? r.first[lane] : ~0ull;
     float low = in ? r.low[lane] : INFINITY;
-    unsigned nan = in ? r.nan[lane] : 0;
+    const bool nan = __any(in && r.nan[lane]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         first = min(first, shfl_xor64(first, o));
         low = fminf(low, __shfl_xor(low, o, 64));
-        nan |= __shfl_xor(nan, o, 64);
     }
-    return {first, low, nan != 0};
+    return {first, low, nan};
 }
 
-__global__ __launch_bounds__(NT) void k_smp_hist(const float* logits, int n, double one, double dead, SmpRules rules,
-                                                 SmpRow* rows) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int bits, SmpRules rules, SmpRow* rows) {
+    __shared__ BinSums h;
     const int c = blockIdx.x, chunks = gridDim.x;
     const gh_sampling rule = rules.r[blockIdx.y];
     SmpRow& r = rows[blockIdx.y];
     const Stat s = row_stat(r, chunks);
-    if (s.nan || s.first == ~0ull || rule.temperature == 0.0f) return;
-    const Weights w = weights_of(s, rule, one);
-    clear_bins(sh);
-    range_hist(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), w,
-               bins_of(s, w, dead), rule.top_k > 0, sh);
-    for (int b = threadIdx.x; b < SMP_BINS; b += NT) {
-        if (sh.mass[b]) atomicAdd(&r.mass[b], sh.mass[b]);
-        if (sh.count[b]) atomicAdd(&r.count[b], sh.count[b]);
+    if (!drawn(s, rule)) return;
+    const Weights w = weights_of(s, rule, bits);
+    range_hist<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), w, bins_of(s, w),
+                   rule.top_k > 0, h);
+    for (int b = threadIdx.x; b < SMP_BINS; b += CT) {
+        if (h.mass[b]) atomicAdd(&r.mass[b], h.mass[b]);
+        if (h.count[b]) atomicAdd(&r.count[b], h.count[b]);
     }
 }
 
-__device__ __forceinline__ void load_bins(const SmpRow& r, Shared& sh) {
-    for (int b = threadIdx.x; b < SMP_BINS; b += NT) sh.mass[b] = r.mass[b], sh.count[b] = r.count[b];
+__global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, int bits, SmpRules rules, SmpRow* rows) {
+    __shared__ Small sh;
+    __shared__ BinSums h;
+    const int c = blockIdx.x, chunks = gridDim.x;
+    const gh_sampling rule = rules.r[blockIdx.y];
+    SmpRow& r = rows[blockIdx.y];
+    const Stat s = row_stat(r, chunks);
+    if (!drawn(s, rule)) return;
+    const Weights w = weights_of(s, rule, bits);
+    const Bins bins = bins_of(s, w);
+    for (int b = threadIdx.x; b < SMP_BINS; b += CT) h.mass[b] = r.mass[b], h.count[b] = r.count[b];
     __syncthreads();
+    const SmpCuts cuts = find_cuts<CT>(w, bins, rule, h, sh);
+    if (c == 0) {  // for the last step
+        for (int b = threadIdx.x; b < SMP_BINS; b += CT) r.run_mass[b] = h.mass[b], r.run_count[b] = h.count[b];
+        if (threadIdx.x == 0) r.cuts = cuts;
+    }
+    range_gather<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
+                     r.list, &r.n_list);
 }
 
-__global__ __launch_bounds__(NT) void k_smp_gather(const float* logits, int n, double one, double dead, SmpRules rules,
-                                                   SmpRow* rows) {
-    __shared__ Shared sh;
-    const int c = blockIdx.x, chunks = gridDim.x;
-    const gh_sampling rule = rules.r[blockIdx.y];
-    SmpRow& r = rows[blockIdx.y];
-    const Stat s = row_stat(r, chunks);
-    if (s.nan || s.first == ~0ull || rule.temperature == 0.0f) return;
-    const Weights w = weights_of(s, rule, one);
-    const Bins bins = bins_of(s, w, dead);
-    load_bins(r, sh);
-    const Cuts cuts = find_cuts(w, bins, rule, sh);
-    range_gather(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
-                 r.list, &r.n_list);
-}
-
-__global__ __launch_bounds__(NT) void k_smp_pick(const float* logits, int n, double one, double dead, SmpRules rules,
-                                                 const SmpRow* rows, int chunks, int32_t* tokens) {
-    __shared__ Shared sh;
+__global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int bits, SmpRules rules, const SmpRow* rows,
+                                                 int chunks, int32_t* tokens) {
+    __shared__ Small sh;
+    __shared__ union {
+        PickShared p;
+        SlowShared slow;
+    } u;
     const gh_sampling rule = rules.r[blockIdx.x];
     const SmpRow& r = rows[blockIdx.x];
-    int32_t* token = tokens + blockIdx.x;
     const Stat s = row_stat(r, chunks);
-    if (settled(s, rule, token)) return;
-    const Weights w = weights_of(s, rule, one);
-    const Bins bins = bins_of(s, w, dead);
-    const unsigned listed = r.n_list;
+    const int listed = (int)min(r.n_list, (unsigned)SMP_LIST + 1);
     int t;
-    if (listed <= SMP_LIST) {
-        for (int i = threadIdx.x; i < (int)listed; i += NT) sh.list[i] = r.list[i];
-        load_bins(r, sh);
-        const Cuts cuts = find_cuts(w, bins, rule, sh);
-        sort_list(sh, listed);
-        t = pick(w, bins, rule, cuts, listed, sh);
+    if (!drawn(s, rule)) {
+        t = token_of_undrawn(s);
     } else {
-        t = slow_row(logits + (size_t)blockIdx.x * n, n, w, rule, sh);
+        const Weights w = weights_of(s, rule, bits);
+        if (listed <= SMP_LIST) {
+            for (int i = threadIdx.x; i < listed; i += PT) u.p.list[i] = r.list[i];
+            __syncthreads();
+            sort_list(u.p.list, listed);
+            t = pick(w, bins_of(s, w), rule, r.cuts, r.run_mass, r.run_count, listed, u.p, sh);
+        } else {
+            t = slow_row(logits + (size_t)blockIdx.x * n, n, w, rule, u.slow, sh);
+        }
     }
-    if (threadIdx.x == 0) *token = t;
+    if (threadIdx.x == 0) tokens[blockIdx.x] = t;
 }
 
 }  // namespace
 
 int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRules& rules, SmpRow* scratch, int32_t* tokens,
                        hipStream_t s) {
-    const int bits = smp_bits(vocab);
-    const double one = ldexp(1.0, bits), dead = (bits + 2) * 0.6931471805599453;
-    const int chunks = smp_chunks(n_rows, vocab);
+    const int bits = smp_bits(vocab), chunks = smp_chunks(n_rows, vocab);
     if (chunks == 0) {
-        hipLaunchKernelGGL(k_smp_row, dim3(n_rows), dim3(NT), 0, s, logits, vocab, one, dead, rules, tokens);
+        hipLaunchKernelGGL(k_smp_row, dim3(n_rows), dim3(PT), 0, s, logits, vocab, bits, rules, tokens);
     } else {
         const dim3 grid(chunks, n_rows);
-        hipLaunchKernelGGL(k_smp_stat, grid, dim3(NT), 0, s, logits, vocab, scratch);
-        hipLaunchKernelGGL(k_smp_hist, grid, dim3(NT), 0, s, logits, vocab, one, dead, rules, scratch);
-        hipLaunchKernelGGL(k_smp_gather, grid, dim3(NT), 0, s, logits, vocab, one, dead, rules, scratch);
-        hipLaunchKernelGGL(k_smp_pick, dim3(n_rows), dim3(NT), 0, s, logits, vocab, one, dead, rules, (const SmpRow*)scratch,
-                           chunks, tokens);
+        hipLaunchKernelGGL(k_smp_stat, grid, dim3(CT), 0, s, logits, vocab, scratch);
+        hipLaunchKernelGGL(k_smp_hist, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
+        hipLaunchKernelGGL(k_smp_gather, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
+        hipLaunchKernelGGL(k_smp_pick, dim3(n_rows), dim3(PT), 0, s, logits, vocab, bits, rules, (const SmpRow*)scratch, chunks,
+                           tokens);
     }
     GH_HIP(hipGetLastError());
     return GH_OK;
