@@ -21,8 +21,8 @@ inline int smp_bits(int n) {
 }
 
 // Steps between a row's largest and smallest logit, elements that the exact
-// search sorts, and workgroups a row at most.
-constexpr int SMP_BINS = 2048, SMP_LIST = 4096, SMP_CHUNKS = 64;
+// search sorts, workgroups a row and groups a row at most.
+constexpr int SMP_BINS = 2048, SMP_LIST = 4096, SMP_CHUNKS = 64, SMP_GROUPS = 1024;
 
 // What the bins alone say of a row's searches.
 struct SmpCuts {
@@ -38,8 +38,11 @@ struct SmpRow {
     unsigned count[SMP_BINS], run_count[SMP_BINS];
     float low[SMP_CHUNKS];
     unsigned nan[SMP_CHUNKS];
+    float group_max[SMP_GROUPS];  // largest logit of each group
     SmpCuts cuts;
-    unsigned n_list, pad[5];
+    unsigned n_list;
+    int is_short;  // 0: long; 1: the list has all the mass that counts; 2: mass[0] has the row's
+    unsigned pad[4];
 };
 
 // Workgroups a row; 0: one, which runs every step (no scratch).

@@ -4,16 +4,21 @@
 // first whose running mass reaches top_p of what top_k left, for the first
 // below min_p, and for the first whose running mass passes u times what the
 // three leave.  None needs the row sorted:
-//   1. largest and smallest logit (k_smp_stat),
-//   2. a histogram over SMP_BINS equal steps of the logit between them, with
-//      the number and the mass of each bin's elements (k_smp_hist): sums over
-//      its bins say in which bin, or few bins, each search ends,
-//   3. the elements of those bins, a list (k_smp_gather),
+//   1. largest and smallest logit, and the largest of each of some hundred
+//      groups of the row (k_smp_stat);
+//   2. (k_smp_hist) a row whose rules keep few elements, a short row: top_k
+//      groups' largest are at least the top_k-th element, min_p is a fixed
+//      distance from the largest: the elements that reach the nearer of the
+//      two go straight to a list.  Any other row, a long one: a histogram over
+//      SMP_BINS equal steps of the logit, with the number and the mass of each
+//      bin's elements; running sums over the bins say in which bin, or few
+//      bins, each search ends;
+//   3. a long row's elements of those bins go to the list (k_smp_gather);
 //   4. the list sorted, its running mass on top of the bins' in front of it:
 //      the exact answers (k_smp_pick).
 // A list that does not fit (rows with thousands of equal logits) is searched
 // digit by digit instead (slow_row).  Rows that one workgroup reads quickly
-// run all four steps in one kernel (k_smp_row).
+// run all steps in one kernel (k_smp_row).
 #include <hip/hip_runtime.h>
 
 #include "sampling.h"
@@ -140,19 +145,34 @@ struct Stat {
     u64 first;  // rank key of the first in rank order; ~0: nothing above -inf
     float low;  // smallest value above -inf; +inf if there is none
     bool nan;
+    float own;  // the largest of the elements that this thread read
 };
 
-// f(index, logit) of the elements [i0, i1), several loads in flight a thread
+// f(index, logit) of the elements [i0, i1): 16-byte loads, two in flight a
+// thread, between the first and last 16-byte boundary (l is aligned to 4).
 template <int NT, class F>
 __device__ __forceinline__ void each_logit(const float* l, int i0, int i1, F&& f) {
-    constexpr int U = 4;
-    for (int i = i0 + threadIdx.x; i < i1; i += U * NT) {
-        float v[U];
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    constexpr int U = 2;
+    const int tid = threadIdx.x;
+    const int head = min((int)(-((uintptr_t)(l + i0) >> 2) & 3), i1 - i0), quads = (i1 - i0 - head) / 4;
+    const int tail = i1 - i0 - head - 4 * quads;
+    const f32x4* p = (const f32x4*)(l + i0 + head);
+#pragma unroll 1
+    for (int q = tid; q < quads; q += U * NT) {
+        f32x4 v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = l[min(i + j * NT, i1 - 1)];
+        for (int j = 0; j < U; ++j) v[j] = p[min(q + j * NT, quads - 1)];
 #pragma unroll
         for (int j = 0; j < U; ++j)
-            if (i + j * NT < i1) f(i + j * NT, v[j]);
+            if (q + j * NT < quads) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f(i0 + head + 4 * (q + j * NT) + e, v[j][e]);
+            }
+    }
+    if (tid < head + tail) {
+        const int i = tid < head ? i0 + tid : i1 - tail + tid - head;
+        f(i, l[i]);
     }
 }
 
@@ -163,7 +183,7 @@ __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small
     bool nan = false;
     each_logit<NT>(l, i0, i1, [&](int i, float v) {
         nan |= v != v;
-        if (v > best) best = v, at = i;  // a thread's indexes ascend: the first of equal ones stays
+        if (v > best || (v == best && i < at)) best = v, at = i;
         low = fminf(low, v > -INFINITY ? v : INFINITY);
     });
     u64 first = at >= 0 ? rank_key(best, at) : ~0ull;
@@ -186,7 +206,7 @@ __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small
         low = fminf(low, sh.redf[i]);
         bad |= sh.red32[i];
     }
-    return {first, low, bad != 0};
+    return {first, low, bad != 0, best};
 }
 
 // the row is drawn from: no NaN, something above -inf, and not greedy
@@ -210,10 +230,15 @@ __device__ __forceinline__ Bins bins_of(const Stat& s, const Weights& w) {
 // step 2
 // ------------------------------------------------------------------
 template <int NT>
-__device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const Weights& w, const Bins& bins, bool counts,
-                                           BinSums& h) {
+__device__ __forceinline__ void clear_bins(BinSums& h) {
     for (int b = threadIdx.x; b < SMP_BINS; b += NT) h.mass[b] = 0, h.count[b] = 0;
     __syncthreads();
+}
+
+template <int NT>
+__device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const Weights& w, const Bins& bins, bool counts,
+                                           BinSums& h) {
+    clear_bins<NT>(h);
     each_logit<NT>(l, i0, i1, [&](int, float v) {
         if (!bins.in_reach(v)) return;
         const u64 m = w.fixed(v);
@@ -229,6 +254,35 @@ __device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const
 // ------------------------------------------------------------------
 // step 3: where the searches end, from the bins alone
 // ------------------------------------------------------------------
+// Sums per bin become running sums.
+template <int NT>
+__device__ __forceinline__ void scan_bins(BinSums& h, Small& sh) {
+    constexpr int PER = SMP_BINS / NT;
+    const int b0 = threadIdx.x * PER;
+    u64 m[PER], sum = 0;
+    unsigned c[PER], csum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        m[j] = h.mass[b0 + j];
+        c[j] = h.count[b0 + j];
+        sum += m[j];
+        csum += c[j];
+    }
+    u64 run = sum;
+    unsigned crun = csum;
+    block_scan<NT>(run, crun, sh);
+    run -= sum;
+    crun -= csum;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        run += m[j];
+        crun += c[j];
+        h.mass[b0 + j] = run;
+        h.count[b0 + j] = crun;
+    }
+    __syncthreads();
+}
+
 // The bin in which a running sum first satisfies `reached`; slot i of sh.
 template <int NT, class P>
 __device__ __forceinline__ void find_bin(int i, const BinSums& h, Small& sh, P&& reached) {
@@ -243,35 +297,16 @@ __device__ __forceinline__ void find_bin(int i, const BinSums& h, Small& sh, P&&
     }
 }
 
+// Where in the bins a weight falls below min_p, to be taken with a bin to
+// either side for roundings.
+__device__ __forceinline__ double min_p_bin(const Weights& w, const Bins& bins, const gh_sampling& rule) {
+    return (double)-log2f(rule.min_p) / w.log2e_t * (double)bins.scale;
+}
+
 // h: per bin; running afterwards.
 template <int NT>
 __device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins, const gh_sampling& rule, BinSums& h, Small& sh) {
-    constexpr int PER = SMP_BINS / NT;
-    const int b0 = threadIdx.x * PER;
-    {
-        u64 m[PER], sum = 0;
-        unsigned c[PER], csum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            m[j] = h.mass[b0 + j];
-            c[j] = h.count[b0 + j];
-            sum += m[j];
-            csum += c[j];
-        }
-        u64 run = sum;
-        unsigned crun = csum;
-        block_scan<NT>(run, crun, sh);
-        run -= sum;
-        crun -= csum;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            run += m[j];
-            crun += c[j];
-            h.mass[b0 + j] = run;
-            h.count[b0 + j] = crun;
-        }
-        __syncthreads();
-    }
+    scan_bins<NT>(h, sh);
     SmpCuts q;
     q.total = h.mass[SMP_BINS - 1];
     // what is behind the last element with a weight cannot be drawn: a top_k
@@ -302,8 +337,7 @@ __device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins,
     }
     q.upto_m = q.total;
     if (q.m) {
-        // the logit at which a weight falls below min_p, a bin to either side for roundings
-        const double d = (double)-log2f(rule.min_p) / w.log2e_t * (double)bins.scale;
+        const double d = min_p_bin(w, bins, rule);
         q.m = d < SMP_BINS + 1;  // else every weight reaches it
         if (q.m) {
             const int b = (int)d;
@@ -323,19 +357,76 @@ __device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins,
     return q;
 }
 
-template <int NT>
-__device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, const SmpCuts& q, u64* list,
-                                             unsigned* n) {
+// To the list: the elements of the bins [lo, hi] that `in` takes.
+template <int NT, class In>
+__device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, int lo, int hi, u64* list,
+                                             unsigned* n, In&& in) {
     each_logit<NT>(l, i0, i1, [&](int i, float v) {
         if (!bins.in_reach(v)) return;
         const int b = bins.of(v);
-        bool in = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) in |= b >= q.lo[j] && b <= q.hi[j];
-        if (!in) return;
+        if (b < lo || b > hi || !in(b)) return;
         const unsigned at = atomicAdd(n, 1u);
         if (at < SMP_LIST) list[at] = rank_key(v, i);
     });
+}
+template <int NT>
+__device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, const SmpCuts& q, u64* list,
+                                             unsigned* n) {
+    int lo = SMP_BINS, hi = -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (q.lo[j] <= q.hi[j]) lo = min(lo, q.lo[j]), hi = max(hi, q.hi[j]);
+    range_gather<NT>(l, i0, i1, bins, lo, hi, list, n, [&](int b) {
+        bool in = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) in |= b >= q.lo[j] && b <= q.hi[j];
+        return in;
+    });
+}
+
+// A short row: the last bin of the elements that its list needs (-1: a long
+// row), and whether top_p needs the mass of all (the list has what top_k
+// leaves).  top_k: the bin in which the groups' largest come to top_k; where
+// top_p asks for the mass that top_k leaves, min_p must not cut the list.  A
+// row is short if at most half of its groups reach that far: about as many
+// elements do.
+struct Short {
+    int last;
+    bool all;
+};
+template <int NT>
+__device__ __forceinline__ Short short_row(const float* group_max, int groups, const Weights& w, const Bins& bins,
+                                           const gh_sampling& rule, BinSums& h, Small& sh) {
+    const bool k = rule.top_k > 0 && rule.top_k <= groups / 2;
+    const bool m = rule.min_p > 0.0f && (rule.top_p >= 1.0f || rule.top_k == 0);
+    if (!k && !m) return {-1, false};
+    clear_bins<NT>(h);
+    for (int i = threadIdx.x; i < groups; i += NT) {
+        const float v = group_max[i];
+        if (v > -INFINITY && bins.in_reach(v)) atomicAdd(&h.count[bins.of(v)], 1u);
+    }
+    __syncthreads();
+    scan_bins<NT>(h, sh);
+    int last = SMP_BINS - 1;
+    if (k && h.count[SMP_BINS - 1] >= (unsigned)rule.top_k) {
+        find_bin<NT>(0, h, sh, [&](u64, unsigned c) { return c >= (unsigned)rule.top_k; });
+        __syncthreads();
+        last = sh.bin[0];
+    }
+    if (m) last = min(last, (int)fmin(min_p_bin(w, bins, rule) + 1.0, (double)(SMP_BINS - 1)));
+    const bool is_short = h.count[last] <= (unsigned)groups / 2;
+    __syncthreads();
+    return {is_short ? last : -1, rule.top_p < 1.0f && rule.top_k == 0};
+}
+
+// Mass of the elements [i0, i1); in every thread.
+template <int NT>
+__device__ __forceinline__ u64 range_mass(const float* l, int i0, int i1, const Weights& w, const Bins& bins, Small& sh) {
+    u64 sum = 0;
+    each_logit<NT>(l, i0, i1, [&](int, float v) {
+        if (bins.in_reach(v)) sum += w.fixed(v);
+    });
+    return block_reduce<NT>(sum, sh, [](u64 a, u64 b) { return a + b; });
 }
 
 // ------------------------------------------------------------------
@@ -396,10 +487,12 @@ __device__ __forceinline__ void sort_list(u64* list, int n) {
     }
 }
 
-// The token, from the bins' running sums (LDS or global) and the sorted list
-// of the cuts' bins.
+// The token, from the sorted list and the running sums of the bins in front
+// of its elements (LDS or global; none for a list that begins with the row's
+// first element and leaves none out).
 __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh_sampling& rule, const SmpCuts& cuts,
                                     const u64* mass, const unsigned* count, int n, PickShared& p, Small& sh) {
+    auto bin_of = [&](float v) { return mass ? bins.of(v) : 0; };
     const int tid = threadIdx.x;
     u64 upto[PER];       // running mass up to and with the element
     unsigned rank[PER];  // and its rank, from 1
@@ -413,7 +506,7 @@ __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh
             const int i = tid * PER + j;
             val[j] = i < n ? key_value((unsigned)(p.list[i] >> 32)) : 0.0f;
             m[j] = i < n ? w.fixed(val[j]) : 0;
-            b[j] = i < n ? bins.of(val[j]) : -1;
+            b[j] = i < n ? bin_of(val[j]) : -1;
             s += m[j];
         }
         u64 at = s;
@@ -423,7 +516,7 @@ __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh
         // What the elements' running sums in the list lack, of each bin of it:
         // written by the bin's first element for those behind it (the bins
         // are at most as many as the elements; p.off_* by the first's place).
-        int prev = tid * PER > 0 && tid * PER <= n ? bins.of(key_value((unsigned)(p.list[tid * PER - 1] >> 32))) : -1;
+        int prev = tid * PER > 0 && tid * PER <= n ? bin_of(key_value((unsigned)(p.list[tid * PER - 1] >> 32))) : -1;
         int head[PER];  // place of the first element of the bin, if it is one of this thread's, else -1
         u64 run = at;
 #pragma unroll
@@ -468,6 +561,9 @@ __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh
     }
     p.upto[tid] = upto[PER - 1];
     if (tid < 4) p.at[tid] = n;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (tid * PER + j == n - 1) p.found[0] = p.found[1] = upto[j];  // a search that ends behind the list: all of it
     __syncthreads();
     // `reached`, false and then true along the list: p.at[slot] the place of
     // the first true, p.found[slot] its running mass
@@ -487,16 +583,17 @@ __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh
         __syncthreads();
     };
     auto of = [&](int j) { return j < 0 ? p.upto[tid - 1] : upto[j]; };
-    u64 left = cuts.total;
+    u64 left = cuts.total ? cuts.total : p.found[0], most = mass ? cuts.upto_m : p.found[0];
+    u64 kept = min(left, p.found[0] | (mass ? ~0ull : 0));
     if (cuts.k) {
+        __syncthreads();
         // ranks of the elements without a weight may repeat; they are the last
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             if (tid * PER + j < n && rank[j] == (unsigned)rule.top_k && m[j]) p.found[0] = upto[j];
         __syncthreads();
-        left = p.found[0];
+        left = kept = p.found[0];
     }
-    u64 kept = left;
     if (cuts.p) {
         const double t = (double)rule.top_p * (double)left;
         first(1, [&](int j) { return (double)of(j) >= t; });
@@ -507,12 +604,68 @@ __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh
         first(2, [&](int j) {
             return w.real(j < 0 ? key_value((unsigned)(p.list[tid * PER - 1] >> 32)) : val[j]) < t;
         });
-        kept = min(kept, cuts.upto_m);
+        kept = min(kept, most);
         if (p.at[2] < n) kept = min(kept, p.found[2] - p.mass_at[2]);
     }
     const double t = (double)rule.u * (double)kept;
     first(3, [&](int j) { return (double)of(j) > t; });
     return (int)(unsigned)p.list[p.at[3]];
+}
+
+// The same for a list of at most 64 by one wave alone: no barriers, and little
+// code, which the first passes of a kernel have to fetch.
+__device__ __forceinline__ int pick_wave(const Weights& w, const Bins& bins, const gh_sampling& rule, const SmpCuts& cuts,
+                                         const u64* mass, const unsigned* count, u64 key, int n) {
+    const int lane = threadIdx.x & 63;
+    if (lane >= n) key = ~0ull;
+#pragma unroll 1
+    for (int k = 2; k <= 64; k *= 2) {
+#pragma unroll 1
+        for (int j = k / 2; j > 0; j /= 2) {
+            const u64 y = shfl_xor64(key, j);
+            const bool up = (lane & k) == 0, lower = (lane & j) == 0;
+            key = (key < y) == (up == lower) ? key : y;
+        }
+    }
+    const bool in = lane < n;
+    const float val = in ? key_value((unsigned)(key >> 32)) : 0.0f;
+    const double real = in ? w.real(val) : 0.0;
+    const u64 m = in ? w.fixed(val) : 0;
+    u64 upto = m;
+#pragma unroll 1
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 a = shfl_up64(upto, o);
+        if (lane >= o) upto += a;
+    }
+    const u64 listed = ((u64)(unsigned)__shfl((int)(upto >> 32), 63, 64) << 32) | (unsigned)__shfl((int)upto, 63, 64);
+    int rank = lane + 1;
+    if (mass) {  // on top of the bins in front: what the bin's first element lacks, for those behind it too
+        const int b = in ? bins.of(val) : -1, prev = __shfl_up(b, 1, 64);
+        const bool head = in && (lane == 0 || b != prev);
+        const u64 off = head ? (b > 0 ? mass[b - 1] : 0) - (upto - m) : 0;
+        const int off_rank = head ? (b > 0 ? (int)count[b - 1] : 0) - lane : 0;
+        const u64 heads = __ballot(head) & (~0ull >> (63 - lane));
+        const int from = 63 - __clzll((long long)(heads | 1));
+        upto += ((u64)(unsigned)__shfl((int)(off >> 32), from, 64) << 32) | (unsigned)__shfl((int)off, from, 64);
+        rank += __shfl(off_rank, from, 64);
+    }
+    auto at = [&](u64 v, u64 lanes, u64 none) {  // v of the first of the lanes
+        if (!lanes) return none;
+        const int from = __ffsll((long long)lanes) - 1;
+        return ((u64)(unsigned)__shfl((int)(v >> 32), from, 64) << 32) | (unsigned)__shfl((int)v, from, 64);
+    };
+    u64 left = cuts.total ? cuts.total : listed, kept = mass ? left : min(left, listed);
+    if (cuts.k) left = kept = at(upto, __ballot(in && m && rank == rule.top_k), listed);
+    if (cuts.p) {
+        const double t = (double)rule.top_p * (double)left;
+        kept = min(kept, at(upto, __ballot(in && (double)upto >= t), listed));
+    }
+    if (cuts.m) {
+        if (mass) kept = min(kept, cuts.upto_m);
+        kept = min(kept, at(upto - m, __ballot(in && real < (double)rule.min_p), kept));
+    }
+    const double t = (double)rule.u * (double)kept;
+    return (int)(unsigned)at(key, __ballot(in && (double)upto > t), 0);
 }
 
 // ------------------------------------------------------------------
@@ -595,6 +748,16 @@ __device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, co
 // ------------------------------------------------------------------
 // kernels
 // ------------------------------------------------------------------
+// Rules of a short row; total 0: its list has all the mass.
+__device__ __forceinline__ SmpCuts short_cuts(const gh_sampling& rule, u64 total) {
+    SmpCuts q;
+    q.total = total;
+    q.k = rule.top_k > 0;
+    q.p = rule.top_p < 1.0f;
+    q.m = rule.min_p > 0.0f;
+    return q;
+}
+
 // one workgroup a row
 __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int bits, SmpRules rules, int32_t* tokens) {
     __shared__ Small sh;
@@ -602,30 +765,46 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
     __shared__ union {
         PickShared p;
         SlowShared slow;
+        float group_max[PT];
     } u;
     const gh_sampling rule = rules.r[blockIdx.x];
     const float* l = logits + (size_t)blockIdx.x * n;
+    const int tid = threadIdx.x;
     const Stat s = range_stat<PT>(l, 0, n, sh);
-    int t;
     if (!drawn(s, rule)) {
-        t = token_of_undrawn(s);
-    } else {
-        const Weights w = weights_of(s, rule, bits);
-        const Bins bins = bins_of(s, w);
-        if (threadIdx.x == 0) sh.n_list = 0;
-        range_hist<PT>(l, 0, n, w, bins, rule.top_k > 0, h);
-        const SmpCuts cuts = find_cuts<PT>(w, bins, rule, h, sh);
-        range_gather<PT>(l, 0, n, bins, cuts, u.p.list, &sh.n_list);
-        __syncthreads();
-        const unsigned listed = sh.n_list;
-        if (listed <= SMP_LIST) {
-            sort_list(u.p.list, listed);
-            t = pick(w, bins, rule, cuts, h.mass, h.count, listed, u.p, sh);
-        } else {
-            t = slow_row(l, n, w, rule, u.slow, sh);
-        }
+        if (tid == 0) tokens[blockIdx.x] = token_of_undrawn(s);
+        return;
     }
-    if (threadIdx.x == 0) tokens[blockIdx.x] = t;
+    const Weights w = weights_of(s, rule, bits);
+    const Bins bins = bins_of(s, w);
+    u.group_max[tid] = s.own;
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
+    const Short row = short_row<PT>(u.group_max, PT, w, bins, rule, h, sh);
+    SmpCuts cuts;
+    const bool is_short = row.last >= 0;
+    if (is_short) {
+        cuts = short_cuts(rule, row.all ? range_mass<PT>(l, 0, n, w, bins, sh) : 0);
+        range_gather<PT>(l, 0, n, bins, 0, row.last, u.p.list, &sh.n_list, [](int) { return true; });
+    } else {
+        range_hist<PT>(l, 0, n, w, bins, rule.top_k > 0, h);
+        cuts = find_cuts<PT>(w, bins, rule, h, sh);
+        range_gather<PT>(l, 0, n, bins, cuts, u.p.list, &sh.n_list);
+    }
+    __syncthreads();
+    const unsigned listed = sh.n_list;
+    const u64* mass = is_short ? nullptr : h.mass;
+    int t;
+    if (listed <= 64) {
+        if (tid >= 64) return;
+        t = pick_wave(w, bins, rule, cuts, mass, h.count, u.p.list[tid], listed);
+    } else if (listed <= SMP_LIST) {
+        sort_list(u.p.list, listed);
+        t = pick(w, bins, rule, cuts, mass, h.count, listed, u.p, sh);
+    } else {
+        t = slow_row(l, n, w, rule, u.slow, sh);
+    }
+    if (tid == 0) tokens[blockIdx.x] = t;
 }
 
 __device__ __forceinline__ int chunk_begin(int n, int c, int chunks) { return (int)((int64_t)n * c / chunks); }
@@ -633,13 +812,16 @@ __device__ __forceinline__ int chunk_begin(int n, int c, int chunks) { return (i
 constexpr int CT = 512;  // threads of a workgroup that reads a chunk of a row
 
 // a row's chunks: stats; the row's bins cleared
-__global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, SmpRow* rows) {
+__global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, int group, SmpRow* rows) {
     __shared__ Small sh;
-    const int c = blockIdx.x, chunks = gridDim.x;
+    const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
     SmpRow& r = rows[blockIdx.y];
-    for (int b = c * CT + threadIdx.x; b < SMP_BINS; b += chunks * CT) r.mass[b] = 0, r.count[b] = 0;
+    for (int b = c * CT + tid; b < SMP_BINS; b += chunks * CT) r.mass[b] = 0, r.count[b] = 0;
     const Stat s = range_stat<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), sh);
-    if (threadIdx.x == 0) {
+    float own = s.own;
+    for (int o = 1; o < group; o <<= 1) own = fmaxf(own, __shfl_xor(own, o, 64));
+    if (tid % group == 0) r.group_max[(c * CT + tid) / group] = own;
+    if (tid == 0) {
         r.first[c] = s.first;
         r.low[c] = s.low;
         r.nan[c] = s.nan;
@@ -659,20 +841,34 @@ __device__ __forceinline__ Stat row_stat(const SmpRow& r, int chunks) {
         first = min(first, shfl_xor64(first, o));
         low = fminf(low, __shfl_xor(low, o, 64));
     }
-    return {first, low, nan};
+    return {first, low, nan, 0.0f};
 }
 
-__global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int bits, SmpRules rules, SmpRow* rows) {
+// A short row: its list.  A long one: its bins.
+__global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int bits, int groups, SmpRules rules, SmpRow* rows) {
+    __shared__ Small sh;
     __shared__ BinSums h;
-    const int c = blockIdx.x, chunks = gridDim.x;
+    const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
     const gh_sampling rule = rules.r[blockIdx.y];
     SmpRow& r = rows[blockIdx.y];
     const Stat s = row_stat(r, chunks);
     if (!drawn(s, rule)) return;
     const Weights w = weights_of(s, rule, bits);
-    range_hist<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), w, bins_of(s, w),
-                   rule.top_k > 0, h);
-    for (int b = threadIdx.x; b < SMP_BINS; b += CT) {
+    const Bins bins = bins_of(s, w);
+    const float* l = logits + (size_t)blockIdx.y * n;
+    const int i0 = chunk_begin(n, c, chunks), i1 = chunk_begin(n, c + 1, chunks);
+    const Short row = short_row<CT>(r.group_max, groups, w, bins, rule, h, sh);
+    if (c == 0 && tid == 0) r.is_short = row.last < 0 ? 0 : row.all ? 2 : 1;
+    if (row.last >= 0) {
+        if (row.all) {
+            const u64 sum = range_mass<CT>(l, i0, i1, w, bins, sh);
+            if (tid == 0) atomicAdd(&r.mass[0], sum);
+        }
+        range_gather<CT>(l, i0, i1, bins, 0, row.last, r.list, &r.n_list, [](int) { return true; });
+        return;
+    }
+    range_hist<CT>(l, i0, i1, w, bins, rule.top_k > 0, h);
+    for (int b = tid; b < SMP_BINS; b += CT) {
         if (h.mass[b]) atomicAdd(&r.mass[b], h.mass[b]);
         if (h.count[b]) atomicAdd(&r.count[b], h.count[b]);
     }
@@ -681,19 +877,19 @@ __global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int
 __global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, int bits, SmpRules rules, SmpRow* rows) {
     __shared__ Small sh;
     __shared__ BinSums h;
-    const int c = blockIdx.x, chunks = gridDim.x;
+    const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
     const gh_sampling rule = rules.r[blockIdx.y];
     SmpRow& r = rows[blockIdx.y];
     const Stat s = row_stat(r, chunks);
-    if (!drawn(s, rule)) return;
+    if (!drawn(s, rule) || r.is_short) return;
     const Weights w = weights_of(s, rule, bits);
     const Bins bins = bins_of(s, w);
-    for (int b = threadIdx.x; b < SMP_BINS; b += CT) h.mass[b] = r.mass[b], h.count[b] = r.count[b];
+    for (int b = tid; b < SMP_BINS; b += CT) h.mass[b] = r.mass[b], h.count[b] = r.count[b];
     __syncthreads();
     const SmpCuts cuts = find_cuts<CT>(w, bins, rule, h, sh);
     if (c == 0) {  // for the last step
-        for (int b = threadIdx.x; b < SMP_BINS; b += CT) r.run_mass[b] = h.mass[b], r.run_count[b] = h.count[b];
-        if (threadIdx.x == 0) r.cuts = cuts;
+        for (int b = tid; b < SMP_BINS; b += CT) r.run_mass[b] = h.mass[b], r.run_count[b] = h.count[b];
+        if (tid == 0) r.cuts = cuts;
     }
     range_gather<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
                      r.list, &r.n_list);
@@ -708,23 +904,32 @@ __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int
     } u;
     const gh_sampling rule = rules.r[blockIdx.x];
     const SmpRow& r = rows[blockIdx.x];
+    const int tid = threadIdx.x;
+    const u64 key = r.list[tid];
     const Stat s = row_stat(r, chunks);
-    const int listed = (int)min(r.n_list, (unsigned)SMP_LIST + 1);
-    int t;
+    const unsigned listed = r.n_list;
     if (!drawn(s, rule)) {
-        t = token_of_undrawn(s);
-    } else {
-        const Weights w = weights_of(s, rule, bits);
-        if (listed <= SMP_LIST) {
-            for (int i = threadIdx.x; i < listed; i += PT) u.p.list[i] = r.list[i];
-            __syncthreads();
-            sort_list(u.p.list, listed);
-            t = pick(w, bins_of(s, w), rule, r.cuts, r.run_mass, r.run_count, listed, u.p, sh);
-        } else {
-            t = slow_row(logits + (size_t)blockIdx.x * n, n, w, rule, u.slow, sh);
-        }
+        if (tid == 0) tokens[blockIdx.x] = token_of_undrawn(s);
+        return;
     }
-    if (threadIdx.x == 0) tokens[blockIdx.x] = t;
+    const Weights w = weights_of(s, rule, bits);
+    const Bins bins = bins_of(s, w);
+    const int is_short = r.is_short;
+    const SmpCuts cuts = is_short ? short_cuts(rule, is_short == 2 ? r.mass[0] : 0) : r.cuts;
+    const u64* mass = is_short ? nullptr : r.run_mass;
+    int t;
+    if (listed <= 64) {
+        if (tid >= 64) return;
+        t = pick_wave(w, bins, rule, cuts, mass, r.run_count, key, listed);
+    } else if (listed <= SMP_LIST) {
+        for (int i = tid; i < (int)listed; i += PT) u.p.list[i] = i < PT ? key : r.list[i];
+        __syncthreads();
+        sort_list(u.p.list, listed);
+        t = pick(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh);
+    } else {
+        t = slow_row(logits + (size_t)blockIdx.x * n, n, w, rule, u.slow, sh);
+    }
+    if (tid == 0) tokens[blockIdx.x] = t;
 }
 
 }  // namespace
@@ -736,8 +941,11 @@ int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRule
         hipLaunchKernelGGL(k_smp_row, dim3(n_rows), dim3(PT), 0, s, logits, vocab, bits, rules, tokens);
     } else {
         const dim3 grid(chunks, n_rows);
-        hipLaunchKernelGGL(k_smp_stat, grid, dim3(CT), 0, s, logits, vocab, scratch);
-        hipLaunchKernelGGL(k_smp_hist, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
+        // threads that share a group: a power of two, and 512 to 1023 groups a row
+        int group = 1;
+        while (chunks * CT / group >= SMP_GROUPS) group *= 2;
+        hipLaunchKernelGGL(k_smp_stat, grid, dim3(CT), 0, s, logits, vocab, group, scratch);
+        hipLaunchKernelGGL(k_smp_hist, grid, dim3(CT), 0, s, logits, vocab, bits, chunks * CT / group, rules, scratch);
         hipLaunchKernelGGL(k_smp_gather, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
         hipLaunchKernelGGL(k_smp_pick, dim3(n_rows), dim3(PT), 0, s, logits, vocab, bits, rules, (const SmpRow*)scratch, chunks,
                            tokens);
