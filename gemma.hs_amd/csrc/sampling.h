@@ -48,7 +48,8 @@ struct SmpRow {
 // Workgroups a row; 0: one, which runs every step (no scratch).
 inline int smp_chunks(int n_rows, int vocab) {
     if (vocab <= 16384) return 0;
-    return std::max(1, std::min({SMP_CHUNKS, 512 / n_rows, (vocab + 4095) / 4096}));
+    const int least = n_rows <= 4 ? 4096 : 8192;  // logits a workgroup
+    return std::max(1, std::min({SMP_CHUNKS, 1024 / n_rows, (vocab + least - 1) / least}));
 }
 
 int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRules& rules, SmpRow* scratch, int32_t* tokens,

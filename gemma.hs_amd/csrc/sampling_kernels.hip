@@ -433,7 +433,6 @@ __device__ __forceinline__ u64 range_mass(const float* l, int i0, int i1, const 
 // step 4, 1024 threads
 // ------------------------------------------------------------------
 constexpr int PT = 1024;
-constexpr int PER = SMP_LIST / PT;
 
 struct PickShared {
     u64 list[SMP_LIST];
@@ -489,7 +488,8 @@ __device__ __forceinline__ void sort_list(u64* list, int n) {
 
 // The token, from the sorted list and the running sums of the bins in front
 // of its elements (LDS or global; none for a list that begins with the row's
-// first element and leaves none out).
+// first element and leaves none out), PER elements a thread.
+template <int PER>
 __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh_sampling& rule, const SmpCuts& cuts,
                                     const u64* mass, const unsigned* count, int n, PickShared& p, Small& sh) {
     auto bin_of = [&](float v) { return mass ? bins.of(v) : 0; };
@@ -800,7 +800,8 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
         t = pick_wave(w, bins, rule, cuts, mass, h.count, u.p.list[tid], listed);
     } else if (listed <= SMP_LIST) {
         sort_list(u.p.list, listed);
-        t = pick(w, bins, rule, cuts, mass, h.count, listed, u.p, sh);
+        t = listed <= PT ? pick<1>(w, bins, rule, cuts, mass, h.count, listed, u.p, sh)
+                         : pick<SMP_LIST / PT>(w, bins, rule, cuts, mass, h.count, listed, u.p, sh);
     } else {
         t = slow_row(l, n, w, rule, u.slow, sh);
     }
@@ -925,7 +926,8 @@ __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int
         for (int i = tid; i < (int)listed; i += PT) u.p.list[i] = i < PT ? key : r.list[i];
         __syncthreads();
         sort_list(u.p.list, listed);
-        t = pick(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh);
+        t = listed <= PT ? pick<1>(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh)
+                         : pick<SMP_LIST / PT>(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh);
     } else {
         t = slow_row(logits + (size_t)blockIdx.x * n, n, w, rule, u.slow, sh);
     }
