@@ -51,6 +51,17 @@ int check_not_capturing(const char* fn, gh_ctx* ctx) {
     return GH_OK;
 }
 
+// Blocks a workgroup of the attention takes at most.  `most`: of the longest
+// tile; `work`: of all `wgs` (entry, kv head, row tile) together.
+int kv8_chunk(int hd, int tile, int most, int64_t work, int64_t wgs) {
+    if (tile == 4) {
+        const int64_t slots = hd <= 64 ? 512 : 256, rounds = (wgs + slots - 1) / slots;
+        const bool full = wgs * 10 >= 9 * rounds * slots && most * wgs * 10 <= 11 * work;
+        return most <= 16 || full ? std::max(most, 1) : (int)std::max<int64_t>(8, (work + 767) / 768);
+    }
+    return (int)std::max<int64_t>(4, (work + 511) / 512);
+}
+
 int blocks_of(int begin, int end) {  // blocks that [begin, end) touches
     return end > begin ? (end - 1) / KV8_BLOCK - begin / KV8_BLOCK + 1 : 0;
 }
@@ -162,18 +173,19 @@ extern "C" int gh_kv8_append(gh_kv8* kv, int32_t n, const int32_t* seqs, const i
     for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
         const int m = std::min(n - i0, KV8_BATCH);
         Kv8Batch b;
-        int blocks = 0;
-        b.off[0] = 0;
+        int blocks = 0, rows = 0;
         for (int i = 0; i < m; ++i) {
             const int s = seqs[i0 + i], t = n_tok[i0 + i];
             b.seq[i] = s;
             b.pos[i] = kv->len[s];
-            b.off[i + 1] = b.off[i] + t;
+            b.off[i] = rows;
+            b.cnt[i] = t;
+            rows += t;
             blocks = std::max(blocks, blocks_of(kv->len[s], kv->len[s] + t));
         }
         if (blocks) GH_CHECK(launch_kv8_append(dev(kv), kv->hd, b, m, blocks, k, v, ctx->stream));
-        k += (size_t)b.off[m] * row;
-        v += (size_t)b.off[m] * row;
+        k += (size_t)rows * row;
+        v += (size_t)rows * row;
     }
     for (int i = 0; i < n; ++i) kv->len[seqs[i]] += n_tok[i];
     return op_sync(ctx);
@@ -200,7 +212,8 @@ extern "C" int gh_kv8_truncate(gh_kv8* kv, int32_t n, const int32_t* seqs, const
             if (lens[i] == kv->len[seqs[i]] || lens[i] % KV8_BLOCK == 0) continue;
             b.seq[m] = seqs[i];
             b.pos[m] = kv->len[seqs[i]];
-            b.off[m++] = lens[i];
+            b.off[m] = 0;
+            b.cnt[m++] = lens[i];
         }
         if (m) GH_CHECK(launch_kv8_truncate(dev(kv), kv->hd, b, m, ctx->stream));
         ran = ran || m;
@@ -230,18 +243,19 @@ extern "C" int gh_kv8_read(gh_kv8* kv, int32_t n, const int32_t* seqs, const int
     for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
         const int m = std::min(n - i0, KV8_BATCH);
         Kv8Batch b;
-        int blocks = 0;
-        b.off[0] = 0;
+        int blocks = 0, rows = 0;
         for (int i = 0; i < m; ++i) {
             const int at = begins[i0 + i], end = ends[i0 + i];
             b.seq[i] = seqs[i0 + i];
             b.pos[i] = at;
-            b.off[i + 1] = b.off[i] + end - at;
+            b.off[i] = rows;
+            b.cnt[i] = end - at;
+            rows += end - at;
             blocks = std::max(blocks, blocks_of(at, end));
         }
         if (blocks) GH_CHECK(launch_kv8_read(dev(kv), kv->hd, b, m, blocks, k_out, v_out, ctx->stream));
-        if (k_out) k_out += (size_t)b.off[m] * row;
-        if (v_out) v_out += (size_t)b.off[m] * row;
+        if (k_out) k_out += (size_t)rows * row;
+        if (v_out) v_out += (size_t)rows * row;
     }
     return op_sync(ctx);
 }
@@ -270,31 +284,43 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
     const size_t row = (size_t)n_heads * kv->hd;
     for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
         const int m = std::min(n - i0, KV8_BATCH);
-        Kv8Batch b;
-        Att8 a{};
-        b.off[0] = 0;
-        int rows = 0;       // query rows of the longest entry
+        // the longest entries first: their workgroups start before the others'
+        struct Entry {
+            int seq, len, off, cnt, blocks;
+        } e[KV8_BATCH];
+        int tokens = 0, rows = 0;  // query tokens of all; query rows of the longest entry
         for (int i = 0; i < m; ++i) {
-            b.seq[i] = seqs[i0 + i];
-            b.pos[i] = kv->len[b.seq[i]];
-            b.off[i + 1] = b.off[i] + n_q[i0 + i];
-            rows = std::max(rows, n_q[i0 + i] * group);
+            const int s = seqs[i0 + i], t = n_q[i0 + i];
+            e[i] = {s, kv->len[s], tokens, t, 0};
+            tokens += t;
+            rows = std::max(rows, t * group);
         }
         if (rows == 0) continue;
+        Att8 a{};
         a.tile = rows <= 4 ? 4 : 16;
         a.tiles = (rows + a.tile - 1) / a.tile;
-        int most = 0;       // blocks of the longest row tile
-        int64_t work = 0;   // blocks of all row tiles
+        int most = 0;      // blocks of the longest row tile
+        int64_t work = 0, wgs = 0;  // blocks of all row tiles, and these
         for (int i = 0; i < m; ++i) {
-            const int len = b.pos[i], t = b.off[i + 1] - b.off[i];
+            if (e[i].cnt == 0) continue;
             // tokens a tile may see: up to the window and its own rows
+            const int len = e[i].len;
             const int span = window ? (int)std::min<int64_t>(len, (int64_t)window + a.tile / group + 1) : len;
-            const int blocks = std::min((len + KV8_BLOCK - 1) / KV8_BLOCK, span / KV8_BLOCK + 2);
-            if (t) most = std::max(most, blocks);
-            work += (int64_t)((t * group + a.tile - 1) / a.tile) * kv->nkv * blocks;
+            e[i].blocks = std::min((len + KV8_BLOCK - 1) / KV8_BLOCK, span / KV8_BLOCK + 2);
+            most = std::max(most, e[i].blocks);
+            const int64_t tiles = (int64_t)((e[i].cnt * group + a.tile - 1) / a.tile) * kv->nkv;
+            wgs += tiles;
+            work += tiles * e[i].blocks;
         }
-        // chunks of whole rounds of a workgroup's 4 waves, about 512 workgroups
-        a.chunk = (int)std::max<int64_t>(4, (work / 512 + 3) / 4 * 4);
+        std::stable_sort(e, e + m, [](const Entry& x, const Entry& y) { return x.blocks > y.blocks; });
+        Kv8Batch b;
+        for (int i = 0; i < m; ++i) {
+            b.seq[i] = e[i].seq;
+            b.pos[i] = e[i].len;
+            b.off[i] = e[i].off;
+            b.cnt[i] = e[i].cnt;
+        }
+        a.chunk = kv8_chunk(kv->hd, a.tile, most, work, wgs);
         a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
         if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
             return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows in one call", rows);
@@ -304,15 +330,15 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
         a.group = group;
         a.group_inv = group == 1 ? 0 : (unsigned)(((uint64_t(1) << 32) + group - 1) / group);
         a.window = window;
-        a.rows = (size_t)b.off[m] * n_heads;
+        a.rows = (size_t)tokens * n_heads;
         if (a.ns > 1) {
             void* part = nullptr;
             GH_CHECK(ctx_scratch(ctx, a.rows * a.ns * (kv->hd + 2) * sizeof(float), &part));
             a.part = (float*)part;
         }
         GH_CHECK(launch_kv8_attention(dev(kv), kv->hd, b, m, a, ctx->stream));
-        q += (size_t)b.off[m] * row;
-        out += (size_t)b.off[m] * row;
+        q += (size_t)tokens * row;
+        out += (size_t)tokens * row;
     }
     return op_sync(ctx);
 }

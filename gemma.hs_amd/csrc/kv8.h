@@ -42,14 +42,15 @@ struct Kv8Dev {
 
 // Up to KV8_BATCH sequences of a call, by value in a kernel's arguments (no
 // copy to the device, and the host has checked every number).
-constexpr int KV8_BATCH = 256;
+constexpr int KV8_BATCH = 240;
 struct Kv8Batch {
     int seq[KV8_BATCH];
-    int pos[KV8_BATCH];      // append: tokens before; truncate: tokens before; read: begin; attention: tokens
-    int off[KV8_BATCH + 1];  // prefix sums of the counts (truncate: the new length itself)
+    int pos[KV8_BATCH];  // append, truncate: tokens before; read: begin; attention: tokens
+    int off[KV8_BATCH];  // first of the entry's rows among the call's
+    int cnt[KV8_BATCH];  // new tokens; tokens to read; query tokens; truncate: the new length itself
 };
 
-// `most`: the largest count (append, read) of the batch's sequences, in blocks touched
+// blocks: the most that one of the entries touches
 int launch_kv8_append(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, const float* k, const float* v,
                       hipStream_t s);
 int launch_kv8_truncate(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, hipStream_t s);
@@ -67,8 +68,8 @@ struct Att8 {
     int window;
     int tile;   // rows a tile
     int tiles;  // row tiles of the longest entry
-    int ns;     // key chunks
-    int chunk;  // blocks a chunk
+    int ns;     // key chunks of the longest entry
+    int chunk;  // blocks a chunk at most: an entry's chunks are of one size
 };
 int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t s);
 

@@ -222,7 +222,7 @@ __global__ __launch_bounds__(4 * HD, 8) void k_kv8_append(Kv8Dev c, Kv8Batch b, 
     __shared__ uint32_t slot[16];
     const int i = blockIdx.z, h = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
-    const int pos = b.pos[i], cnt = b.off[i + 1] - b.off[i], end = pos + cnt;
+    const int pos = b.pos[i], cnt = b.cnt[i], end = pos + cnt;
     const int first = pos / KV8_BLOCK, blk = first + blockIdx.x;
     if (cnt == 0 || blk * KV8_BLOCK >= end) return;
     const int r0 = max(pos - blk * KV8_BLOCK, 0), r1 = min(end - blk * KV8_BLOCK, KV8_BLOCK);
@@ -270,7 +270,7 @@ template <int HD>
 __global__ __launch_bounds__(4 * HD, 8) void k_kv8_truncate(Kv8Dev c, Kv8Batch b) {
     __shared__ uint32_t slot[16];
     const int i = blockIdx.z, h = blockIdx.y >> 1;
-    const int blk = b.off[i] / KV8_BLOCK, r1 = b.off[i] % KV8_BLOCK;
+    const int blk = b.cnt[i] / KV8_BLOCK, r1 = b.cnt[i] % KV8_BLOCK;
     const bool same = blk == b.pos[i] / KV8_BLOCK;
     const size_t head = (size_t)b.seq[i] * c.nkv + h, at = head * c.nb + blk;
     if (blockIdx.y & 1)
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(4 * HD, 8) void k_kv8_read(Kv8Dev c, Kv8Batch b, fl
     const int i = blockIdx.z, h = blockIdx.y >> 1;
     const bool is_v = blockIdx.y & 1;
     float* out = is_v ? v : k;
-    const int pos = b.pos[i], cnt = b.off[i + 1] - b.off[i], end = pos + cnt;
+    const int pos = b.pos[i], cnt = b.cnt[i], end = pos + cnt;
     const int blk = pos / KV8_BLOCK + blockIdx.x;
     if (!out || cnt == 0 || blk * KV8_BLOCK >= end) return;
     const int r0 = max(pos - blk * KV8_BLOCK, 0), r1 = min(end - blk * KV8_BLOCK, KV8_BLOCK);
@@ -347,11 +347,12 @@ __device__ __forceinline__ uint32_t byte_of(const uint32_t* d, int n) {
 // digit n of row r and the last four zero (Narrow).  Narrow is for decoding,
 // where a kv head has few query rows: a third of the products, and of the
 // conversions of their results.
+template <bool ONCE>  // one tile a kv head: each code is read once a call
 struct Wide {
     static constexpr int ROWS = 16, DIG = 3, WAVES = 4;
     int row;
     __device__ __forceinline__ explicit Wide(int col) : row(col) {}
-    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return *p; }  // other tiles read the same codes
+    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return ONCE ? __builtin_nontemporal_load(p) : *p; }
     // digit n of four probabilities
     __device__ __forceinline__ int share(const uint32_t* d, int n) const {
         return (int)(n < 2 ? byte_of(d, n) ^ DIGIT_BIAS : byte_of(d, n));
@@ -359,10 +360,10 @@ struct Wide {
     // column of digit n of a query row in the digit's operand
     __device__ __forceinline__ static int place(int r, int) { return r; }
     __device__ __forceinline__ static int operand(int n) { return n; }
-    // a product's value times w: each sum is below 2^24
+    // a product's value; a digit's sum is below 2^22 (256 dims, or 64 tokens)
     __device__ __forceinline__ float scaled(float w) const { return w; }
     __device__ __forceinline__ float sum(const i32x4* acc, int j) const {
-        return fmaf((float)acc[2][j], 65536.0f, fmaf((float)acc[1][j], 256.0f, (float)acc[0][j]));
+        return fmaf((float)acc[2][j], 65536.0f, (float)(acc[1][j] * 256 + acc[0][j]));
     }
     __device__ __forceinline__ float join(float v) const { return v; }
 };
@@ -405,7 +406,7 @@ struct Narrow {
 template <int HD, class Cols>
 __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
     constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Cols::ROWS, DIG = Cols::DIG, WAVES = Cols::WAVES;
-    constexpr bool LATE_K = HD == 256, LATE_V = HD == 256 && ROWS == 16;
+    constexpr bool LATE_K = HD >= 128, LATE_V = HD == 256 && ROWS == 16;
     __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
     __shared__ uint32_t qmax[ROWS];
     __shared__ i32x4 qs[DIG][KD][64];
@@ -422,7 +423,7 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         tile = a.tiles - 1 - t;
     }
     const int row0 = tile * ROWS;
-    const int n_q = b.off[i + 1] - b.off[i], rows = min(n_q * a.group - row0, ROWS), len = b.pos[i];
+    const int n_q = b.cnt[i], rows = min(n_q * a.group - row0, ROWS), len = b.pos[i];
     if (rows <= 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const Cols col(lane & 15);
@@ -435,7 +436,10 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
     // positions of the tile's first and last row, and the blocks they see
     const int p0 = len - n_q + token_of(0), p1 = len - n_q + token_of(rows - 1);
     const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
-    const int blk0 = begin + chunk * a.chunk, blk1 = min(blk0 + a.chunk, end);
+    // chunks of one size: as many as a.chunk makes, evenly
+    const unsigned blocks = max(end - begin, 0), parts = (blocks + a.chunk - 1) / (unsigned)a.chunk;
+    const int size = a.ns > 1 && parts ? (int)((blocks + parts - 1) / parts) : (int)blocks;
+    const int blk0 = begin + chunk * size, blk1 = min(blk0 + size, end);
     if (blk0 >= blk1) {  // nothing to see in this chunk
         if (a.ns > 1) {
             if (tid < rows) {
@@ -471,18 +475,26 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
     }
 
     // digits of the query rows, a wave a row, a lane 4 dims
-#pragma unroll 1
-    for (int r = wave; r < ROWS; r += WAVES) {
-        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < rows && 4 * lane < HD) x = ((const f32x4*)(a.q + slot_of(r) * HD))[lane];
-        uint32_t m = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
+    constexpr int RW = (ROWS + WAVES - 1) / WAVES;
+    f32x4 x[RW];
+#pragma unroll
+    for (int e = 0; e < RW; ++e) {
+        const int r = wave + e * WAVES;
+        x[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < rows && 4 * lane < HD) x[e] = ((const f32x4*)(a.q + slot_of(r) * HD))[lane];
+    }
+#pragma unroll
+    for (int e = 0; e < RW; ++e) {
+        const int r = wave + e * WAVES;
+        if (ROWS % WAVES && r >= ROWS) break;
+        uint32_t m = max(max(abs_bits(x[e].x), abs_bits(x[e].y)), max(abs_bits(x[e].z), abs_bits(x[e].w)));
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
         // a row that is nearly zero: its digits vanish
         const float inv = DIGIT_MAX / fmaxf(__uint_as_float(m), 0x1p-100f);
         uint32_t dg[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dg[e] = digits_of(fminf(fmaxf(x[e] * inv, -DIGIT_MAX), DIGIT_MAX));
+        for (int d = 0; d < 4; ++d) dg[d] = digits_of(fminf(fmaxf(x[e][d] * inv, -DIGIT_MAX), DIGIT_MAX));
         if (4 * lane < KR) {
 #pragma unroll
             for (int n = 0; n < (ROWS == 4 ? 4 : 3); ++n)
@@ -751,7 +763,8 @@ int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int block
 int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t s) {
     return with_hd(hd, [&](auto h) {
         if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value, Narrow>), dim3(a.ns, c.nkv, n), dim3(64 * Narrow::WAVES), 0, s, c, b, a);
-        else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide::WAVES), 0, s, c, b, a);
+        else if (a.tiles == 1) hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<true>>), dim3(a.ns * c.nkv, 1, n), dim3(64 * Wide<true>::WAVES), 0, s, c, b, a);
+        else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<false>>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide<false>::WAVES), 0, s, c, b, a);
         if (a.ns > 1) hipLaunchKernelGGL(k_kv8_combine<h.value>, dim3(a.rows * (h.value / 32)), dim3(NT), 0, s, a);
     });
 }

@@ -48,9 +48,10 @@ static void look(const Kv8Batch& b, int n) {
 int launch_kv8_append(const Kv8Dev&, int, const Kv8Batch& b, int n, int blocks, const float* k, const float* v, hipStream_t) {
     look(b, n);
     WANT(k && v && b.off[0] == 0);
+    for (int i = 1; i < n; ++i) WANT(b.off[i] == b.off[i - 1] + b.cnt[i - 1]);
     int most = 0;
     for (int i = 0; i < n; ++i) {
-        const int cnt = b.off[i + 1] - b.off[i], end = b.pos[i] + cnt;
+        const int cnt = b.cnt[i], end = b.pos[i] + cnt;
         WANT(cnt >= 0 && end <= cap_tokens);
         if (cnt) most = std::max(most, (end - 1) / 64 - b.pos[i] / 64 + 1);
     }
@@ -59,20 +60,26 @@ int launch_kv8_append(const Kv8Dev&, int, const Kv8Batch& b, int n, int blocks, 
 }
 int launch_kv8_truncate(const Kv8Dev&, int, const Kv8Batch& b, int n, hipStream_t) {
     look(b, n);
-    for (int i = 0; i < n; ++i) WANT(b.off[i] % 64 != 0 && b.off[i] < b.pos[i]);
+    for (int i = 0; i < n; ++i) WANT(b.cnt[i] % 64 != 0 && b.cnt[i] < b.pos[i]);
     return GH_OK;
 }
 int launch_kv8_read(const Kv8Dev&, int, const Kv8Batch& b, int n, int blocks, float* k, float* v, hipStream_t) {
     look(b, n);
     WANT((k || v) && blocks > 0);
-    for (int i = 0; i < n; ++i) WANT(b.off[i + 1] >= b.off[i] && b.pos[i] + b.off[i + 1] - b.off[i] <= cap_tokens);
+    for (int i = 0; i < n; ++i) WANT(b.cnt[i] >= 0 && b.pos[i] + b.cnt[i] <= cap_tokens);
     return GH_OK;
 }
 int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t) {
     look(b, n);
     attentions.push_back(a);
     WANT(a.q && a.out && a.group * c.nkv == a.heads && (a.tile == 4 || a.tile == 16) && a.tiles > 0 && a.ns > 0);
-    WANT(a.rows == (size_t)b.off[n] * a.heads);
+    std::vector<char> taken(a.rows / a.heads, 0);  // every query token has one entry
+    for (int i = 0; i < n; ++i)
+        for (int t = b.off[i]; t < b.off[i] + b.cnt[i]; ++t) {
+            WANT(t >= 0 && (size_t)t < taken.size() && !taken[t]);
+            if (t >= 0 && (size_t)t < taken.size()) taken[t] = 1;
+        }
+    for (char c : taken) WANT(c);
     WANT((int64_t)a.ns * a.tiles * c.nkv <= 1 << 23);
     if (a.tile == 4) WANT(a.tiles == 1);
     if (a.ns > 1) {  // the scratch holds every state
@@ -80,7 +87,7 @@ int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, cons
         if (a.part) std::memset(a.part, 0, a.rows * a.ns * (hd + 2) * sizeof(float));
     }
     for (int i = 0; i < n; ++i) {
-        const int rows = (b.off[i + 1] - b.off[i]) * a.group;
+        const int rows = b.cnt[i] * a.group;
         WANT(rows <= a.tiles * a.tile && b.pos[i] <= cap_tokens);
         for (int r : {0, 1, rows / 2, rows - 1})
             if (r >= 0 && a.group > 1) WANT((int)(((uint64_t)r * a.group_inv) >> 32) == r / a.group);
@@ -183,7 +190,7 @@ int refusals() {
     CHECK(length(kv, 0) == 64 && length(kv, 1) == 100);
     const int32_t to2[] = {63, 70};
     CHECK(gh_kv8_truncate(kv, 2, s01, to2) == GH_OK && launches == before + 1);
-    CHECK(batches.back().pos[0] == 64 && batches.back().off[0] == 63 && batches.back().pos[1] == 100);
+    CHECK(batches.back().pos[0] == 64 && batches.back().cnt[0] == 63 && batches.back().pos[1] == 100);
 
     // read
     const int32_t b0[] = {0}, e63[] = {63}, e64[] = {64}, b9[] = {9}, e8[] = {8};
@@ -240,7 +247,7 @@ int refusals() {
     for (float x : {-0.1f, 1.1f, nan, inf}) CHECK(refused({1, 0, x, 0, 0}) && refused({1, 0, 1, x, 0}) && refused({1, 0, 1, 0, x}));
     CHECK(refused({1, 0, 1, 0, 1.0f}));
     CHECK(launches == l0);
-    CHECK(gh_sample_rows(ctx, P, 300, 10, r, t) == GH_OK && launches == l0 + 3 && sample_rows.back() == 300 - 256);
+    CHECK(gh_sample_rows(ctx, P, 300, 10, r, t) == GH_OK && launches == l0 + 3 && sample_rows.back() == 300 - 2 * SMP_BATCH);
     CHECK(gh_sample_rows(ctx, P, 300, 262144, r, t) == GH_OK && launches == l0 + 6);
     CHECK(gh_ctx_destroy(ctx) == GH_OK);
     CHECK(bad_launches == 0 && hip_stub_live_bytes() == 0);
