@@ -669,16 +669,16 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
     }
 }
 
-// Joins the chunk states of one output row: a workgroup takes 32 of its dims,
-// its threads the chunks side by side, their outputs on the way before the
-// weights are known.
-template <int HD>
+// Joins the chunk states of one output row: a workgroup takes 4 LN of its
+// dims, its threads the chunks side by side, their outputs on the way before
+// the weights are known.
+template <int HD, int LN>
 __global__ __launch_bounds__(NT) void k_kv8_combine(Att8 a) {
-    constexpr int LN = 8, GR = NT / LN, U = 4;  // float4 lanes, groups that share the chunks, loads in flight
+    constexpr int GR = NT / LN, U = 4;  // groups that share the chunks, loads in flight
     __shared__ float red[8];
     __shared__ __align__(16) f32x4 sum[GR][LN];
-    const size_t slot = blockIdx.x / (HD / 32);
-    const int d4 = blockIdx.x % (HD / 32) * LN;
+    const size_t slot = blockIdx.x / (HD / 4 / LN);
+    const int d4 = blockIdx.x % (HD / 4 / LN) * LN;
     const float* pm = a.part + slot * a.ns;
     const float* pl = a.part + (a.rows + slot) * a.ns;
     const f32x4* po = (const f32x4*)(a.part + 2 * a.rows * a.ns + slot * a.ns * HD) + d4;
@@ -716,12 +716,12 @@ __global__ __launch_bounds__(NT) void k_kv8_combine(Att8 a) {
         if (pm[j] != -INFINITY) acc += po[(size_t)j * (HD / 4) + ln] * weight(pm[j]);
     sum[gr][ln] = acc;
     __syncthreads();
-    if (tid < 32) {
+    if (tid < 4 * LN) {
         const float* t = (const float*)sum;
         const float L = (red[4] + red[5]) + (red[6] + red[7]);
         float r = 0.0f;
 #pragma unroll
-        for (int j = 0; j < GR; ++j) r += t[j * 32 + tid];
+        for (int j = 0; j < GR; ++j) r += t[j * 4 * LN + tid];
         a.out[slot * HD + 4 * d4 + tid] = r * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
     }
 }
@@ -765,7 +765,10 @@ int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, cons
         if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value, Narrow>), dim3(a.ns, c.nkv, n), dim3(64 * Narrow::WAVES), 0, s, c, b, a);
         else if (a.tiles == 1) hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<true>>), dim3(a.ns * c.nkv, 1, n), dim3(64 * Wide<true>::WAVES), 0, s, c, b, a);
         else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<false>>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide<false>::WAVES), 0, s, c, b, a);
-        if (a.ns > 1) hipLaunchKernelGGL(k_kv8_combine<h.value>, dim3(a.rows * (h.value / 32)), dim3(NT), 0, s, a);
+        // few chunks: a row a workgroup (of 64 rows or more, so that they fill the device)
+        constexpr int LN = h.value / 4;
+        if (a.ns > 1 && (a.ns > 4 * (NT / LN) || a.rows < 64)) hipLaunchKernelGGL((k_kv8_combine<h.value, 8>), dim3(a.rows * (h.value / 32)), dim3(NT), 0, s, a);
+        else if (a.ns > 1) hipLaunchKernelGGL((k_kv8_combine<h.value, LN>), dim3(a.rows), dim3(NT), 0, s, a);
     });
 }
 
