@@ -148,12 +148,11 @@ struct Stat {
     float own;  // the largest of the elements that this thread read
 };
 
-// f(index, logit) of the elements [i0, i1): 16-byte loads, two in flight a
+// f(index, logit) of the elements [i0, i1): 16-byte loads, U in flight a
 // thread, between the first and last 16-byte boundary (l is aligned to 4).
-template <int NT, class F>
+template <int NT, int U, class F>
 __device__ __forceinline__ void each_logit(const float* l, int i0, int i1, F&& f) {
     typedef float f32x4 __attribute__((ext_vector_type(4)));
-    constexpr int U = 2;
     const int tid = threadIdx.x;
     const int head = min((int)(-((uintptr_t)(l + i0) >> 2) & 3), i1 - i0), quads = (i1 - i0 - head) / 4;
     const int tail = i1 - i0 - head - 4 * quads;
@@ -181,7 +180,7 @@ __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small
     float best = -INFINITY, low = INFINITY;
     int at = -1;
     bool nan = false;
-    each_logit<NT>(l, i0, i1, [&](int i, float v) {
+    each_logit<NT, 4>(l, i0, i1, [&](int i, float v) {
         nan |= v != v;
         if (v > best || (v == best && i < at)) best = v, at = i;
         low = fminf(low, v > -INFINITY ? v : INFINITY);
@@ -239,7 +238,7 @@ template <int NT>
 __device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const Weights& w, const Bins& bins, bool counts,
                                            BinSums& h) {
     clear_bins<NT>(h);
-    each_logit<NT>(l, i0, i1, [&](int, float v) {
+    each_logit<NT, 2>(l, i0, i1, [&](int, float v) {
         if (!bins.in_reach(v)) return;
         const u64 m = w.fixed(v);
         const int b = bins.of(v);
@@ -280,6 +279,31 @@ __device__ __forceinline__ void scan_bins(BinSums& h, Small& sh) {
         h.mass[b0 + j] = run;
         h.count[b0 + j] = crun;
     }
+    __syncthreads();
+}
+
+// The counts alone.
+template <int NT>
+__device__ __forceinline__ void scan_counts(BinSums& h, Small& sh) {
+    constexpr int PER = SMP_BINS / NT;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b0 = threadIdx.x * PER;
+    unsigned c[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += c[j] = h.count[b0 + j];
+    unsigned run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned a = __shfl_up(run, o, 64);
+        if (lane >= o) run += a;
+    }
+    if (lane == 63) sh.red32[w] = run;
+    __syncthreads();
+    run -= sum;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i)
+        if (i < w) run += sh.red32[i];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) h.count[b0 + j] = run += c[j];
     __syncthreads();
 }
 
@@ -357,26 +381,45 @@ __device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins,
     return q;
 }
 
-// To the list: the elements of the bins [lo, hi] that `in` takes.
+// To the list, n elements of it taken: the elements of the bins [lo, hi] that
+// `in` takes.  They meet in LDS (`near`, SMP_BINS of them; sh.n_list 0 before)
+// and go out together: an atomic on the row's own counter for each would hold
+// its wave for a round trip.
 template <int NT, class In>
 __device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, int lo, int hi, u64* list,
-                                             unsigned* n, In&& in) {
-    each_logit<NT>(l, i0, i1, [&](int i, float v) {
+                                             unsigned* n, u64* near, Small& sh, In&& in) {
+    const float from = (float)lo, to = hi < SMP_BINS - 1 ? (float)(hi + 1) : INFINITY;
+    each_logit<NT, 4>(l, i0, i1, [&](int i, float v) {
+        // most elements are none of them, and are known by one product
+        const float t = (bins.top - v) * bins.scale;
+        if (t < from || t >= to) return;
         if (!bins.in_reach(v)) return;
         const int b = bins.of(v);
         if (b < lo || b > hi || !in(b)) return;
-        const unsigned at = atomicAdd(n, 1u);
-        if (at < SMP_LIST) list[at] = rank_key(v, i);
+        unsigned at = atomicAdd(&sh.n_list, 1u);
+        if (at < SMP_BINS) {
+            near[at] = rank_key(v, i);
+        } else {
+            at = atomicAdd(n, 1u);
+            if (at < SMP_LIST) list[at] = rank_key(v, i);
+        }
     });
+    __syncthreads();
+    const unsigned count = min(sh.n_list, (unsigned)SMP_BINS);
+    if (threadIdx.x == 0 && count) sh.bin[7] = (int)atomicAdd(n, count);
+    __syncthreads();
+    const unsigned first = sh.bin[7];
+    for (unsigned i = threadIdx.x; i < count; i += NT)
+        if (first + i < SMP_LIST) list[first + i] = near[i];
 }
 template <int NT>
 __device__ __forceinline__ void range_gather(const float* l, int i0, int i1, const Bins& bins, const SmpCuts& q, u64* list,
-                                             unsigned* n) {
+                                             unsigned* n, u64* near, Small& sh) {
     int lo = SMP_BINS, hi = -1;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (q.lo[j] <= q.hi[j]) lo = min(lo, q.lo[j]), hi = max(hi, q.hi[j]);
-    range_gather<NT>(l, i0, i1, bins, lo, hi, list, n, [&](int b) {
+    range_gather<NT>(l, i0, i1, bins, lo, hi, list, n, near, sh, [&](int b) {
         bool in = false;
 #pragma unroll
         for (int j = 0; j < 4; ++j) in |= b >= q.lo[j] && b <= q.hi[j];
@@ -400,16 +443,18 @@ __device__ __forceinline__ Short short_row(const float* group_max, int groups, c
     const bool k = rule.top_k > 0 && rule.top_k <= groups / 2;
     const bool m = rule.min_p > 0.0f && (rule.top_p >= 1.0f || rule.top_k == 0);
     if (!k && !m) return {-1, false};
-    clear_bins<NT>(h);
+    for (int b = threadIdx.x; b < SMP_BINS; b += NT) h.count[b] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < groups; i += NT) {
         const float v = group_max[i];
         if (v > -INFINITY && bins.in_reach(v)) atomicAdd(&h.count[bins.of(v)], 1u);
     }
     __syncthreads();
-    scan_bins<NT>(h, sh);
+    scan_counts<NT>(h, sh);
     int last = SMP_BINS - 1;
     if (k && h.count[SMP_BINS - 1] >= (unsigned)rule.top_k) {
-        find_bin<NT>(0, h, sh, [&](u64, unsigned c) { return c >= (unsigned)rule.top_k; });
+        for (int b = threadIdx.x; b < SMP_BINS; b += NT)
+            if (h.count[b] >= (unsigned)rule.top_k && (b == 0 || h.count[b - 1] < (unsigned)rule.top_k)) sh.bin[0] = b;
         __syncthreads();
         last = sh.bin[0];
     }
@@ -423,7 +468,7 @@ __device__ __forceinline__ Short short_row(const float* group_max, int groups, c
 template <int NT>
 __device__ __forceinline__ u64 range_mass(const float* l, int i0, int i1, const Weights& w, const Bins& bins, Small& sh) {
     u64 sum = 0;
-    each_logit<NT>(l, i0, i1, [&](int, float v) {
+    each_logit<NT, 2>(l, i0, i1, [&](int, float v) {
         if (bins.in_reach(v)) sum += w.fixed(v);
     });
     return block_reduce<NT>(sum, sh, [](u64 a, u64 b) { return a + b; });
@@ -692,7 +737,7 @@ __device__ void find(const float* l, int n, const Weights& w, unsigned k, double
         if (tid < 256) sh.mass[tid] = 0, sh.count[tid] = 0;
         __syncthreads();
         const u64 prefix = sh.key;
-        each_logit<PT>(l, 0, n, [&](int i, float v) {
+        each_logit<PT, 2>(l, 0, n, [&](int i, float v) {
             const u64 key = rank_key(v, i);
             if (shift < 56 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
             const int d = (int)(key >> shift) & 255;
@@ -724,7 +769,7 @@ __device__ void find(const float* l, int n, const Weights& w, unsigned k, double
 
 __device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, const gh_sampling& rule, SlowShared& sh, Small& red) {
     u64 total = 0, at_least = 0;
-    each_logit<PT>(l, 0, n, [&](int, float v) {
+    each_logit<PT, 2>(l, 0, n, [&](int, float v) {
         const u64 m = w.fixed(v);
         total += m;
         if (w.real(v) >= (double)rule.min_p) at_least += m;
@@ -767,6 +812,8 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
         SlowShared slow;
         float group_max[PT];
     } u;
+    __shared__ u64 near[SMP_BINS];
+    __shared__ unsigned listed_row;
     const gh_sampling rule = rules.r[blockIdx.x];
     const float* l = logits + (size_t)blockIdx.x * n;
     const int tid = threadIdx.x;
@@ -778,21 +825,21 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
     const Weights w = weights_of(s, rule, bits);
     const Bins bins = bins_of(s, w);
     u.group_max[tid] = s.own;
-    if (tid == 0) sh.n_list = 0;
+    if (tid == 0) sh.n_list = listed_row = 0;
     __syncthreads();
     const Short row = short_row<PT>(u.group_max, PT, w, bins, rule, h, sh);
     SmpCuts cuts;
     const bool is_short = row.last >= 0;
     if (is_short) {
         cuts = short_cuts(rule, row.all ? range_mass<PT>(l, 0, n, w, bins, sh) : 0);
-        range_gather<PT>(l, 0, n, bins, 0, row.last, u.p.list, &sh.n_list, [](int) { return true; });
+        range_gather<PT>(l, 0, n, bins, 0, row.last, u.p.list, &listed_row, near, sh, [](int) { return true; });
     } else {
         range_hist<PT>(l, 0, n, w, bins, rule.top_k > 0, h);
         cuts = find_cuts<PT>(w, bins, rule, h, sh);
-        range_gather<PT>(l, 0, n, bins, cuts, u.p.list, &sh.n_list);
+        range_gather<PT>(l, 0, n, bins, cuts, u.p.list, &listed_row, near, sh);
     }
     __syncthreads();
-    const unsigned listed = sh.n_list;
+    const unsigned listed = listed_row;
     const u64* mass = is_short ? nullptr : h.mass;
     int t;
     if (listed <= 64) {
@@ -859,13 +906,15 @@ __global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int
     const float* l = logits + (size_t)blockIdx.y * n;
     const int i0 = chunk_begin(n, c, chunks), i1 = chunk_begin(n, c + 1, chunks);
     const Short row = short_row<CT>(r.group_max, groups, w, bins, rule, h, sh);
+    if (tid == 0) sh.n_list = 0;
     if (c == 0 && tid == 0) r.is_short = row.last < 0 ? 0 : row.all ? 2 : 1;
     if (row.last >= 0) {
         if (row.all) {
             const u64 sum = range_mass<CT>(l, i0, i1, w, bins, sh);
             if (tid == 0) atomicAdd(&r.mass[0], sum);
         }
-        range_gather<CT>(l, i0, i1, bins, 0, row.last, r.list, &r.n_list, [](int) { return true; });
+        __syncthreads();
+        range_gather<CT>(l, i0, i1, bins, 0, row.last, r.list, &r.n_list, h.mass, sh, [](int) { return true; });
         return;
     }
     range_hist<CT>(l, i0, i1, w, bins, rule.top_k > 0, h);
@@ -892,8 +941,10 @@ __global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, i
         for (int b = tid; b < SMP_BINS; b += CT) r.run_mass[b] = h.mass[b], r.run_count[b] = h.count[b];
         if (tid == 0) r.cuts = cuts;
     }
+    if (tid == 0) sh.n_list = 0;
+    __syncthreads();
     range_gather<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
-                     r.list, &r.n_list);
+                     r.list, &r.n_list, h.mass, sh);
 }
 
 __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int bits, SmpRules rules, const SmpRow* rows,
