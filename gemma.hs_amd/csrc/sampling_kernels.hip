@@ -28,6 +28,7 @@ namespace gh {
 namespace {
 
 typedef unsigned long long u64;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // Ascending in rank order: value descending, then index ascending.
 __device__ __forceinline__ uint32_t value_key(float v) {
@@ -42,28 +43,30 @@ __device__ __forceinline__ u64 rank_key(float v, int i) { return ((u64)value_key
 // A row's weights exp((l - max) / T), as integers of `bits` fractional bits:
 // their sums do not depend on the order, and are exact to 2^-bits a weight.
 // In 64 bits because a draw compares sums over the whole vocabulary.
-// 2^y = 2^k 2^f with |f| <= 1/2 and the series of exp(f ln 2) up to f^12,
-// whose first term left out is below 2^-52.
+// 2^y = 2^k 2^f with |f| <= 1/2 and the series of exp(f ln 2) up to f^11, whose
+// first term left out is below 2^-47; the sums' own steps are 2^-44 for 262144
+// logits.  An infinite largest logit counts as 0, whose equals give y = inf,
+// taken as 0; none of the others is asked for.
 struct Weights {
     float top;
+    double base;     // top, or 0 for an infinite one
     double log2e_t;  // log2(e) / T
     int bits;        // at most 51
+    // (l - top) log2(e) / T must be above -1000
     __device__ __forceinline__ double scaled(float l, int e) const {
-        if (l == top) return ldexp(1.0, e);  // an infinite one among them
-        const double y = fmax(((double)l - (double)top) * log2e_t, -1000.0);
-        const double k = rint(y), f = (y - k) * 0.693147180559945309417;
-        double p = 1.0 / 479001600;
-        p = fma(p, f, 1.0 / 39916800);
-        p = fma(p, f, 1.0 / 3628800);
-        p = fma(p, f, 1.0 / 362880);
-        p = fma(p, f, 1.0 / 40320);
-        p = fma(p, f, 1.0 / 5040);
-        p = fma(p, f, 1.0 / 720);
-        p = fma(p, f, 1.0 / 120);
-        p = fma(p, f, 1.0 / 24);
-        p = fma(p, f, 1.0 / 6);
-        p = fma(p, f, 0.5);
-        p = fma(p, f, 1.0);
+        constexpr double L = 0.693147180559945309417, L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
+        const double y = fmin(((double)l - base) * log2e_t, 0.0), k = rint(y), f = y - k;
+        double p = L8 * L2 * L / 39916800;
+        p = fma(p, f, L8 * L2 / 3628800);
+        p = fma(p, f, L8 * L / 362880);
+        p = fma(p, f, L8 / 40320);
+        p = fma(p, f, L4 * L2 * L / 5040);
+        p = fma(p, f, L4 * L2 / 720);
+        p = fma(p, f, L4 * L / 120);
+        p = fma(p, f, L4 / 24);
+        p = fma(p, f, L2 * L / 6);
+        p = fma(p, f, L2 / 2);
+        p = fma(p, f, L);
         p = fma(p, f, 1.0);
         return ldexp(p, (int)k + e);
     }
@@ -75,13 +78,12 @@ struct Weights {
 };
 
 // What the bins are: equal steps of top - l up to `reach`, behind which every
-// weight is zero.  Monotonic in l, so that bins follow the ranks.
+// weight is zero.  Monotonic in l, so that bins follow the ranks.  (An infinite
+// top and its equals: a NaN, which is in reach and becomes bin 0.)
 struct Bins {
     float top, scale, reach;
-    __device__ __forceinline__ bool in_reach(float l) const { return l == top || top - l <= reach; }
-    __device__ __forceinline__ int of(float l) const {
-        return l == top ? 0 : (int)fminf((top - l) * scale, (float)(SMP_BINS - 1));
-    }
+    __device__ __forceinline__ bool in_reach(float l) const { return !(top - l > reach); }
+    __device__ __forceinline__ int of(float l) const { return min((int)((top - l) * scale), SMP_BINS - 1); }
 };
 
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int o) {
@@ -148,43 +150,82 @@ struct Stat {
     float own;  // the largest of the elements that this thread read
 };
 
-// f(index, logit) of the elements [i0, i1): 16-byte loads, U in flight a
-// thread, between the first and last 16-byte boundary (l is aligned to 4).
+// The elements [i0, i1) of a row (l is aligned to 4) as 16-byte quads between
+// the first and the last 16-byte boundary, and up to 6 elements at the edges.
+struct Quads {
+    const f32x4* p;
+    int first, quads, i0, head, i1, tail;
+    __device__ __forceinline__ Quads(const float* l, int i0, int i1) : i0(i0), i1(i1) {
+        head = min((int)(-((uintptr_t)(l + i0) >> 2) & 3), i1 - i0);
+        first = i0 + head;
+        quads = (i1 - first) / 4;
+        tail = i1 - first - 4 * quads;
+        p = (const f32x4*)(l + first);
+    }
+    // index of the thread's element at the edges, or -1
+    __device__ __forceinline__ int edge(int tid) const {
+        return tid < head ? i0 + tid : tid < head + tail ? i1 - tail + tid - head : -1;
+    }
+};
+
+// f(index, logit) of the elements [i0, i1), U loads in flight a thread
 template <int NT, int U, class F>
 __device__ __forceinline__ void each_logit(const float* l, int i0, int i1, F&& f) {
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-    const int tid = threadIdx.x;
-    const int head = min((int)(-((uintptr_t)(l + i0) >> 2) & 3), i1 - i0), quads = (i1 - i0 - head) / 4;
-    const int tail = i1 - i0 - head - 4 * quads;
-    const f32x4* p = (const f32x4*)(l + i0 + head);
+    const Quads r(l, i0, i1);
 #pragma unroll 1
-    for (int q = tid; q < quads; q += U * NT) {
+    for (int q = threadIdx.x; q < r.quads; q += U * NT) {
         f32x4 v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) v[j] = p[min(q + j * NT, quads - 1)];
+        for (int j = 0; j < U; ++j) v[j] = r.p[min(q + j * NT, r.quads - 1)];
 #pragma unroll
         for (int j = 0; j < U; ++j)
-            if (q + j * NT < quads) {
+            if (q + j * NT < r.quads) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f(i0 + head + 4 * (q + j * NT) + e, v[j][e]);
+                for (int e = 0; e < 4; ++e) f(r.first + 4 * (q + j * NT) + e, v[j][e]);
             }
     }
-    if (tid < head + tail) {
-        const int i = tid < head ? i0 + tid : i1 - tail + tid - head;
-        f(i, l[i]);
-    }
+    if (const int i = r.edge(threadIdx.x); i >= 0) f(i, l[i]);
 }
 
 template <int NT>
 __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small& sh) {
+    constexpr int U = 4;
+    const Quads r(l, i0, i1);
     float best = -INFINITY, low = INFINITY;
-    int at = -1;
+    int at = -1;  // index of the best, or of the first of its quad
     bool nan = false;
-    each_logit<NT, 4>(l, i0, i1, [&](int i, float v) {
+    auto one = [&](int i, float v) {
         nan |= v != v;
         if (v > best || (v == best && i < at)) best = v, at = i;
         low = fminf(low, v > -INFINITY ? v : INFINITY);
-    });
+    };
+#pragma unroll 1
+    for (int q = threadIdx.x; q < r.quads; q += U * NT) {
+        f32x4 v[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j] = r.p[min(q + j * NT, r.quads - 1)];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            // The last quad may come more than once: not for `best`, which is
+            // also the largest of this thread's elements alone.  A thread's
+            // quads ascend, so that the first of equal ones stays.
+            const float hi = q + j * NT < r.quads ? fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)) : -INFINITY;
+            float lo = fminf(fminf(v[j].x, v[j].y), fminf(v[j].z, v[j].w));
+            nan |= __builtin_isunordered(v[j].x, v[j].y) | __builtin_isunordered(v[j].z, v[j].w);
+            if (hi > best) best = hi, at = r.first + 4 * (q + j * NT);
+            if (lo == -INFINITY) {
+                lo = INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) lo = fminf(lo, v[j][e] > -INFINITY ? v[j][e] : INFINITY);
+            }
+            low = fminf(low, lo);
+        }
+    }
+    if (at >= 0) {  // which of the quad
+        const f32x4 v = r.p[(at - r.first) / 4];
+        at += v.x == best ? 0 : v.y == best ? 1 : v.z == best ? 2 : 3;
+    }
+    if (const int i = r.edge(threadIdx.x); i >= 0) one(i, l[i]);
     u64 first = at >= 0 ? rank_key(best, at) : ~0ull;
     unsigned bad = __any(nan);
 #pragma unroll
@@ -215,7 +256,8 @@ __device__ __forceinline__ bool drawn(const Stat& s, const gh_sampling& rule) {
 __device__ __forceinline__ int token_of_undrawn(const Stat& s) { return s.nan || s.first == ~0ull ? -1 : (int)(unsigned)s.first; }
 
 __device__ __forceinline__ Weights weights_of(const Stat& s, const gh_sampling& rule, int bits) {
-    return {key_value((unsigned)(s.first >> 32)), 1.44269504088896340736 / (double)rule.temperature, bits};
+    const float top = key_value((unsigned)(s.first >> 32));
+    return {top, top == INFINITY ? 0.0 : (double)top, 1.44269504088896340736 / (double)rule.temperature, bits};
 }
 
 __device__ __forceinline__ Bins bins_of(const Stat& s, const Weights& w) {
@@ -253,73 +295,62 @@ __device__ __forceinline__ void range_hist(const float* l, int i0, int i1, const
 // ------------------------------------------------------------------
 // step 3: where the searches end, from the bins alone
 // ------------------------------------------------------------------
-// Sums per bin become running sums.
+// Running sums over the bins, a thread's own ones in its registers: m[j], c[j]
+// in front of bin b0 + j.
 template <int NT>
-__device__ __forceinline__ void scan_bins(BinSums& h, Small& sh) {
-    constexpr int PER = SMP_BINS / NT;
-    const int b0 = threadIdx.x * PER;
-    u64 m[PER], sum = 0;
-    unsigned c[PER], csum = 0;
+struct Running {
+    static constexpr int PER = SMP_BINS / NT;
+    u64 m[PER + 1];
+    unsigned c[PER + 1];
+    int b0;
+    __device__ __forceinline__ Running(const u64* mass, const unsigned* count, Small& sh) : b0(threadIdx.x * PER) {
+        u64 sum = 0;
+        unsigned csum = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        m[j] = h.mass[b0 + j];
-        c[j] = h.count[b0 + j];
-        sum += m[j];
-        csum += c[j];
+        for (int j = 0; j < PER; ++j) {
+            m[j + 1] = mass[b0 + j];
+            c[j + 1] = count[b0 + j];
+            sum += m[j + 1];
+            csum += c[j + 1];
+        }
+        u64 run = sum;
+        unsigned crun = csum;
+        block_scan<NT>(run, crun, sh);
+        m[0] = run - sum;
+        c[0] = crun - csum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) m[j + 1] += m[j], c[j + 1] += c[j];
+        if (threadIdx.x == NT - 1) sh.upto[7] = m[PER], sh.bin[6] = (int)c[PER];  // of all
     }
-    u64 run = sum;
-    unsigned crun = csum;
-    block_scan<NT>(run, crun, sh);
-    run -= sum;
-    crun -= csum;
+    // The bin in which a running sum first satisfies `reached` (false for 0):
+    // slot i of sh.
+    template <class P>
+    __device__ __forceinline__ void find(int i, Small& sh, P&& reached) const {
+        bool there = reached(m[0], c[0]);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        run += m[j];
-        crun += c[j];
-        h.mass[b0 + j] = run;
-        h.count[b0 + j] = crun;
-    }
-    __syncthreads();
-}
-
-// The counts alone.
-template <int NT>
-__device__ __forceinline__ void scan_counts(BinSums& h, Small& sh) {
-    constexpr int PER = SMP_BINS / NT;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b0 = threadIdx.x * PER;
-    unsigned c[PER], sum = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) sum += c[j] = h.count[b0 + j];
-    unsigned run = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned a = __shfl_up(run, o, 64);
-        if (lane >= o) run += a;
-    }
-    if (lane == 63) sh.red32[w] = run;
-    __syncthreads();
-    run -= sum;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i)
-        if (i < w) run += sh.red32[i];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) h.count[b0 + j] = run += c[j];
-    __syncthreads();
-}
-
-// The bin in which a running sum first satisfies `reached`; slot i of sh.
-template <int NT, class P>
-__device__ __forceinline__ void find_bin(int i, const BinSums& h, Small& sh, P&& reached) {
-    for (int b = threadIdx.x; b < SMP_BINS; b += NT) {
-        const bool here = reached(h.mass[b], h.count[b]);
-        const bool there = b > 0 && reached(h.mass[b - 1], h.count[b - 1]);
-        if (here && !there) {
-            sh.bin[i] = b;
-            sh.before[i] = b > 0 ? h.mass[b - 1] : 0;
-            sh.upto[i] = h.mass[b];
+        for (int j = 0; j < PER; ++j) {
+            const bool here = reached(m[j + 1], c[j + 1]);
+            if (here && !there) put(i, j, sh);
+            there = here;
         }
     }
-}
+    __device__ __forceinline__ void put(int i, int j, Small& sh) const {
+        sh.bin[i] = b0 + j;
+        sh.before[i] = m[j];
+        sh.upto[i] = m[j + 1];
+    }
+    // bin b as slot i
+    __device__ __forceinline__ void look(int i, int b, Small& sh) const {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (b0 + j == b) put(i, j, sh);
+    }
+    // the sums up to and with each bin
+    __device__ __forceinline__ void store(u64* mass, unsigned* count) const {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) mass[b0 + j] = m[j + 1], count[b0 + j] = c[j + 1];
+    }
+};
 
 // Where in the bins a weight falls below min_p, to be taken with a bin to
 // either side for roundings.
@@ -327,57 +358,60 @@ __device__ __forceinline__ double min_p_bin(const Weights& w, const Bins& bins, 
     return (double)-log2f(rule.min_p) / w.log2e_t * (double)bins.scale;
 }
 
-// h: per bin; running afterwards.
 template <int NT>
-__device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins, const gh_sampling& rule, BinSums& h, Small& sh) {
-    scan_bins<NT>(h, sh);
+__device__ __forceinline__ SmpCuts find_cuts(const Weights& w, const Bins& bins, const gh_sampling& rule, const Running<NT>& run,
+                                             Small& sh) {
+    __syncthreads();
     SmpCuts q;
-    q.total = h.mass[SMP_BINS - 1];
+    q.total = sh.upto[7];
     // what is behind the last element with a weight cannot be drawn: a top_k
     // that reaches there leaves all the mass
-    q.k = rule.top_k > 0 && (unsigned)rule.top_k < h.count[SMP_BINS - 1];
+    q.k = rule.top_k > 0 && rule.top_k < sh.bin[6];
     q.p = rule.top_p < 1.0f;
-    q.m = rule.min_p > 0.0f;
+    const double d = rule.min_p > 0.0f ? min_p_bin(w, bins, rule) : SMP_BINS + 1;
+    q.m = d < SMP_BINS + 1;  // else every weight reaches it
     for (int i = 0; i < 4; ++i) q.lo[i] = 1, q.hi[i] = 0;
-    u64 zlo = q.total, zhi = q.total;  // mass that top_k leaves
     if (q.k) {
         const unsigned k = rule.top_k;
-        find_bin<NT>(0, h, sh, [&](u64, unsigned c) { return c >= k; });
-        __syncthreads();
+        run.find(0, sh, [&](u64, unsigned c) { return c >= k; });
+    }
+    if (q.m) {
+        q.lo[2] = max((int)d - 1, 0);
+        q.hi[2] = min((int)d + 1, SMP_BINS - 1);
+        run.look(1, q.lo[2], sh);
+        run.look(2, q.hi[2], sh);
+    }
+    if (q.k || q.m) __syncthreads();
+    u64 zlo = q.total, zhi = q.total;  // mass that top_k leaves
+    if (q.k) {
         q.lo[0] = q.hi[0] = sh.bin[0];
         zlo = sh.before[0];
         zhi = sh.upto[0];
     }
     u64 lo = zlo, hi = zhi;  // mass that all three leave
-    if (q.p) {
-        const double tlo = (double)rule.top_p * (double)zlo, thi = (double)rule.top_p * (double)zhi;
-        find_bin<NT>(1, h, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= tlo; });
-        find_bin<NT>(2, h, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= thi; });
-        __syncthreads();
-        q.lo[1] = sh.bin[1];
-        q.hi[1] = sh.bin[2];
-        lo = min(lo, sh.before[1]);
-        hi = min(hi, sh.upto[2]);
-    }
     q.upto_m = q.total;
     if (q.m) {
-        const double d = min_p_bin(w, bins, rule);
-        q.m = d < SMP_BINS + 1;  // else every weight reaches it
-        if (q.m) {
-            const int b = (int)d;
-            q.lo[2] = max(b - 1, 0);
-            q.hi[2] = min(b + 1, SMP_BINS - 1);
-            q.upto_m = h.mass[q.hi[2]];
-            lo = min(lo, q.lo[2] > 0 ? h.mass[q.lo[2] - 1] : 0);
-            hi = min(hi, q.upto_m);
-        }
+        q.upto_m = sh.upto[2];
+        lo = min(lo, sh.before[1]);
+        hi = min(hi, q.upto_m);
+    }
+    if (q.p) {
+        const double tlo = (double)rule.top_p * (double)zlo, thi = (double)rule.top_p * (double)zhi;
+        run.find(3, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= tlo; });
+        run.find(4, sh, [&](u64 m, unsigned) { return m > 0 && (double)m >= thi; });
+        __syncthreads();
+        q.lo[1] = sh.bin[3];
+        q.hi[1] = sh.bin[4];
+        lo = min(lo, sh.before[3]);
+        hi = min(hi, sh.upto[4]);
     }
     const double ulo = (double)rule.u * (double)lo, uhi = (double)rule.u * (double)hi;
-    find_bin<NT>(3, h, sh, [&](u64 m, unsigned) { return (double)m > ulo; });
-    find_bin<NT>(4, h, sh, [&](u64 m, unsigned) { return (double)m > uhi; });
+    run.find(5, sh, [&](u64 m, unsigned) { return (double)m > ulo; });
+    run.find(7, sh, [&](u64 m, unsigned) { return (double)m > uhi; });
     __syncthreads();
-    q.lo[3] = sh.bin[3];
-    q.hi[3] = sh.bin[4];
+    q.lo[3] = sh.bin[5];
+    q.hi[3] = sh.bin[7];
+    __syncthreads();
     return q;
 }
 
@@ -427,6 +461,31 @@ __device__ __forceinline__ void range_gather(const float* l, int i0, int i1, con
     });
 }
 
+// Counts per bin become running counts.
+template <int NT>
+__device__ __forceinline__ void scan_counts(unsigned* count, Small& sh) {
+    constexpr int PER = SMP_BINS / NT;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, b0 = threadIdx.x * PER;
+    unsigned c[PER], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += c[j] = count[b0 + j];
+    unsigned run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned a = __shfl_up(run, o, 64);
+        if (lane >= o) run += a;
+    }
+    if (lane == 63) sh.red32[w] = run;
+    __syncthreads();
+    run -= sum;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i)
+        if (i < w) run += sh.red32[i];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) count[b0 + j] = run += c[j];
+    __syncthreads();
+}
+
 // A short row: the last bin of the elements that its list needs (-1: a long
 // row), and whether top_p needs the mass of all (the list has what top_k
 // leaves).  top_k: the bin in which the groups' largest come to top_k; where
@@ -450,7 +509,7 @@ __device__ __forceinline__ Short short_row(const float* group_max, int groups, c
         if (v > -INFINITY && bins.in_reach(v)) atomicAdd(&h.count[bins.of(v)], 1u);
     }
     __syncthreads();
-    scan_counts<NT>(h, sh);
+    scan_counts<NT>(h.count, sh);
     int last = SMP_BINS - 1;
     if (k && h.count[SMP_BINS - 1] >= (unsigned)rule.top_k) {
         for (int b = threadIdx.x; b < SMP_BINS; b += NT)
@@ -728,7 +787,7 @@ struct SlowShared {
 // key, from the counts and masses of the 256 values of each digit among the
 // elements that share the digits before.  The mass up to and with it goes to
 // sh.base_mass, its key to sh.key.
-__device__ void find(const float* l, int n, const Weights& w, unsigned k, double t, bool strict, SlowShared& sh) {
+__device__ void find(const float* l, int n, const Weights& w, const Bins& bins, unsigned k, double t, bool strict, SlowShared& sh) {
     const int tid = threadIdx.x;
     __syncthreads();
     if (tid == 0) sh.key = sh.base_mass = 0, sh.base_count = 0;
@@ -742,7 +801,7 @@ __device__ void find(const float* l, int n, const Weights& w, unsigned k, double
             if (shift < 56 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
             const int d = (int)(key >> shift) & 255;
             atomicAdd(&sh.count[d], 1u);
-            const u64 m = w.fixed(v);
+            const u64 m = bins.in_reach(v) ? w.fixed(v) : 0;
             if (m) atomicAdd(&sh.mass[d], m);
         });
         __syncthreads();
@@ -763,13 +822,14 @@ __device__ void find(const float* l, int n, const Weights& w, unsigned k, double
         }
         __syncthreads();
     }
-    if (tid == 0) sh.base_mass += w.fixed(l[(unsigned)sh.key]);
+    if (tid == 0 && bins.in_reach(l[(unsigned)sh.key])) sh.base_mass += w.fixed(l[(unsigned)sh.key]);
     __syncthreads();
 }
 
-__device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, const gh_sampling& rule, SlowShared& sh, Small& red) {
+__device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, const Bins& bins, const gh_sampling& rule, SlowShared& sh, Small& red) {
     u64 total = 0, at_least = 0;
     each_logit<PT, 2>(l, 0, n, [&](int, float v) {
+        if (!bins.in_reach(v)) return;
         const u64 m = w.fixed(v);
         total += m;
         if (w.real(v) >= (double)rule.min_p) at_least += m;
@@ -778,15 +838,15 @@ __device__ __noinline__ int slow_row(const float* l, int n, const Weights& w, co
     total = block_reduce<PT>(total, red, plus);
     at_least = block_reduce<PT>(at_least, red, plus);
     if (rule.top_k > 0 && rule.top_k < n) {
-        find(l, n, w, rule.top_k, 0.0, false, sh);
+        find(l, n, w, bins, rule.top_k, 0.0, false, sh);
         total = sh.base_mass;
     }
     u64 kept = min(total, at_least);
     if (rule.top_p < 1.0f) {
-        find(l, n, w, 0, (double)rule.top_p * (double)total, false, sh);
+        find(l, n, w, bins, 0, (double)rule.top_p * (double)total, false, sh);
         kept = min(kept, sh.base_mass);
     }
-    find(l, n, w, 0, (double)rule.u * (double)kept, true, sh);
+    find(l, n, w, bins, 0, (double)rule.u * (double)kept, true, sh);
     return (int)(unsigned)sh.key;
 }
 
@@ -835,7 +895,9 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
         range_gather<PT>(l, 0, n, bins, 0, row.last, u.p.list, &listed_row, near, sh, [](int) { return true; });
     } else {
         range_hist<PT>(l, 0, n, w, bins, rule.top_k > 0, h);
-        cuts = find_cuts<PT>(w, bins, rule, h, sh);
+        const Running<PT> run(h.mass, h.count, sh);
+        cuts = find_cuts<PT>(w, bins, rule, run, sh);
+        run.store(h.mass, h.count);
         range_gather<PT>(l, 0, n, bins, cuts, u.p.list, &listed_row, near, sh);
     }
     __syncthreads();
@@ -850,7 +912,7 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
         t = listed <= PT ? pick<1>(w, bins, rule, cuts, mass, h.count, listed, u.p, sh)
                          : pick<SMP_LIST / PT>(w, bins, rule, cuts, mass, h.count, listed, u.p, sh);
     } else {
-        t = slow_row(l, n, w, rule, u.slow, sh);
+        t = slow_row(l, n, w, bins, rule, u.slow, sh);
     }
     if (tid == 0) tokens[blockIdx.x] = t;
 }
@@ -926,7 +988,7 @@ __global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int
 
 __global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, int bits, SmpRules rules, SmpRow* rows) {
     __shared__ Small sh;
-    __shared__ BinSums h;
+    __shared__ u64 near[SMP_BINS];
     const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
     const gh_sampling rule = rules.r[blockIdx.y];
     SmpRow& r = rows[blockIdx.y];
@@ -934,17 +996,16 @@ __global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, i
     if (!drawn(s, rule) || r.is_short) return;
     const Weights w = weights_of(s, rule, bits);
     const Bins bins = bins_of(s, w);
-    for (int b = tid; b < SMP_BINS; b += CT) h.mass[b] = r.mass[b], h.count[b] = r.count[b];
-    __syncthreads();
-    const SmpCuts cuts = find_cuts<CT>(w, bins, rule, h, sh);
+    const Running<CT> run(r.mass, r.count, sh);
+    const SmpCuts cuts = find_cuts<CT>(w, bins, rule, run, sh);
     if (c == 0) {  // for the last step
-        for (int b = tid; b < SMP_BINS; b += CT) r.run_mass[b] = h.mass[b], r.run_count[b] = h.count[b];
+        run.store(r.run_mass, r.run_count);
         if (tid == 0) r.cuts = cuts;
     }
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
     range_gather<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
-                     r.list, &r.n_list, h.mass, sh);
+                     r.list, &r.n_list, near, sh);
 }
 
 __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int bits, SmpRules rules, const SmpRow* rows,
@@ -980,7 +1041,7 @@ __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int
         t = listed <= PT ? pick<1>(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh)
                          : pick<SMP_LIST / PT>(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh);
     } else {
-        t = slow_row(logits + (size_t)blockIdx.x * n, n, w, rule, u.slow, sh);
+        t = slow_row(logits + (size_t)blockIdx.x * n, n, w, bins, rule, u.slow, sh);
     }
     if (tid == 0) tokens[blockIdx.x] = t;
 }
