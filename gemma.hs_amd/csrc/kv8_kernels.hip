@@ -335,6 +335,12 @@ __device__ __forceinline__ i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
+// a b as a number of its own: not part of a fused addition
+__device__ __forceinline__ float rounded(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 // byte n of four words
 __device__ __forceinline__ uint32_t byte_of(const uint32_t* d, int n) {
     const uint32_t lo = __builtin_amdgcn_perm(d[1], d[0], n == 0 ? 0x0c0c0400u : n == 1 ? 0x0c0c0501u : 0x0c0c0602u);
@@ -388,8 +394,12 @@ struct Narrow {
     // the lane's digit alone; join() adds the row's other two
     __device__ __forceinline__ float scaled(float w) const { return w * weight; }
     __device__ __forceinline__ float sum(const i32x4* acc, int j) const { return (float)acc[0][j]; }
+    // The row's lanes have to get the same sum to the last bit, since each
+    // takes its own digit of the probability that comes of it: additions of
+    // the same values in either order, none fused with the product before.
     __device__ __forceinline__ float join(float v) const {
-        v += dpp<DPP_ROW_ROR8>(v);
+#pragma clang fp contract(off)
+        v = v + dpp<DPP_ROW_ROR8>(v);
         return v + dpp<DPP_ROW_ROR4>(v);
     }
 };
@@ -535,7 +545,7 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.join(col.sum(acc, j) * f);
+            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.join(rounded(col.sum(acc, j), f));
         }
         if (LATE_V) load_v(blk);
         if (!LATE_K && blk + WAVES < blk1) load_k(blk + WAVES);

@@ -380,6 +380,41 @@ def test_sharp_and_flat_scores(ctx):
     _check(c.attention([0], [2], q, 4), ks, vs, q, [2], 0)
 
 
+@pytest.mark.parametrize("nq,hd", [(4, 256), (3, 128), (4, 64), (2, 32), (8, 256)])
+def test_every_digit_of_millions_of_probabilities(ctx, nq, hd):
+    """A probability's digits are taken by different lanes, which have to agree
+    on it to the last bit: where they do not, one in some hundred thousand
+    probabilities is off by 1/128 of its block's largest.  V is 1 at dim
+    token % hd and 0 elsewhere, so that the output is sums of few
+    probabilities and shows one.
+
+    Bound for output d: a score's error changes every term by a factor of
+    2 ds; rounding p to its digits costs half a 2^-23rd of the block's
+    largest for each of the 64 / hd + 1 tokens of a block, and of the sums'
+    roundings each costs 2^-24 of them, 40 in a row at most."""
+    rng = np.random.default_rng(67 + nq + hd)
+    L, n = 20000, 64
+    k, q = rows(rng, L, 1, hd, 1.2), rows(rng, n, nq, hd, 1.5)
+    v = np.zeros((L, 1, hd), F32)
+    v[np.arange(L), 0, np.arange(L) % hd] = 1
+    c = gh.KVCache8(ctx, 1, L, 1, hd)
+    c.append([0], [L], k, v)
+    got = c.attention([0] * n, [1] * n, q, nq).reshape(n * nq, hd)
+    kk, qq = quantise(k)[2][:, 0].astype(np.float64), q.reshape(n * nq, hd).astype(np.float64)
+    s = qq @ kk.T / np.sqrt(hd)
+    p = np.exp(s - s.max(1, keepdims=True))
+    l = p.sum(1, keepdims=True)
+    pad = -L % (64 * hd)
+    pp = np.concatenate([p, np.zeros((n * nq, pad))], 1)
+    want = pp.reshape(n * nq, -1, hd).sum(1) / l
+    eps = 2.0 ** -24
+    ds = eps * (np.abs(kk).sum(1).max() * np.abs(qq).max(1, keepdims=True) / np.sqrt(hd) + 4 * np.abs(s).max(1, keepdims=True))
+    largest = pp.reshape(n * nq, -1, 64).max(2).sum(1, keepdims=True)
+    bound = want * (2 * ds + 40 * eps) + (64 // hd + 1) * eps * largest / l
+    err = np.abs(got - want)
+    assert np.all(err <= bound), (float((err / bound).max()), int((err > bound).sum()))
+
+
 def test_results_do_not_change_from_call_to_call(ctx):
     rng = np.random.default_rng(47)
     lens = [900, 4000, 77]
