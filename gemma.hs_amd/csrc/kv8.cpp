@@ -1,6 +1,6 @@
 // Host side of the 8-bit KV cache: the handle, the checks of its calls and
 // the split of an attention call into workgroups.
-#include <cstring>
+#include <algorithm>
 #include <memory>
 
 #include "host.h"
@@ -13,6 +13,7 @@ namespace {
 constexpr int MAX_SEQ = 1 << 22;   // tokens a sequence
 constexpr int MAX_ROWS = 1 << 20;  // query rows a kv head and sequence
 constexpr int MAX_GROUP = 1024;    // heads a kv head: rows * group stays below 2^32 (Att8::group_inv)
+constexpr int WASTE = 4096;        // empty workgroups that cost about what another launch does
 constexpr int MAX_GRID = 1 << 23;  // workgroups of 256 threads in a grid's x (2^32 threads at most)
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -62,8 +63,126 @@ int kv8_chunk(int hd, int tile, int most, int64_t work, int64_t wgs) {
     return (int)std::max<int64_t>(4, (work + 511) / 512);
 }
 
+// How many of the entries from `at` on one launch takes, their sizes
+// descending: its grid has as many workgroups for each as for the first, so
+// that small ones behind a large one would be passed over in empty workgroups,
+// a microsecond a thousand.  A prompt of 16384 tokens among 239 single ones
+// is appended in 591 us by one launch, in 107 by these.
+// `heads`: workgroups of size 1.
+int launch_end(const int* size, int at, int n, int64_t heads) {
+    int64_t sum = size[at];
+    int end = at + 1;
+    for (; end < n; ++end) {
+        const int64_t grid = (int64_t)size[at] * (end + 1 - at);
+        sum += size[end];
+        if ((grid - sum) * heads > std::max<int64_t>(sum * heads, WASTE)) break;
+    }
+    return end;
+}
+
 int blocks_of(int begin, int end) {  // blocks that [begin, end) touches
     return end > begin ? (end - 1) / KV8_BLOCK - begin / KV8_BLOCK + 1 : 0;
+}
+
+// One entry of an append, a read or an attention.
+struct Entry {
+    int seq, pos, off, cnt;  // as in Kv8Batch
+    int size, blocks;        // of the grid, and (attention) of the keys
+};
+
+void to_batch(const Entry* e, int n, Kv8Batch& b) {
+    int part = 0;
+    for (int i = 0; i < n; ++i) {
+        b.seq[i] = e[i].seq;
+        b.pos[i] = e[i].pos;
+        b.off[i] = e[i].off;
+        b.cnt[i] = e[i].cnt;
+        b.part[i] = part;
+        part += e[i].cnt;
+    }
+}
+
+int most_blocks(const Entry* e, int n) {
+    int most = 0;
+    for (int i = 0; i < n; ++i) most = std::max(most, e[i].size);
+    return most;
+}
+
+// launch(entries, n) of the entries that have tokens, in launches of like sizes.
+template <class F>
+int launch_by_size(Entry* e, int n, int64_t heads, F&& launch) {
+    int size[KV8_BATCH], most = 0;
+    int64_t sum = 0;
+    n = (int)(std::remove_if(e, e + n, [](const Entry& x) { return x.cnt == 0; }) - e);
+    for (int i = 0; i < n; ++i) {
+        most = std::max(most, e[i].size);
+        sum += e[i].size;
+    }
+    const bool one = ((int64_t)most * n - sum) * heads <= std::max<int64_t>(sum * heads, WASTE);
+    if (!one) std::stable_sort(e, e + n, [](const Entry& x, const Entry& y) { return x.size > y.size; });
+    for (int i = 0; i < n; ++i) size[i] = e[i].size;
+    for (int at = 0, end; at < n; at = end) {
+        end = one ? n : launch_end(size, at, n, heads);
+        GH_CHECK(launch(e + at, end - at));
+    }
+    return GH_OK;
+}
+
+// Key blocks that a row tile of the entry may see: up to the window and the
+// tile's own rows.
+int keys_of(const Entry& e, const Att8& a, int tile) {
+    const int span = a.window ? (int)std::min<int64_t>(e.pos, (int64_t)a.window + tile / a.group + 1) : e.pos;
+    return std::min((e.pos + KV8_BLOCK - 1) / KV8_BLOCK, span / KV8_BLOCK + 2);
+}
+
+int tiles_of(const Entry& e, const Att8& a, int tile) { return (e.cnt * a.group + tile - 1) / tile; }
+
+// One launch (and one that joins the chunks) for entries with query tokens.
+int attention_launch(gh_kv8* kv, Entry* e, int n, int tile, Att8 a) {
+    a.tile = tile;
+    int most = 0;               // blocks of the longest row tile
+    int64_t work = 0, wgs = 0;  // blocks of all row tiles, and these
+    for (int i = 0; i < n; ++i) {
+        e[i].blocks = keys_of(e[i], a, tile);
+        most = std::max(most, e[i].blocks);
+        const int t = tiles_of(e[i], a, tile);
+        a.tiles = std::max(a.tiles, t);
+        a.most_q = std::max(a.most_q, e[i].cnt);
+        a.rows += (size_t)e[i].cnt * a.heads;
+        wgs += (int64_t)t * kv->nkv;
+        work += (int64_t)t * kv->nkv * e[i].blocks;
+    }
+    a.chunk = kv8_chunk(kv->hd, tile, most, work, wgs);
+    if ((int64_t)a.most_q * a.heads * (kv->hd / 32) > MAX_GRID) a.chunk = std::max(most, 1);  // nothing to join
+    a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
+    if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
+        return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows in one call", a.most_q * a.group);
+    if (a.ns > 1) {
+        void* part = nullptr;
+        GH_CHECK(ctx_scratch(kv->ctx, a.rows * a.ns * (kv->hd + 2) * sizeof(float), &part));
+        a.part = (float*)part;
+    }
+    // the longest first: their workgroups start before the others'
+    std::stable_sort(e, e + n, [](const Entry& x, const Entry& y) { return x.blocks > y.blocks; });
+    Kv8Batch b;
+    to_batch(e, n, b);
+    return launch_kv8_attention(dev(kv), kv->hd, b, n, a, kv->ctx->stream);
+}
+
+// Entries of up to four query rows a kv head (decoding) have a kernel of their
+// own, but join the others where one row tile holds any of these (drafts): 64
+// sequences of 4096 tokens, half of them with drafts of 4, take 97 us joined
+// and 111 apart.  Beside a prompt they would be passed over by most of the
+// grid: 63 of them and a prompt of 16 tokens 196 us joined, 102 apart.
+int attention_batch(gh_kv8* kv, Entry* e, int n, const Att8& a) {
+    n = (int)(std::remove_if(e, e + n, [](const Entry& x) { return x.cnt == 0; }) - e);
+    Entry* wide = std::stable_partition(e, e + n, [&](const Entry& x) { return x.cnt * a.group <= 4; });
+    int most = 0;
+    for (Entry* x = e; x < e + n; ++x) most = std::max(most, x->size = tiles_of(*x, a, 16));
+    if (most == 1 && wide < e + n) wide = e;
+    if (wide > e) GH_CHECK(attention_launch(kv, e, (int)(wide - e), 4, a));
+    return launch_by_size(wide, (int)(e + n - wide), kv->nkv,
+                          [&](Entry* x, int c) { return attention_launch(kv, x, c, 16, a); });
 }
 
 }  // namespace
@@ -172,18 +291,18 @@ extern "C" int gh_kv8_append(gh_kv8* kv, int32_t n, const int32_t* seqs, const i
     const size_t row = (size_t)kv->nkv * kv->hd;
     for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
         const int m = std::min(n - i0, KV8_BATCH);
-        Kv8Batch b;
-        int blocks = 0, rows = 0;
+        Entry e[KV8_BATCH];
+        int rows = 0;
         for (int i = 0; i < m; ++i) {
             const int s = seqs[i0 + i], t = n_tok[i0 + i];
-            b.seq[i] = s;
-            b.pos[i] = kv->len[s];
-            b.off[i] = rows;
-            b.cnt[i] = t;
+            e[i] = {s, kv->len[s], rows, t, blocks_of(kv->len[s], kv->len[s] + t), 0};
             rows += t;
-            blocks = std::max(blocks, blocks_of(kv->len[s], kv->len[s] + t));
         }
-        if (blocks) GH_CHECK(launch_kv8_append(dev(kv), kv->hd, b, m, blocks, k, v, ctx->stream));
+        GH_CHECK(launch_by_size(e, m, 2 * kv->nkv, [&](const Entry* x, int c) {
+            Kv8Batch b;
+            to_batch(x, c, b);
+            return launch_kv8_append(dev(kv), kv->hd, b, c, most_blocks(x, c), k, v, ctx->stream);
+        }));
         k += (size_t)rows * row;
         v += (size_t)rows * row;
     }
@@ -242,18 +361,18 @@ extern "C" int gh_kv8_read(gh_kv8* kv, int32_t n, const int32_t* seqs, const int
     const size_t row = (size_t)kv->nkv * kv->hd;
     for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
         const int m = std::min(n - i0, KV8_BATCH);
-        Kv8Batch b;
-        int blocks = 0, rows = 0;
+        Entry e[KV8_BATCH];
+        int rows = 0;
         for (int i = 0; i < m; ++i) {
             const int at = begins[i0 + i], end = ends[i0 + i];
-            b.seq[i] = seqs[i0 + i];
-            b.pos[i] = at;
-            b.off[i] = rows;
-            b.cnt[i] = end - at;
+            e[i] = {seqs[i0 + i], at, rows, end - at, blocks_of(at, end), 0};
             rows += end - at;
-            blocks = std::max(blocks, blocks_of(at, end));
         }
-        if (blocks) GH_CHECK(launch_kv8_read(dev(kv), kv->hd, b, m, blocks, k_out, v_out, ctx->stream));
+        GH_CHECK(launch_by_size(e, m, 2 * kv->nkv, [&](const Entry* x, int c) {
+            Kv8Batch b;
+            to_batch(x, c, b);
+            return launch_kv8_read(dev(kv), kv->hd, b, c, most_blocks(x, c), k_out, v_out, ctx->stream);
+        }));
         if (k_out) k_out += (size_t)rows * row;
         if (v_out) v_out += (size_t)rows * row;
     }
@@ -281,64 +400,25 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
     if (total == 0) return GH_OK;
     if (!q || !out || !aligned(q) || !aligned(out))
         return set_error(GH_ERR_INVALID, "gh_kv8_attention: q and out must be 16-byte aligned device pointers");
-    const size_t row = (size_t)n_heads * kv->hd;
+    Att8 a{};
+    a.heads = n_heads;
+    a.group = group;
+    a.group_inv = group == 1 ? 0 : (unsigned)(((uint64_t(1) << 32) + group - 1) / group);
+    a.window = window >= kv->max_seq ? 0 : window;
+    a.q = q;
+    a.out = out;
     for (int i0 = 0; i0 < n; i0 += KV8_BATCH) {
         const int m = std::min(n - i0, KV8_BATCH);
-        // the longest entries first: their workgroups start before the others'
-        struct Entry {
-            int seq, len, off, cnt, blocks;
-        } e[KV8_BATCH];
-        int tokens = 0, rows = 0;  // query tokens of all; query rows of the longest entry
+        Entry e[KV8_BATCH];
+        int tokens = 0;
         for (int i = 0; i < m; ++i) {
             const int s = seqs[i0 + i], t = n_q[i0 + i];
-            e[i] = {s, kv->len[s], tokens, t, 0};
+            e[i] = {s, kv->len[s], tokens, t, 0, 0};
             tokens += t;
-            rows = std::max(rows, t * group);
         }
-        if (rows == 0) continue;
-        Att8 a{};
-        a.tile = rows <= 4 ? 4 : 16;
-        a.tiles = (rows + a.tile - 1) / a.tile;
-        int most = 0;      // blocks of the longest row tile
-        int64_t work = 0, wgs = 0;  // blocks of all row tiles, and these
-        for (int i = 0; i < m; ++i) {
-            if (e[i].cnt == 0) continue;
-            // tokens a tile may see: up to the window and its own rows
-            const int len = e[i].len;
-            const int span = window ? (int)std::min<int64_t>(len, (int64_t)window + a.tile / group + 1) : len;
-            e[i].blocks = std::min((len + KV8_BLOCK - 1) / KV8_BLOCK, span / KV8_BLOCK + 2);
-            most = std::max(most, e[i].blocks);
-            const int64_t tiles = (int64_t)((e[i].cnt * group + a.tile - 1) / a.tile) * kv->nkv;
-            wgs += tiles;
-            work += tiles * e[i].blocks;
-        }
-        std::stable_sort(e, e + m, [](const Entry& x, const Entry& y) { return x.blocks > y.blocks; });
-        Kv8Batch b;
-        for (int i = 0; i < m; ++i) {
-            b.seq[i] = e[i].seq;
-            b.pos[i] = e[i].len;
-            b.off[i] = e[i].off;
-            b.cnt[i] = e[i].cnt;
-        }
-        a.chunk = kv8_chunk(kv->hd, a.tile, most, work, wgs);
-        a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
-        if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
-            return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows in one call", rows);
-        a.q = q;
-        a.out = out;
-        a.heads = n_heads;
-        a.group = group;
-        a.group_inv = group == 1 ? 0 : (unsigned)(((uint64_t(1) << 32) + group - 1) / group);
-        a.window = window;
-        a.rows = (size_t)tokens * n_heads;
-        if (a.ns > 1) {
-            void* part = nullptr;
-            GH_CHECK(ctx_scratch(ctx, a.rows * a.ns * (kv->hd + 2) * sizeof(float), &part));
-            a.part = (float*)part;
-        }
-        GH_CHECK(launch_kv8_attention(dev(kv), kv->hd, b, m, a, ctx->stream));
-        q += (size_t)tokens * row;
-        out += (size_t)tokens * row;
+        GH_CHECK(attention_batch(kv, e, m, a));
+        a.q += (size_t)tokens * n_heads * kv->hd;
+        a.out += (size_t)tokens * n_heads * kv->hd;
     }
     return op_sync(ctx);
 }

@@ -42,12 +42,13 @@ struct Kv8Dev {
 
 // Up to KV8_BATCH sequences of a call, by value in a kernel's arguments (no
 // copy to the device, and the host has checked every number).
-constexpr int KV8_BATCH = 240;
+constexpr int KV8_BATCH = 192;
 struct Kv8Batch {
     int seq[KV8_BATCH];
-    int pos[KV8_BATCH];  // append, truncate: tokens before; read: begin; attention: tokens
-    int off[KV8_BATCH];  // first of the entry's rows among the call's
-    int cnt[KV8_BATCH];  // new tokens; tokens to read; query tokens; truncate: the new length itself
+    int pos[KV8_BATCH];   // append, truncate: tokens before; read: begin; attention: tokens
+    int off[KV8_BATCH];   // first of the entry's rows among the call's
+    int cnt[KV8_BATCH];   // new tokens; tokens to read; query tokens; truncate: the new length itself
+    int part[KV8_BATCH];  // attention: first of the entry's query tokens among the launch's
 };
 
 // blocks: the most that one of the entries touches
@@ -63,6 +64,7 @@ struct Att8 {
     float* out;
     float* part;  // chunk states: m [rows][ns], l [rows][ns], o [rows][ns][hd]; rows = heads * query tokens
     size_t rows;
+    int most_q;          // query tokens of the entry that has most
     int heads, group;    // query heads, per kv head
     unsigned group_inv;  // ceil(2^32 / group): the upper half of row * group_inv is row / group (0 for group 1)
     int window;

@@ -443,6 +443,8 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         const int t = token_of(r);
         return ((size_t)b.off[i] + t) * a.heads + (h * a.group + row0 + r - t * a.group);
     };
+    // and among the chunk states
+    auto part_of = [&](int r) { return slot_of(r) + ((ptrdiff_t)b.part[i] - b.off[i]) * a.heads; };
     // positions of the tile's first and last row, and the blocks they see
     const int p0 = len - n_q + token_of(0), p1 = len - n_q + token_of(rows - 1);
     const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
@@ -453,8 +455,8 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
     if (blk0 >= blk1) {  // nothing to see in this chunk
         if (a.ns > 1) {
             if (tid < rows) {
-                a.part[slot_of(tid) * a.ns + chunk] = -INFINITY;
-                a.part[(a.rows + slot_of(tid)) * a.ns + chunk] = 0.0f;
+                a.part[part_of(tid) * a.ns + chunk] = -INFINITY;
+                a.part[(a.rows + part_of(tid)) * a.ns + chunk] = 0.0f;
             }
         } else {
             for (int e = tid; e < rows * HD; e += 64 * WAVES) a.out[slot_of(e / HD) * HD + e % HD] = 0.0f;
@@ -629,16 +631,15 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
     __syncthreads();
     auto weight = [&](int w, int r, float M) { return st_m[w][r] == -INFINITY ? 0.0f : exp2_fast(st_m[w][r] - M); };
     auto put = [&](int r, int q4, f32x4 v, float M, float L) {  // dims 4 q4 .. of the tile's row r
-        const size_t slot = slot_of(r);
         if (a.ns > 1) {
-            const size_t at = slot * a.ns + chunk;
+            const size_t at = part_of(r) * a.ns + chunk;
             if (q4 == 0) {
                 a.part[at] = M;
                 a.part[a.rows * a.ns + at] = L;
             }
             ((f32x4*)(a.part + 2 * a.rows * a.ns + at * HD))[q4] = v;
         } else {
-            ((f32x4*)(a.out + slot * HD))[q4] = v * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
+            ((f32x4*)(a.out + slot_of(r) * HD))[q4] = v * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
         }
     };
     const int jr = ROWS == 4 ? tid / (HD / 4) : col.row;  // row that this thread joins
@@ -683,11 +684,13 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
 // dims, its threads the chunks side by side, their outputs on the way before
 // the weights are known.
 template <int HD, int LN>
-__global__ __launch_bounds__(NT) void k_kv8_combine(Att8 a) {
+__global__ __launch_bounds__(NT) void k_kv8_combine(Kv8Batch b, Att8 a) {
     constexpr int GR = NT / LN, U = 4;  // groups that share the chunks, loads in flight
     __shared__ float red[8];
     __shared__ __align__(16) f32x4 sum[GR][LN];
-    const size_t slot = blockIdx.x / (HD / 4 / LN);
+    const int i = blockIdx.y, row = blockIdx.x / (HD / 4 / LN);
+    if (row >= b.cnt[i] * a.heads) return;
+    const size_t slot = (size_t)b.part[i] * a.heads + row;
     const int d4 = blockIdx.x % (HD / 4 / LN) * LN;
     const float* pm = a.part + slot * a.ns;
     const float* pl = a.part + (a.rows + slot) * a.ns;
@@ -732,7 +735,7 @@ __global__ __launch_bounds__(NT) void k_kv8_combine(Att8 a) {
         float r = 0.0f;
 #pragma unroll
         for (int j = 0; j < GR; ++j) r += t[j * 4 * LN + tid];
-        a.out[slot * HD + 4 * d4 + tid] = r * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
+        a.out[((size_t)b.off[i] * a.heads + row) * HD + 4 * d4 + tid] = r * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
     }
 }
 
@@ -777,8 +780,9 @@ int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, cons
         else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<false>>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide<false>::WAVES), 0, s, c, b, a);
         // few chunks: a row a workgroup (of 64 rows or more, so that they fill the device)
         constexpr int LN = h.value / 4;
-        if (a.ns > 1 && (a.ns > 4 * (NT / LN) || a.rows < 64)) hipLaunchKernelGGL((k_kv8_combine<h.value, 8>), dim3(a.rows * (h.value / 32)), dim3(NT), 0, s, a);
-        else if (a.ns > 1) hipLaunchKernelGGL((k_kv8_combine<h.value, LN>), dim3(a.rows), dim3(NT), 0, s, a);
+        const unsigned rows = (unsigned)a.most_q * a.heads;
+        if (a.ns > 1 && (a.ns > 4 * (NT / LN) || a.rows < 64)) hipLaunchKernelGGL((k_kv8_combine<h.value, 8>), dim3(rows * (h.value / 32), n), dim3(NT), 0, s, b, a);
+        else if (a.ns > 1) hipLaunchKernelGGL((k_kv8_combine<h.value, LN>), dim3(rows, n), dim3(NT), 0, s, b, a);
     });
 }
 

@@ -13,6 +13,8 @@ extern "C" int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, 
         return set_error(GH_ERR_INVALID, "gh_sample_rows: %d rows of %d logits", n_rows, vocab);
     if (n_rows == 0) return GH_OK;
     if (!logits || !rules || !tokens_out) return set_error(GH_ERR_INVALID, "gh_sample_rows: null argument");
+    if (((uintptr_t)logits | (uintptr_t)tokens_out) & 3)
+        return set_error(GH_ERR_INVALID, "gh_sample_rows: logits and tokens_out must be 4-byte aligned device pointers");
     for (int i = 0; i < n_rows; ++i) {
         const gh_sampling& r = rules[i];
         if (!(r.temperature >= 0.0f) || std::isinf(r.temperature))

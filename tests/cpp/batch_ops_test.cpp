@@ -3,10 +3,12 @@
 // and lifetimes.  Linked against hip_stub.cpp / kernel_stub.cpp and the
 // launchers below, which check each launch against the cache's shape instead
 // of running it; built with AddressSanitizer by tests/test_batch_ops_host.py.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <limits>
+#include <numeric>
 #include <thread>
 #include <vector>
 
@@ -32,6 +34,8 @@ int n_seq = 0;
 std::vector<Kv8Batch> batches;
 std::vector<Att8> attentions;
 std::vector<int> sample_rows;
+std::vector<char> covered;        // of a call's tokens: once each, in whichever launch
+const float* rows_at = nullptr;  // first row of the calls, where tokens are watched
 #define WANT(c)                                                             \
     do {                                                                    \
         if (!(c)) {                                                         \
@@ -45,15 +49,24 @@ static void look(const Kv8Batch& b, int n) {
     for (int i = 0; i < n; ++i) WANT(b.seq[i] >= 0 && b.seq[i] < n_seq && b.pos[i] >= 0);
     batches.push_back(b);
 }
-int launch_kv8_append(const Kv8Dev&, int, const Kv8Batch& b, int n, int blocks, const float* k, const float* v, hipStream_t) {
+static void cover(const Kv8Batch& b, int n, const float* rows, size_t ld) {
+    const size_t first = rows_at ? (rows - rows_at) / ld : 0;
+    for (int i = 0; rows_at && i < n; ++i)
+        for (size_t t = first + b.off[i]; t < first + b.off[i] + b.cnt[i]; ++t) {
+            if (t >= covered.size()) covered.resize(t + 1, 0);
+            WANT(!covered[t]);
+            covered[t] = 1;
+        }
+}
+int launch_kv8_append(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int blocks, const float* k, const float* v, hipStream_t) {
     look(b, n);
-    WANT(k && v && b.off[0] == 0);
-    for (int i = 1; i < n; ++i) WANT(b.off[i] == b.off[i - 1] + b.cnt[i - 1]);
+    WANT(k && v);
+    cover(b, n, k, (size_t)c.nkv * hd);
     int most = 0;
     for (int i = 0; i < n; ++i) {
         const int cnt = b.cnt[i], end = b.pos[i] + cnt;
-        WANT(cnt >= 0 && end <= cap_tokens);
-        if (cnt) most = std::max(most, (end - 1) / 64 - b.pos[i] / 64 + 1);
+        WANT(cnt > 0 && end <= cap_tokens);
+        most = std::max(most, (end - 1) / 64 - b.pos[i] / 64 + 1);
     }
     WANT(blocks == most && blocks > 0);
     return GH_OK;
@@ -73,13 +86,14 @@ int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, cons
     look(b, n);
     attentions.push_back(a);
     WANT(a.q && a.out && a.group * c.nkv == a.heads && (a.tile == 4 || a.tile == 16) && a.tiles > 0 && a.ns > 0);
-    std::vector<char> taken(a.rows / a.heads, 0);  // every query token has one entry
-    for (int i = 0; i < n; ++i)
-        for (int t = b.off[i]; t < b.off[i] + b.cnt[i]; ++t) {
-            WANT(t >= 0 && (size_t)t < taken.size() && !taken[t]);
-            if (t >= 0 && (size_t)t < taken.size()) taken[t] = 1;
-        }
-    for (char c : taken) WANT(c);
+    cover(b, n, a.q, (size_t)a.heads * hd);
+    int part = 0, most_q = 0;  // every query token has its own place among the states
+    for (int i = 0; i < n; ++i) {
+        WANT(b.part[i] == part && b.cnt[i] > 0);
+        part += b.cnt[i];
+        most_q = std::max(most_q, b.cnt[i]);
+    }
+    WANT((size_t)part * a.heads == a.rows && most_q == a.most_q);
     WANT((int64_t)a.ns * a.tiles * c.nkv <= 1 << 23);
     if (a.tile == 4) WANT(a.tiles == 1);
     if (a.ns > 1) {  // the scratch holds every state
@@ -232,6 +246,8 @@ int refusals() {
     CHECK(gh_sample_rows(ctx, P, 1, 10, nullptr, t) == GH_ERR_INVALID);
     CHECK(gh_sample_rows(ctx, P, 1, 10, r, nullptr) == GH_ERR_INVALID);
     CHECK(gh_sample_rows(ctx, P, -1, 10, r, t) == GH_ERR_INVALID);
+    CHECK(gh_sample_rows(ctx, (float*)((char*)P + 2), 1, 10, r, t) == GH_ERR_INVALID);
+    CHECK(gh_sample_rows(ctx, P, 1, 10, r, (int32_t*)((char*)t + 1)) == GH_ERR_INVALID);
     CHECK(gh_sample_rows(ctx, P, 1, 0, r, t) == GH_ERR_INVALID);
     CHECK(gh_sample_rows(ctx, P, 1, (1 << 24) + 1, r, t) == GH_ERR_INVALID);
     CHECK(gh_sample_rows(ctx, nullptr, 0, 10, nullptr, nullptr) == GH_OK);
@@ -257,6 +273,7 @@ int refusals() {
 // What the attention hands to its kernels, over many shapes.
 int splits() {
     gh_ctx* ctx = nullptr;
+    rows_at = P;
     CHECK(gh_ctx_create(0, &ctx) == GH_OK);
     for (int nkv : {1, 2, 4}) {
         for (int max_seq : {1, 64, 700, 5000, 40000}) {
@@ -267,15 +284,35 @@ int splits() {
                 seqs[i] = 299 - i;
                 lens[i] = (int)((int64_t)i * i * 7 % (max_seq + 1));
             }
-            CHECK(gh_kv8_append(kv, 300, seqs.data(), lens.data(), P, P) == GH_OK);
+            auto all = [](const std::vector<int32_t>& cnt, int n) {  // the call's tokens, each in one launch
+                const size_t want = std::accumulate(cnt.begin(), cnt.begin() + n, (size_t)0);
+                const bool ok = covered.size() == want && std::count(covered.begin(), covered.end(), 1) == (ptrdiff_t)want;
+                covered.clear();
+                return ok;
+            };
+            covered.clear();
+            CHECK(gh_kv8_append(kv, 300, seqs.data(), lens.data(), P, P) == GH_OK && all(lens, 300));
             for (int group : {1, 2, 3, 4, 8, 20})
                 for (int window : {0, 1, 512})
                     for (int t : {1, 2, 5, 33, 700}) {
                         for (int n : {1, 7, 300}) {
                             for (int i = 0; i < n; ++i) nq[i] = i % 3 == 2 ? 0 : std::max(0, t - i % 5);
                             CHECK(gh_kv8_attention(kv, n, seqs.data(), nq.data(), P, group * nkv, window, P) == GH_OK);
+                            CHECK(all(nq, n));
                         }
+                        // one long entry among single tokens, and lengths of every size
+                        for (int i = 0; i < 300; ++i) nq[i] = i % 7 == 3 ? t * (i % 49 == 3 ? 40 : 1) : 1;
+                        CHECK(gh_kv8_attention(kv, 300, seqs.data(), nq.data(), P, group * nkv, window, P) == GH_OK);
+                        CHECK(all(nq, 300));
                     }
+            std::vector<int32_t> none(300, 0);
+            launches = 0;
+            CHECK(gh_kv8_truncate(kv, 300, seqs.data(), none.data()) == GH_OK);
+            // tokens of one long and many short sequences: not a grid of the long one's size for each
+            for (int i = 0; i < 300; ++i) lens[i] = i == 5 ? max_seq : 1;
+            CHECK(gh_kv8_append(kv, 300, seqs.data(), lens.data(), P, P) == GH_OK && all(lens, 300));
+            CHECK(launches == (max_seq >= 5000 || (max_seq == 700 && nkv > 1) ? 3 : 2));
+            launches = 1001;
             CHECK(gh_kv8_destroy(kv) == GH_OK);
         }
     }

@@ -315,9 +315,35 @@ def test_queries_in_front_of_the_cache_see_nothing_and_give_zeros(ctx):
     c = gh.KVCache8(ctx, 2, 64, 1, 64)
     ks, vs = _fill(c, rng, [3])
     q = rows(rng, 21 + 2, 4, 64)
-    got = c.attention([0, 1], [21, 2], q, 4)
-    assert np.array_equal(got[:18], np.zeros_like(got[:18])) and np.array_equal(got[21:], np.zeros_like(got[21:]))
-    _check(got[18:21], ks, vs, q[18:21], [3], 0)
+    for window in (0, 2, 2 ** 31 - 1):  # the last: further back than 32 bits count
+        got = c.attention([0, 1], [21, 2], q, 4, window)
+        assert np.array_equal(got[:18], np.zeros_like(got[:18])) and np.array_equal(got[21:], np.zeros_like(got[21:]))
+        _check(got[18:21], ks, vs, q[18:21], [3], window)
+
+
+def test_a_prompt_and_drafts_among_single_tokens(ctx):
+    """One call of sizes far apart, which goes in several launches: 150
+    sequences take one token each, one a prompt of 1200, a few take drafts."""
+    rng = np.random.default_rng(30)
+    n, nkv, nq, hd = 156, 4, 8, 32
+    new = np.ones(n, int)
+    new[[3, 50]], new[[7, 70, 101, 155]], new[20] = (1200, 90), (5, 2, 9, 17), 0
+    old = rng.integers(1, 700, n)
+    old[[3, 20, 60]] = 0, 5, 1500
+    c = gh.KVCache8(ctx, n, 1600, nkv, hd)
+    order = rng.permutation(n)
+    held = [[rows(rng, a + b, nkv, hd) for a, b in zip(old, new)] for _ in (0, 1)]
+    for lo, hi in ((np.zeros(n, int), old), (old, old + new)):
+        c.append(order, (hi - lo)[order], *[np.concatenate([x[s][lo[s]:hi[s]] for s in order]) for x in held])
+    stored = [[quantise(x)[2] for x in h] for h in held]
+    begins = np.maximum(old + new - 40, 0)
+    begins[3] = 0
+    got = c.read(order, begins[order], (old + new)[order])
+    for g, x in zip(got, stored):
+        assert same_bits(g, np.concatenate([x[s][begins[s]:] for s in order]))
+    q = rows(rng, int(new.sum()), nq, hd)
+    for window in (0, 100):
+        _check(c.attention(order, new[order], q, nq, window), *stored, q, new[order], window, order)
 
 
 def test_tokens_that_were_truncated_away_are_not_seen(ctx):
