@@ -21,6 +21,8 @@
 // run all steps in one kernel (k_smp_row).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "sampling.h"
 
 namespace gh {
@@ -29,6 +31,7 @@ namespace {
 
 typedef unsigned long long u64;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr double LOG2E = 1.44269504088896340736;
 
 // Ascending in rank order: value descending, then index ascending.
 __device__ __forceinline__ uint32_t value_key(float v) {
@@ -78,12 +81,15 @@ struct Weights {
 };
 
 // What the bins are: equal steps of top - l up to `reach`, behind which every
-// weight is zero.  Monotonic in l, so that bins follow the ranks.  (An infinite
+// weight is zero.  Monotonic in l, so that bins follow the ranks.  Half the
+// distance, which no two finite logits take out of f32's range.  (An infinite
 // top and its equals: a NaN, which is in reach and becomes bin 0.)
 struct Bins {
-    float top, scale, reach;
-    __device__ __forceinline__ bool in_reach(float l) const { return !(top - l > reach); }
-    __device__ __forceinline__ int of(float l) const { return min((int)((top - l) * scale), SMP_BINS - 1); }
+    float half_top, scale, reach;  // bins a unit of half the distance; largest half the distance
+    __device__ __forceinline__ float half(float l) const { return fmaf(-0.5f, l, half_top); }
+    __device__ __forceinline__ bool in_reach(float l) const { return !(half(l) > reach); }
+    __device__ __forceinline__ float place(float l) const { return half(l) * scale; }
+    __device__ __forceinline__ int of(float l) const { return min((int)place(l), SMP_BINS - 1); }
 };
 
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int o) {
@@ -140,12 +146,19 @@ __device__ __forceinline__ void block_scan(u64& m, unsigned& c, Small& sh) {
         if (i < w) m += sh.red[i], c += sh.red32[i];
 }
 
+// The distance from the largest logit at which a weight, below 2^-(bits + 2),
+// rounds to zero; as f32 no shorter than it is.
+__device__ __forceinline__ double dead_of(int bits, double log2e_t) { return (bits + 2) / log2e_t; }
+__device__ __forceinline__ float dead_of(int bits, float temperature) {
+    return (float)(dead_of(bits, LOG2E / (double)temperature) * 1.000001);
+}
+
 // ------------------------------------------------------------------
 // step 1
 // ------------------------------------------------------------------
 struct Stat {
     u64 first;  // rank key of the first in rank order; ~0: nothing above -inf
-    float low;  // smallest value above -inf; +inf if there is none
+    float low;  // smallest of those that may have a weight, or one below it
     bool nan;
     float own;  // the largest of the elements that this thread read
 };
@@ -187,23 +200,46 @@ __device__ __forceinline__ void each_logit(const float* l, int i0, int i1, F&& f
     if (const int i = r.edge(threadIdx.x); i >= 0) f(i, l[i]);
 }
 
+// largest over 16 lanes
+__device__ __forceinline__ float max16(float v) {
+    auto turned = [](float x, auto by) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + by.value, 0xF, 0xF, true));
+    };
+    v = fmaxf(v, turned(v, std::integral_constant<int, 8>{}));
+    v = fmaxf(v, turned(v, std::integral_constant<int, 4>{}));
+    v = fmaxf(v, turned(v, std::integral_constant<int, 2>{}));
+    return fmaxf(v, turned(v, std::integral_constant<int, 1>{}));
+}
+
+// dead: the distance from the largest at which a weight is zero.  Masked
+// logits, of the type's lowest value or the like, have to stay out of `low`:
+// bins that reached so far would be few for the others.  What is that far
+// below the largest of the first 256 that 16 lanes read is that far below the
+// row's.
 template <int NT>
-__device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small& sh) {
+__device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, float dead, Small& sh) {
     constexpr int U = 4;
     const Quads r(l, i0, i1);
     float best = -INFINITY, low = INFINITY;
     int at = -1;  // index of the best, or of the first of its quad
+    float floor = -3.4028234e38f;
     bool nan = false;
     auto one = [&](int i, float v) {
         nan |= v != v;
         if (v > best || (v == best && i < at)) best = v, at = i;
-        low = fminf(low, v > -INFINITY ? v : INFINITY);
+        low = fminf(low, v >= floor ? v : INFINITY);
     };
 #pragma unroll 1
     for (int q = threadIdx.x; q < r.quads; q += U * NT) {
         f32x4 v[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) v[j] = r.p[min(q + j * NT, r.quads - 1)];
+        if (q == threadIdx.x) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < U; ++j) m = fmaxf(m, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
+            floor = fmaxf(floor, max16(m) - dead);
+        }
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             // The last quad may come more than once: not for `best`, which is
@@ -213,10 +249,10 @@ __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, Small
             float lo = fminf(fminf(v[j].x, v[j].y), fminf(v[j].z, v[j].w));
             nan |= __builtin_isunordered(v[j].x, v[j].y) | __builtin_isunordered(v[j].z, v[j].w);
             if (hi > best) best = hi, at = r.first + 4 * (q + j * NT);
-            if (lo == -INFINITY) {
+            if (lo < floor) {
                 lo = INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) lo = fminf(lo, v[j][e] > -INFINITY ? v[j][e] : INFINITY);
+                for (int e = 0; e < 4; ++e) lo = fminf(lo, v[j][e] >= floor ? v[j][e] : INFINITY);
             }
             low = fminf(low, lo);
         }
@@ -257,14 +293,13 @@ __device__ __forceinline__ int token_of_undrawn(const Stat& s) { return s.nan ||
 
 __device__ __forceinline__ Weights weights_of(const Stat& s, const gh_sampling& rule, int bits) {
     const float top = key_value((unsigned)(s.first >> 32));
-    return {top, top == INFINITY ? 0.0 : (double)top, 1.44269504088896340736 / (double)rule.temperature, bits};
+    return {top, top == INFINITY ? 0.0 : (double)top, LOG2E / (double)rule.temperature, bits};
 }
 
 __device__ __forceinline__ Bins bins_of(const Stat& s, const Weights& w) {
-    // below 2^-(bits + 2) a weight rounds to zero
-    const double dead = (w.bits + 2) / w.log2e_t, span = (double)w.top - (double)s.low, d = span < dead ? span : dead;
-    if (!(d > 0.0)) return {w.top, 0.0f, 0.0f};  // one value: one bin
-    return {w.top, (float)fmin((double)SMP_BINS / d, 3e38), (float)fmin(d * 1.000001, 3.4e38)};
+    const double dead = dead_of(w.bits, w.log2e_t), span = (double)w.top - (double)s.low, d = span < dead ? span : dead;
+    if (!(d > 0.0)) return {0.5f * w.top, 0.0f, 0.0f};  // one value: one bin
+    return {0.5f * w.top, (float)fmin(2.0 * SMP_BINS / d, 3e38), (float)fmin(d * 0.5000005, 3.4028234e38)};
 }
 
 // ------------------------------------------------------------------
@@ -355,7 +390,7 @@ struct Running {
 // Where in the bins a weight falls below min_p, to be taken with a bin to
 // either side for roundings.
 __device__ __forceinline__ double min_p_bin(const Weights& w, const Bins& bins, const gh_sampling& rule) {
-    return (double)-log2f(rule.min_p) / w.log2e_t * (double)bins.scale;
+    return (double)-log2f(rule.min_p) / w.log2e_t * 0.5 * (double)bins.scale;
 }
 
 template <int NT>
@@ -425,7 +460,7 @@ __device__ __forceinline__ void range_gather(const float* l, int i0, int i1, con
     const float from = (float)lo, to = hi < SMP_BINS - 1 ? (float)(hi + 1) : INFINITY;
     each_logit<NT, 4>(l, i0, i1, [&](int i, float v) {
         // most elements are none of them, and are known by one product
-        const float t = (bins.top - v) * bins.scale;
+        const float t = bins.place(v);
         if (t < from || t >= to) return;
         if (!bins.in_reach(v)) return;
         const int b = bins.of(v);
@@ -506,7 +541,7 @@ __device__ __forceinline__ Short short_row(const float* group_max, int groups, c
     __syncthreads();
     for (int i = threadIdx.x; i < groups; i += NT) {
         const float v = group_max[i];
-        if (v > -INFINITY && bins.in_reach(v)) atomicAdd(&h.count[bins.of(v)], 1u);
+        if (bins.in_reach(v)) atomicAdd(&h.count[bins.of(v)], 1u);
     }
     __syncthreads();
     scan_counts<NT>(h.count, sh);
@@ -796,14 +831,27 @@ __device__ void find(const float* l, int n, const Weights& w, const Bins& bins, 
         if (tid < 256) sh.mass[tid] = 0, sh.count[tid] = 0;
         __syncthreads();
         const u64 prefix = sh.key;
+        // equal logits are what brings rows here: a thread's equal digits in a row go out together
+        int last = 0;
+        u64 mass = 0;
+        unsigned count = 0;
+        auto out = [&] {
+            if (count) atomicAdd(&sh.count[last], count);
+            if (mass) atomicAdd(&sh.mass[last], mass);
+        };
         each_logit<PT, 2>(l, 0, n, [&](int i, float v) {
             const u64 key = rank_key(v, i);
             if (shift < 56 && (key >> (shift + 8)) != (prefix >> (shift + 8))) return;
             const int d = (int)(key >> shift) & 255;
-            atomicAdd(&sh.count[d], 1u);
-            const u64 m = bins.in_reach(v) ? w.fixed(v) : 0;
-            if (m) atomicAdd(&sh.mass[d], m);
+            if (d != last) {
+                out();
+                last = d;
+                mass = count = 0;
+            }
+            ++count;
+            if (bins.in_reach(v)) mass += w.fixed(v);
         });
+        out();
         __syncthreads();
         if (tid == 0) {
             u64 mass = sh.base_mass;
@@ -877,7 +925,7 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
     const gh_sampling rule = rules.r[blockIdx.x];
     const float* l = logits + (size_t)blockIdx.x * n;
     const int tid = threadIdx.x;
-    const Stat s = range_stat<PT>(l, 0, n, sh);
+    const Stat s = range_stat<PT>(l, 0, n, dead_of(bits, rule.temperature), sh);
     if (!drawn(s, rule)) {
         if (tid == 0) tokens[blockIdx.x] = token_of_undrawn(s);
         return;
@@ -922,12 +970,13 @@ __device__ __forceinline__ int chunk_begin(int n, int c, int chunks) { return (i
 constexpr int CT = 512;  // threads of a workgroup that reads a chunk of a row
 
 // a row's chunks: stats; the row's bins cleared
-__global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, int group, SmpRow* rows) {
+__global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, int bits, int group, SmpRules rules, SmpRow* rows) {
     __shared__ Small sh;
     const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
     SmpRow& r = rows[blockIdx.y];
     for (int b = c * CT + tid; b < SMP_BINS; b += chunks * CT) r.mass[b] = 0, r.count[b] = 0;
-    const Stat s = range_stat<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), sh);
+    const Stat s = range_stat<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks),
+                                   dead_of(bits, rules.r[blockIdx.y].temperature), sh);
     float own = s.own;
     for (int o = 1; o < group; o <<= 1) own = fmaxf(own, __shfl_xor(own, o, 64));
     if (tid % group == 0) r.group_max[(c * CT + tid) / group] = own;
@@ -1058,7 +1107,7 @@ int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRule
         // threads that share a group: a power of two, and 512 to 1023 groups a row
         int group = 1;
         while (chunks * CT / group >= SMP_GROUPS) group *= 2;
-        hipLaunchKernelGGL(k_smp_stat, grid, dim3(CT), 0, s, logits, vocab, group, scratch);
+        hipLaunchKernelGGL(k_smp_stat, grid, dim3(CT), 0, s, logits, vocab, bits, group, rules, scratch);
         hipLaunchKernelGGL(k_smp_hist, grid, dim3(CT), 0, s, logits, vocab, bits, chunks * CT / group, rules, scratch);
         hipLaunchKernelGGL(k_smp_gather, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
         hipLaunchKernelGGL(k_smp_pick, dim3(n_rows), dim3(PT), 0, s, logits, vocab, bits, rules, (const SmpRow*)scratch, chunks,

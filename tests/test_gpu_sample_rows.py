@@ -140,6 +140,31 @@ def test_extreme_temperatures(ctx, t):
     check(ctx, l, gh.sampling(3, t, [0, 50, 0], [1, 1, 0.5], 0.0, [0.2, 0.6, 0.9]))
 
 
+@pytest.mark.parametrize("vocab", [9, 700, 40000])
+def test_logits_as_far_apart_as_f32_reaches(ctx, vocab):
+    """Distances that f32 does not hold, at a temperature that leaves them a
+    weight (exp(-2) at 3e38), beside masked ones."""
+    rng = np.random.default_rng(16)
+    l = rng.uniform(-3.4e38, 3.4e38, (5, vocab)).astype(F32)
+    l[:, [1, 4]] = -np.inf, np.finfo(F32).max
+    l[:, 7] = np.finfo(F32).min
+    r = gh.sampling(5, [3.4e38, 1e38, 3.4e38, 2e38, 3e37], [0, 0, 5, 0, 0], [1, 0.9, 1, 1, 1], [0, 0, 0, 0.1, 0], 0.0)
+    for u in (0.1, 0.6, 0.97):
+        r["u"] = u
+        check(ctx, l, r)
+    l[0, 3] = np.inf
+    assert check(ctx, l[:1], r[:1])[0] == 3
+
+
+@pytest.mark.parametrize("mask", [-1e9, -65504.0, np.finfo(F32).min])
+def test_flat_logits_under_a_finite_mask(ctx, mask):
+    rng = np.random.default_rng(18)
+    l = logits(rng, 12, 262144, 0.3)
+    l[rng.random(l.shape) < 0.5] = mask
+    l[:4, :200000] = mask
+    check(ctx, l, mixed(rng, 12, 262144))
+
+
 def test_zero_and_minus_zero_are_equal(ctx):
     l = np.array([[-0.0, 0.0, -1.0, 0.0]], F32)
     assert [int(gh.sample_rows(ctx, l, 4, gh.sampling(1, 1.0, 3, 1.0, 0.0, u))[0]) for u in (0.0, 0.4, 0.7)] == [0, 1, 3]
