@@ -317,10 +317,10 @@ constexpr float DIGIT_MAX = 8355711.0f;
 // Digits of v, |v| <= DIGIT_MAX, as the three low bytes, 128 too large: adding
 // 128 (65536 + 256 + 1) makes every digit an unsigned byte.
 __device__ __forceinline__ uint32_t digits_of(float v) { return (uint32_t)((int)rintf(v) + 0x808080); }
-// The same for DIGIT_MAX p with 0 <= p <= 1, the two low digits 128 too large:
-// an f32 between 2^23 and 2^24 has its integer in its low bits, and the sum
+// The same for m p with 0 <= p <= 1, m <= DIGIT_MAX, the two low digits 128 too
+// large: an f32 between 2^23 and 2^24 has its integer in its low bits, and the sum
 // below stays in front of 2^24.
-__device__ __forceinline__ uint32_t digits_of_share(float p) { return __float_as_uint(fmaf(p, DIGIT_MAX, 0x1p23f + 0x8080)); }
+__device__ __forceinline__ uint32_t digits_of_share(float p, float m) { return __float_as_uint(fmaf(p, m, 0x1p23f + 0x8080)); }
 constexpr uint32_t DIGIT_BIAS = 0x80808080u;  // what an exclusive or takes off four digits that are 128 too large
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -348,152 +348,87 @@ __device__ __forceinline__ uint32_t byte_of(const uint32_t* d, int n) {
     return lo | hi;
 }
 
-// The 16 columns of a product: 16 query rows, a product for each digit
-// (Wide), or 4 query rows with their three digits side by side, column 4 n + r
-// digit n of row r and the last four zero (Narrow).  Narrow is for decoding,
-// where a kv head has few query rows: a third of the products, and of the
-// conversions of their results.
-template <bool ONCE>  // one tile a kv head: each code is read once a call
-struct Wide {
-    static constexpr int ROWS = 16, DIG = 3, WAVES = 4;
-    int row;
-    __device__ __forceinline__ explicit Wide(int col) : row(col) {}
-    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return ONCE ? __builtin_nontemporal_load(p) : *p; }
-    // digit n of four probabilities
-    __device__ __forceinline__ int share(const uint32_t* d, int n) const {
-        return (int)(n < 2 ? byte_of(d, n) ^ DIGIT_BIAS : byte_of(d, n));
+// The query rows of a workgroup: ROWS (token, head) pairs of one kv head, and
+// the chunk of key blocks that they look at.
+template <int ROWS>
+struct Tile {
+    const Kv8Batch& b;
+    const Att8& a;
+    int i, h, chunk;  // entry, kv head, chunk
+    int row0, rows;   // first row, and how many there are
+    int first;        // position of the entry's first query token
+    int p0, p1;       // positions of the tile's first and last row
+    int blk0, blk1;   // key blocks
+    __device__ __forceinline__ Tile(const Kv8Batch& b, const Att8& a, int i, int h, int chunk, int tile)
+        : b(b), a(a), i(i), h(h), chunk(chunk), row0(tile * ROWS) {
+        const int n_q = b.cnt[i];
+        rows = min(n_q * a.group - row0, ROWS);
+        first = b.pos[i] - n_q;
+        p0 = first + token_of(0);
+        p1 = first + token_of(rows - 1);
+        // the blocks that they see, in chunks of one size: as many as a.chunk makes, evenly
+        const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
+        const unsigned blocks = max(end - begin, 0), parts = (blocks + a.chunk - 1) / (unsigned)a.chunk;
+        const int size = a.ns > 1 && parts ? (int)((blocks + parts - 1) / parts) : (int)blocks;
+        blk0 = begin + chunk * size;
+        blk1 = min(blk0 + size, end);
     }
-    // column of digit n of a query row in the digit's operand
-    __device__ __forceinline__ static int place(int r, int) { return r; }
-    __device__ __forceinline__ static int operand(int n) { return n; }
-    // a product's value; a digit's sum is below 2^22 (256 dims, or 64 tokens)
-    __device__ __forceinline__ float scaled(float w) const { return w; }
-    __device__ __forceinline__ float sum(const i32x4* acc, int j) const {
-        return fmaf((float)acc[2][j], 65536.0f, (float)(acc[1][j] * 256 + acc[0][j]));
+    // query token of row r, and the row's place in q and out
+    __device__ __forceinline__ int token_of(int r) const {
+        return (int)__umulhi((unsigned)(row0 + r), a.group_inv) + (a.group == 1 ? row0 + r : 0);
     }
-    __device__ __forceinline__ float join(float v) const { return v; }
-};
-struct Narrow {
-    static constexpr int ROWS = 4, DIG = 1, WAVES = 8;
-    int row, digit;
-    uint32_t lo, hi, bias;  // byte selectors of the lane's digit, and what its bytes are too large
-    float weight;
-    // each code is read once a call
-    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return __builtin_nontemporal_load(p); }
-    __device__ __forceinline__ explicit Narrow(int col) : row(col & 3), digit(col >> 2) {
-        lo = digit == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * digit;
-        hi = digit == 3 ? 0x0c0c0c0cu : 0x04000c0cu + 0x01010000u * digit;
-        bias = digit < 2 ? DIGIT_BIAS : 0u;
-        weight = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
-    }
-    __device__ __forceinline__ int share(const uint32_t* d, int) const {
-        return (int)((__builtin_amdgcn_perm(d[1], d[0], lo) | __builtin_amdgcn_perm(d[3], d[2], hi)) ^ bias);
-    }
-    __device__ __forceinline__ static int place(int r, int n) { return 4 * n + r; }
-    __device__ __forceinline__ static int operand(int) { return 0; }
-    // the lane's digit alone; join() adds the row's other two
-    __device__ __forceinline__ float scaled(float w) const { return w * weight; }
-    __device__ __forceinline__ float sum(const i32x4* acc, int j) const { return (float)acc[0][j]; }
-    // The row's lanes have to get the same sum to the last bit, since each
-    // takes its own digit of the probability that comes of it: additions of
-    // the same values in either order, none fused with the product before.
-    __device__ __forceinline__ float join(float v) const {
-#pragma clang fp contract(off)
-        v = v + dpp<DPP_ROW_ROR8>(v);
-        return v + dpp<DPP_ROW_ROR4>(v);
-    }
-};
-
-// One workgroup: the columns' query rows of one kv head x one chunk of key
-// blocks, the blocks dealt to its waves; each wave keeps its own running
-// maximum, sum and output, joined through LDS at the end.
-//   S^T = K Q^T   operand A: codes of 16 tokens, B: digits of the query rows;
-//                 lane (g, col) gets tokens 16 t + 4 g + i of its row
-//   O^T = V^T P^T operand A: codes of 16 dims, B: digits of the lane's own
-//                 16 probabilities (the layout of V has their order)
-// The codes of the next block are on their way while the present one is
-// worked on, as far as the registers reach.
-template <int HD, class Cols>
-__global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
-    constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Cols::ROWS, DIG = Cols::DIG, WAVES = Cols::WAVES;
-    constexpr bool LATE_K = HD >= 128, LATE_V = HD == 256 && ROWS == 16;
-    __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
-    __shared__ uint32_t qmax[ROWS];
-    __shared__ i32x4 qs[DIG][KD][64];
-    __shared__ __align__(16) float ob[ROWS == 4 ? WAVES : 2][ROWS][HD + 4];
-    // Narrow: one tile, grid (chunks, kv heads).  Wide: grid x over the kv
-    // heads, then the chunks, then the tiles, the longest (last) first.
-    const int i = blockIdx.z;
-    int h = blockIdx.y, chunk = blockIdx.x, tile = 0;
-    if (ROWS > 4) {
-        const unsigned x = blockIdx.x / (unsigned)c.nkv;
-        h = blockIdx.x - x * c.nkv;
-        const unsigned t = a.ns > 1 ? x / (unsigned)a.ns : x;
-        chunk = x - t * a.ns;
-        tile = a.tiles - 1 - t;
-    }
-    const int row0 = tile * ROWS;
-    const int n_q = b.cnt[i], rows = min(n_q * a.group - row0, ROWS), len = b.pos[i];
-    if (rows <= 0) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
-    const Cols col(lane & 15);
-    // query token of the tile's row r, and the row's place in q and out
-    auto token_of = [&](int r) { return (int)__umulhi((unsigned)(row0 + r), a.group_inv) + (a.group == 1 ? row0 + r : 0); };
-    auto slot_of = [&](int r) {
+    __device__ __forceinline__ size_t slot_of(int r) const {
         const int t = token_of(r);
         return ((size_t)b.off[i] + t) * a.heads + (h * a.group + row0 + r - t * a.group);
-    };
+    }
     // and among the chunk states
-    auto part_of = [&](int r) { return slot_of(r) + ((ptrdiff_t)b.part[i] - b.off[i]) * a.heads; };
-    // positions of the tile's first and last row, and the blocks they see
-    const int p0 = len - n_q + token_of(0), p1 = len - n_q + token_of(rows - 1);
-    const int begin = a.window ? max(p0 - a.window + 1, 0) / KV8_BLOCK : 0, end = p1 < 0 ? 0 : p1 / KV8_BLOCK + 1;
-    // chunks of one size: as many as a.chunk makes, evenly
-    const unsigned blocks = max(end - begin, 0), parts = (blocks + a.chunk - 1) / (unsigned)a.chunk;
-    const int size = a.ns > 1 && parts ? (int)((blocks + parts - 1) / parts) : (int)blocks;
-    const int blk0 = begin + chunk * size, blk1 = min(blk0 + size, end);
-    if (blk0 >= blk1) {  // nothing to see in this chunk
+    __device__ __forceinline__ size_t part_of(int r) const {
+        return slot_of(r) + ((ptrdiff_t)b.part[i] - b.off[i]) * a.heads;
+    }
+    // a chunk with nothing to see
+    template <int HD>
+    __device__ __forceinline__ void put_nothing(int tid, int threads) const {
         if (a.ns > 1) {
             if (tid < rows) {
                 a.part[part_of(tid) * a.ns + chunk] = -INFINITY;
                 a.part[(a.rows + part_of(tid)) * a.ns + chunk] = 0.0f;
             }
         } else {
-            for (int e = tid; e < rows * HD; e += 64 * WAVES) a.out[slot_of(e / HD) * HD + e % HD] = 0.0f;
+            for (int e = tid; e < rows * HD; e += threads) a.out[slot_of(e / HD) * HD + e % HD] = 0.0f;
         }
-        return;
     }
-    const size_t head = ((size_t)b.seq[i] * c.nkv + h) * c.nb;
-    i32x4 kk[4][KD], vv[VD];
-    float ks, vs;
-    auto load_k = [&](int blk) {
-        const i32x4* p = (const i32x4*)(c.kc + (head + blk) * KV8_BLOCK * KR) + lane;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int d = 0; d < KD; ++d) kk[t][d] = Cols::load(p + (t * KD + d) * 64);
-        ks = c.ks[head + blk];
-    };
-    auto load_v = [&](int blk) {
-        const i32x4* p = (const i32x4*)(c.vc + (head + blk) * KV8_BLOCK * HD) + lane;
-#pragma unroll
-        for (int d = 0; d < VD; ++d) vv[d] = Cols::load(p + d * 64);
-        vs = c.vs[head + blk];
-    };
-    int blk = blk0 + wave;
-    if (blk < blk1) {
-        load_k(blk);
-        if (!LATE_V) load_v(blk);
+    // dims 4 q4 .. of row r: v, with the maximum M and the sum L that go with it
+    template <int HD>
+    __device__ __forceinline__ void put(int r, int q4, f32x4 v, float M, float L) const {
+        if (a.ns > 1) {
+            const size_t at = part_of(r) * a.ns + chunk;
+            if (q4 == 0) {
+                a.part[at] = M;
+                a.part[a.rows * a.ns + at] = L;
+            }
+            ((f32x4*)(a.part + 2 * a.rows * a.ns + at * HD))[q4] = v;
+        } else {
+            ((f32x4*)(a.out + slot_of(r) * HD))[q4] = v * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
+        }
     }
+    // not every row sees all of the block
+    __device__ __forceinline__ bool masked(int blk) const {
+        return blk * KV8_BLOCK + KV8_BLOCK - 1 > p0 || (a.window && blk * KV8_BLOCK < p1 - a.window + 1);
+    }
+};
 
-    // digits of the query rows, a wave a row, a lane 4 dims
-    constexpr int RW = (ROWS + WAVES - 1) / WAVES;
+// Digits of the tile's query rows into the columns of Cols (a wave a row, a
+// lane 4 dims), and the rows' largest magnitudes.  Ends with a barrier.
+template <int HD, class Cols, int N>
+__device__ __forceinline__ void put_queries(const Tile<Cols::ROWS>& tile, i32x4 (&qs)[N][kv8_k_row(HD) / 64][64],
+                                            uint32_t (&qmax)[Cols::ROWS], int lane, int wave) {
+    constexpr int KR = kv8_k_row(HD), ROWS = Cols::ROWS, WAVES = Cols::WAVES, RW = (ROWS + WAVES - 1) / WAVES;
     f32x4 x[RW];
 #pragma unroll
     for (int e = 0; e < RW; ++e) {
         const int r = wave + e * WAVES;
         x[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (r < rows && 4 * lane < HD) x[e] = ((const f32x4*)(a.q + slot_of(r) * HD))[lane];
+        if (r < tile.rows && 4 * lane < HD) x[e] = ((const f32x4*)(tile.a.q + tile.slot_of(r) * HD))[lane];
     }
 #pragma unroll
     for (int e = 0; e < RW; ++e) {
@@ -509,22 +444,107 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         for (int d = 0; d < 4; ++d) dg[d] = digits_of(fminf(fmaxf(x[e][d] * inv, -DIGIT_MAX), DIGIT_MAX));
         if (4 * lane < KR) {
 #pragma unroll
-            for (int n = 0; n < (ROWS == 4 ? 4 : 3); ++n)
+            for (int n = 0; n < Cols::PLACES; ++n)
                 ((uint32_t*)&qs[Cols::operand(n)][lane >> 4][(lane >> 2 & 3) * 16 + Cols::place(r, n)])[lane & 3] =
                     n < 3 ? byte_of(dg, n) ^ DIGIT_BIAS : 0u;
         }
         if (lane == 0) qmax[r] = m;
     }
     __syncthreads();
-    // score = q . k / sqrt(HD) in units of ln 2; a row that is not finite gives NaN
-    float qscale;
-    {
-        const uint32_t m = qmax[col.row];
-        qscale = m >= INF_BITS ? __uint_as_float(0x7fc00000u)
-                               : fmaxf(__uint_as_float(m), 0x1p-100f) * (1.44269504088896340736f / DIGIT_MAX / (HD == 32 ? 5.65685424949238f : HD == 64 ? 8.0f : HD == 128 ? 11.3137084989848f : 16.0f));
-        qscale = col.scaled(qscale);
+}
+
+// What turns a row's integer products into scores q . k / sqrt(HD) in units of
+// ln 2, but for the scale of K; NaN for a row that is not finite.
+template <int HD>
+__device__ __forceinline__ float query_scale(uint32_t m) {
+    constexpr float ROOT = HD == 32 ? 5.65685424949238f : HD == 64 ? 8.0f : HD == 128 ? 11.3137084989848f : 16.0f;
+    return m >= INF_BITS ? __uint_as_float(0x7fc00000u)
+                         : fmaxf(__uint_as_float(m), 0x1p-100f) * (1.44269504088896340736f / DIGIT_MAX / ROOT);
+}
+
+// The 16 columns of a product where a kv head has few query rows (decoding): 4
+// rows with their three digits side by side, column 4 n + r digit n of row r
+// and the last four zero.  A third of the products, and of the conversions of
+// their results, that a product for each digit would take.
+struct Narrow {
+    static constexpr int ROWS = 4, WAVES = 8, PLACES = 4;
+    int row, digit;
+    uint32_t lo, hi, bias;  // byte selectors of the lane's digit, and what its bytes are too large
+    float weight;
+    // each code is read once a call
+    __device__ __forceinline__ static i32x4 load(const i32x4* p) { return __builtin_nontemporal_load(p); }
+    __device__ __forceinline__ explicit Narrow(int col) : row(col & 3), digit(col >> 2) {
+        lo = digit == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * digit;
+        hi = digit == 3 ? 0x0c0c0c0cu : 0x04000c0cu + 0x01010000u * digit;
+        bias = digit < 2 ? DIGIT_BIAS : 0u;
+        weight = digit == 0 ? 1.0f : digit == 1 ? 256.0f : 65536.0f;
     }
-    const int pos = col.row < rows ? len - n_q + token_of(col.row) : -1;
+    // the lane's digit of four probabilities
+    __device__ __forceinline__ int share(const uint32_t* d) const {
+        return (int)((__builtin_amdgcn_perm(d[1], d[0], lo) | __builtin_amdgcn_perm(d[3], d[2], hi)) ^ bias);
+    }
+    // column of digit n of a query row
+    __device__ __forceinline__ static int place(int r, int n) { return 4 * n + r; }
+    __device__ __forceinline__ static int operand(int) { return 0; }
+    // The row's value from its digits' ones.  Its lanes have to get the same sum to the last bit, since each
+    // takes its own digit of the probability that comes of it: additions of
+    // the same values in either order, none fused with the product before.
+    __device__ __forceinline__ float join(float v) const {
+#pragma clang fp contract(off)
+        v = v + dpp<DPP_ROW_ROR8>(v);
+        return v + dpp<DPP_ROW_ROR4>(v);
+    }
+};
+
+// One workgroup: up to four query rows of one kv head x one chunk of key
+// blocks, the blocks dealt to its waves; each wave keeps its own running
+// maximum, sum and output, joined through LDS at the end.
+//   S^T = K Q^T   operand A: codes of 16 tokens, B: digits of the query rows;
+//                 lane (g, col) gets tokens 16 t + 4 g + i of its row
+//   O^T = V^T P^T operand A: codes of 16 dims, B: digits of the lane's own
+//                 16 probabilities (the layout of V has their order)
+// The codes of the next block are on their way while the present one is
+// worked on, as far as the registers reach.
+template <int HD>
+__global__ __launch_bounds__(64 * Narrow::WAVES, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
+    constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Narrow::ROWS, WAVES = Narrow::WAVES;
+    constexpr bool LATE_K = HD >= 128;
+    __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
+    __shared__ uint32_t qmax[ROWS];
+    __shared__ i32x4 qs[1][KD][64];
+    __shared__ __align__(16) float ob[WAVES][ROWS][HD + 4];
+    // grid: chunks, kv heads, entries
+    const int i = blockIdx.z, h = blockIdx.y;
+    const Tile<ROWS> tile(b, a, i, h, blockIdx.x, 0);
+    const int rows = tile.rows, blk1 = tile.blk1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
+    const Narrow col(lane & 15);
+    if (tile.blk0 >= blk1) return tile.put_nothing<HD>(tid, 64 * WAVES);
+    const size_t head = ((size_t)b.seq[i] * c.nkv + h) * c.nb;
+    i32x4 kk[4][KD], vv[VD];
+    float ks, vs;
+    auto load_k = [&](int blk) {
+        const i32x4* p = (const i32x4*)(c.kc + (head + blk) * KV8_BLOCK * KR) + lane;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < KD; ++d) kk[t][d] = Narrow::load(p + (t * KD + d) * 64);
+        ks = c.ks[head + blk];
+    };
+    auto load_v = [&](int blk) {
+        const i32x4* p = (const i32x4*)(c.vc + (head + blk) * KV8_BLOCK * HD) + lane;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) vv[d] = Narrow::load(p + d * 64);
+        vs = c.vs[head + blk];
+    };
+    int blk = tile.blk0 + wave;
+    if (blk < blk1) {
+        load_k(blk);
+        load_v(blk);
+    }
+    put_queries<HD, Narrow>(tile, qs, qmax, lane, wave);
+    const float qscale = query_scale<HD>(qmax[col.row]) * col.weight;
+    const int pos = col.row < rows ? tile.first + tile.token_of(col.row) : -1;
     const int from = a.window ? pos - a.window + 1 : 0;
     float m_run = -INFINITY, l_run = 0.0f;
     f32x4 o[VD];
@@ -537,22 +557,14 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         float s[16], mb = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            i32x4 acc[DIG];
+            i32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int n = 0; n < DIG; ++n) {
-                acc[n] = i32x4{0, 0, 0, 0};
+            for (int d = 0; d < KD; ++d) acc = mfma(kk[t][d], qs[0][d][at], acc);
 #pragma unroll
-                for (int d = 0; d < KD; ++d) {
-                    acc[n] = mfma(kk[t][d], qs[n][d][at], acc[n]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.join(rounded(col.sum(acc, j), f));
+            for (int j = 0; j < 4; ++j) s[4 * t + j] = col.join(rounded((float)acc[j], f));
         }
-        if (LATE_V) load_v(blk);
         if (!LATE_K && blk + WAVES < blk1) load_k(blk + WAVES);
-        // not every row sees all of the block
-        if (blk * KV8_BLOCK + KV8_BLOCK - 1 > p0 || (a.window && blk * KV8_BLOCK < p1 - a.window + 1)) {
+        if (tile.masked(blk)) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const int p = blk * KV8_BLOCK + 16 * (j / 4) + 4 * g + j % 4;
@@ -574,19 +586,17 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         for (int j = 0; j < 16; ++j) {
             const float e = exp2_fast(s[j] - top);
             lb += e;
-            pd[j] = digits_of_share(e);
+            pd[j] = digits_of_share(e, DIGIT_MAX);
         }
         const float m_new = fmaxf(m_run, mb);
         const float alpha = m_run == m_new ? 1.0f : exp2_fast(m_run - m_new);
         const float beta = mb == -INFINITY ? 0.0f : exp2_fast(mb - m_new);
         m_run = m_new;
         l_run = l_run * alpha + (mb == -INFINITY ? lb : lb * beta);
-        const float w = mb == -INFINITY ? 0.0f : col.scaled(beta * vs * (1.0f / DIGIT_MAX));
-        i32x4 pb[DIG];
+        const float w = mb == -INFINITY ? 0.0f : beta * vs * (1.0f / DIGIT_MAX) * col.weight;
+        i32x4 pb;
 #pragma unroll
-        for (int n = 0; n < DIG; ++n)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) pb[n][t] = col.share(pd + 4 * t, n);
+        for (int t = 0; t < 4; ++t) pb[t] = col.share(pd + 4 * t);
         __builtin_amdgcn_sched_barrier(0);  // scores and probabilities leave their registers here
         if (LATE_K && blk + WAVES < blk1) load_k(blk + WAVES);
         if (__any(alpha != 1.0f)) {
@@ -595,13 +605,11 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         }
 #pragma unroll
         for (int d = 0; d < VD; ++d) {
-            i32x4 acc[DIG];
+            const i32x4 acc = mfma(vv[d], pb, i32x4{0, 0, 0, 0});
 #pragma unroll
-            for (int n = 0; n < DIG; ++n) acc[n] = mfma(vv[d], pb[n], i32x4{0, 0, 0, 0});
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[d][j] = fmaf(col.sum(acc, j), w, o[d][j]);
+            for (int j = 0; j < 4; ++j) o[d][j] = fmaf((float)acc[j], w, o[d][j]);
         }
-        if (!LATE_V && blk + WAVES < blk1) load_v(blk + WAVES);
+        if (blk + WAVES < blk1) load_v(blk + WAVES);
     }
     // join the waves
     l_run += __shfl_xor(l_run, 16, 64);
@@ -610,74 +618,231 @@ __global__ __launch_bounds__(64 * Cols::WAVES, 2) void k_kv8_attention(Kv8Dev c,
         st_m[wave][col.row] = m_run;
         st_l[wave][col.row] = l_run;
     }
-    if constexpr (ROWS == 4) {
-        // the row's four lanes add their digits' parts; each writes a quarter (all of it where there are fewer)
-        constexpr int STEP = VD < 4 ? 1 : 4;
+    // the row's four lanes add their digits' parts; each writes a quarter (all of it where there are fewer)
+    constexpr int STEP = VD < 4 ? 1 : 4;
 #pragma unroll
-        for (int d = 0; d < VD; d += STEP) {
-            f32x4 v[STEP];
+    for (int d = 0; d < VD; d += STEP) {
+        f32x4 v[STEP];
 #pragma unroll
-            for (int e = 0; e < STEP; ++e)
+        for (int e = 0; e < STEP; ++e)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[e][j] = col.join(o[d + e][j]);
-            f32x4 mine = v[0];
-            if constexpr (STEP == 4) {
-                const f32x4 x = col.digit & 1 ? v[1] : v[0], y = col.digit & 1 ? v[3] : v[2];
-                mine = col.digit & 2 ? y : x;
-            }
-            *(f32x4*)&ob[wave][col.row][16 * (d + (STEP == 4 ? col.digit : 0)) + 4 * g] = mine;
+            for (int j = 0; j < 4; ++j) v[e][j] = col.join(o[d + e][j]);
+        f32x4 mine = v[0];
+        if constexpr (STEP == 4) {
+            const f32x4 x = col.digit & 1 ? v[1] : v[0], y = col.digit & 1 ? v[3] : v[2];
+            mine = col.digit & 2 ? y : x;
         }
+        *(f32x4*)&ob[wave][col.row][16 * (d + (STEP == 4 ? col.digit : 0)) + 4 * g] = mine;
     }
     __syncthreads();
-    auto weight = [&](int w, int r, float M) { return st_m[w][r] == -INFINITY ? 0.0f : exp2_fast(st_m[w][r] - M); };
-    auto put = [&](int r, int q4, f32x4 v, float M, float L) {  // dims 4 q4 .. of the tile's row r
-        if (a.ns > 1) {
-            const size_t at = part_of(r) * a.ns + chunk;
-            if (q4 == 0) {
-                a.part[at] = M;
-                a.part[a.rows * a.ns + at] = L;
-            }
-            ((f32x4*)(a.part + 2 * a.rows * a.ns + at * HD))[q4] = v;
-        } else {
-            ((f32x4*)(a.out + slot_of(r) * HD))[q4] = v * (M == -INFINITY && L == 0.0f ? 0.0f : 1.0f / L);
-        }
-    };
-    const int jr = ROWS == 4 ? tid / (HD / 4) : col.row;  // row that this thread joins
-    if (ROWS == 4 && jr >= rows) return;
+    const int jr = tid / (HD / 4), q4 = tid % (HD / 4);  // row and dims that this thread joins
+    if (jr >= rows) return;
     float M = -INFINITY, L = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) M = fmaxf(M, st_m[w][jr]);
-    if constexpr (ROWS == 4) {
-        const int q4 = tid % (HD / 4);
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float x = st_m[w][jr] == -INFINITY ? 0.0f : exp2_fast(st_m[w][jr] - M);
+        L += st_l[w][jr] * x;
+        v += *(const f32x4*)&ob[w][jr][4 * q4] * x;
+    }
+    tile.put<HD>(jr, q4, v, M, L);
+}
+
+// A scale that is the same for a wave, by a scalar load: a vector load would
+// come back behind the codes that are on their way.
+__device__ __forceinline__ float scalar_load(const float* p) {
+    return *(const __attribute__((address_space(4))) float*)(uintptr_t)p;
+}
+
+// The 16 columns where a kv head has more: a query row each, a product for
+// each digit.
+struct Wide {
+    static constexpr int ROWS = 16, WAVES = 4, PLACES = 3;
+    __device__ __forceinline__ static int place(int r, int) { return r; }
+    __device__ __forceinline__ static int operand(int n) { return n; }
+    // the digits' products together; each is below 2^24 (256 dims, or tokens)
+    __device__ __forceinline__ static float sum(int d0, int d1, int d2) {
+        return fmaf((float)d2, 65536.0f, (float)(d1 * 256 + d0));
+    }
+};
+
+// One workgroup: up to 16 query rows of one kv head x one chunk of key blocks,
+// four blocks a step.  A wave takes one of them for the scores, and a quarter
+// of the dims for all four of them: the probabilities' digits pass through
+// LDS.  So the integer sums of four blocks become floats once, no wave holds
+// more than a quarter of the output, and nothing is joined at the end.
+// The probabilities are relative to the step's largest, and carry the block's
+// share of the largest scale of V.
+// Bound by the conversions around the products and by the latency of one
+// phase behind the other, two workgroups a CU (256 dims; three and four for
+// 128 and 64): the matrix cores are busy for a third of the time, L2 gives 12
+// of the 33 TB/s that it could.  8192 tokens of 4 heads of 256 dims over one
+// kv head 334 us (430 TFLOP/s of the formula's), 4096 of 32 of 128 over 8: 370.
+// Four waves with blocks and outputs of their own, joined at the end: 325 and
+// 426; a prompt of 1907 tokens in a window of 1024 53 us (here 50), drafts for
+// 16 sequences of 2011 32 us (here 30).
+// ONCE: one tile a kv head, each code is read once a call.
+template <int HD, bool ONCE>
+__global__ __launch_bounds__(64 * Wide::WAVES, HD == 256 ? 2 : HD == 128 ? 3 : 4) void k_kv8_attention_wide(Kv8Dev c, Kv8Batch b, Att8 a) {
+    constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Wide::ROWS, WAVES = Wide::WAVES;
+    constexpr int DT = VD < WAVES ? 1 : VD / WAVES;  // 16-dim tiles a wave
+    __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
+    __shared__ uint32_t qmax[ROWS];
+    __shared__ i32x4 qs[3][KD][64], ps[WAVES][3][64];
+    // grid: kv heads, then the chunks, then the tiles, the longest (last) first; entries
+    const int i = blockIdx.z;
+    const unsigned by_head = blockIdx.x / (unsigned)c.nkv, by_chunk = a.ns > 1 ? by_head / (unsigned)a.ns : by_head;
+    const int h = blockIdx.x - by_head * c.nkv, t0 = a.tiles - 1 - by_chunk;
+    if (t0 * ROWS >= b.cnt[i] * a.group) return;
+    const Tile<ROWS> tile(b, a, i, h, by_head - by_chunk * a.ns, t0);
+    const int blk1 = tile.blk1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, row = lane & 15;
+    if (tile.blk0 >= blk1) return tile.put_nothing<HD>(tid, 64 * WAVES);
+    const size_t head = ((size_t)b.seq[i] * c.nkv + h) * c.nb;
+    const bool has_dims = VD >= WAVES || wave * DT < VD;
+    auto load = [](const i32x4* p) { return ONCE ? __builtin_nontemporal_load(p) : *p; };
+    i32x4 kk[4][KD], vv[WAVES][DT];
+    // a block's n-th kilobyte
+    const uint32_t lane16 = lane * 16;
+    auto kilo = [&](const int8_t* block, int n) { return load((const i32x4*)(block + n * 1024 + lane16)); };
+    auto load_k = [&](int blk) {
+        const int8_t* p = c.kc + (head + blk) * KV8_BLOCK * KR;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < KD; ++d) kk[t][d] = kilo(p, t * KD + d);
+    };
+    auto load_v = [&](int base) {  // the wave's dims; a block behind the last: the last once more
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            const float x = weight(w, jr, M);
-            L += st_l[w][jr] * x;
-            v += *(const f32x4*)&ob[w][jr][4 * q4] * x;
+            const int8_t* p = c.vc + (head + min(base + w, blk1 - 1)) * KV8_BLOCK * HD + wave * DT * 1024;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vv[w][d] = kilo(p, d);
         }
-        put(jr, q4, v, M, L);
-    } else {
+    };
+    if (tile.blk0 + wave < blk1) load_k(tile.blk0 + wave);
+    put_queries<HD, Wide>(tile, qs, qmax, lane, wave);
+    const float qscale = 256.0f * query_scale<HD>(qmax[row]);
+    const int pos = row < tile.rows ? tile.first + tile.token_of(row) : -1;
+    const int from = a.window ? pos - a.window + 1 : 0;
+    float m_run = -INFINITY, l_run = 0.0f;
+    f32x4 o[DT];
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) L += st_l[w][jr] * weight(w, jr, M);
-        const float mine = weight(wave, jr, M);
+    for (int d = 0; d < DT; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int base = tile.blk0; base < blk1; base += WAVES) {
+        const int blk = base + wave, blocks = min(blk1 - base, WAVES);
+        if (has_dims) load_v(base);
+        // the blocks' scales of V relative to the largest; one that is NaN is left out, and spoils the rows' sums instead
+        const float ks = scalar_load(c.ks + head + min(blk, blk1 - 1));
+        float vs[WAVES], top_vs = 0.0f;
 #pragma unroll
-        for (int d = 0; d < VD; ++d) o[d] *= mine;
-#pragma unroll 1
-        for (int half = WAVES / 2; half > 0; half >>= 1) {
-            if (wave >= half && wave < 2 * half)
-#pragma unroll
-                for (int d = 0; d < VD; ++d) *(f32x4*)&ob[wave - half][jr][16 * d + 4 * g] = o[d];
-            __syncthreads();
-            if (wave < half)
-#pragma unroll
-                for (int d = 0; d < VD; ++d) o[d] += *(const f32x4*)&ob[wave][jr][16 * d + 4 * g];
-            __syncthreads();
+        for (int w = 0; w < WAVES; ++w) {
+            vs[w] = scalar_load(c.vs + head + min(base + w, blk1 - 1));
+            top_vs = fmaxf(top_vs, vs[w]);
         }
-        if (wave != 0 || jr >= rows) return;
+        float s[16], mb = -INFINITY, f = 0.0f;
+        if (blk < blk1) {
+            f = qscale * ks;
+            f = f < 0x1p-126f ? 0x1p-126f : f;  // not zero: it meets -inf
+            // The lowest digit's sum goes on top of the next one's, but for its
+            // last 8 bits: an error below 2^-15 of q's largest magnitude times
+            // one code, for all dims together, and much the same for all keys.
+            i32x4 acc[4][3] = {};
+            auto step = [&](int n, int d) {
+                const i32x4 q = qs[n][d][lane];
 #pragma unroll
-        for (int d = 0; d < VD; ++d) put(jr, 4 * d + g, o[d], M, L);
+                for (int t = 0; t < 4; ++t) acc[t][n] = mfma(kk[t][d], q, acc[t][n]);
+            };
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+#pragma unroll
+                for (int t = 0; t < 4 && n == 1; ++t) acc[t][1] = acc[t][0] >> 8;
+#pragma unroll
+                for (int d = 0; d < KD; ++d) step(n, d);
+            }
+            if (blk + WAVES < blk1) load_k(blk + WAVES);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] = (float)(acc[j / 4][2][j % 4] * 256 + acc[j / 4][1][j % 4]);
+            if (tile.masked(blk)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int p = blk * KV8_BLOCK + 16 * (j / 4) + 4 * g + j % 4;
+                    s[j] = p <= pos && p >= from ? s[j] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mb = fmaxf(mb, s[j]);
+            mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
+            mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+            // nothing to see of the block: its scale, which may be NaN, has no say
+            if (mb == -INFINITY) f = 1.0f;
+            // in units of ln 2, and no less than any of them before its rounding
+            mb *= f;
+            mb = mb == -INFINITY ? mb : fmaf(fabsf(mb), 0x1p-23f, mb);
+        }
+        if (g == 0) st_m[wave][row] = mb;
+        __syncthreads();
+        const float ms = fmaxf(fmaxf(st_m[0][row], st_m[1][row]), fmaxf(st_m[2][row], st_m[3][row]));
+        // A row that sees nothing of the step has -inf for all its scores; one
+        // whose scores are all NaN has the same maximum, and its sum becomes NaN.
+        const float top = ms == -INFINITY ? 0.0f : ms;
+        const float m_new = fmaxf(m_run, ms);
+        const float alpha = m_run == m_new ? 1.0f : exp2_fast(m_run - m_new);
+        const float beta = ms == -INFINITY ? 0.0f : exp2_fast(ms - m_new);
+        m_run = m_new;
+        if (blk < blk1) {
+            const float mine = wave == 0 ? vs[0] : wave == 1 ? vs[1] : wave == 2 ? vs[2] : vs[3];
+            const float share = mine == mine ? mine / top_vs * DIGIT_MAX : 0.0f;
+            float lb = 0.0f;
+            uint32_t pd[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float e = exp2_fast(fmaf(s[j], f, -top));
+                lb += e;
+                pd[j] = digits_of_share(e, share);
+            }
+            if (mine != mine && mb != -INFINITY) lb = mine;
+            l_run = l_run * alpha + (ms == -INFINITY ? lb : lb * beta);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                i32x4 p;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) p[t] = (int)(n < 2 ? byte_of(pd + 4 * t, n) ^ DIGIT_BIAS : byte_of(pd + 4 * t, n));
+                ps[wave][n][lane] = p;
+            }
+        } else {
+            l_run *= alpha;
+        }
+        __syncthreads();
+        if (!has_dims) continue;
+        i32x4 sum[DT][3];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            if (w >= blocks) break;
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                const i32x4 p = ps[w][n][lane];
+#pragma unroll
+                for (int d = 0; d < DT; ++d) sum[d][n] = mfma(vv[w][d], p, w ? sum[d][n] : i32x4{0, 0, 0, 0});
+            }
+        }
+        const float w = beta * top_vs * (1.0f / DIGIT_MAX);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[d][j] = fmaf(Wide::sum(sum[d][0][j], sum[d][1][j], sum[d][2][j]), w, o[d][j] * alpha);
     }
+    // a row's sum: of its lanes, and of the waves' blocks
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (g == 0) st_l[wave][row] = l_run;
+    __syncthreads();
+    if (row >= tile.rows || !has_dims) return;
+    const float L = (st_l[0][row] + st_l[1][row]) + (st_l[2][row] + st_l[3][row]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) tile.put<HD>(row, 4 * (wave * DT + d) + g, o[d], m_run, L);
 }
 
 // Joins the chunk states of one output row: a workgroup takes 4 LN of its
@@ -775,9 +940,9 @@ int launch_kv8_read(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, int block
 
 int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, const Att8& a, hipStream_t s) {
     return with_hd(hd, [&](auto h) {
-        if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value, Narrow>), dim3(a.ns, c.nkv, n), dim3(64 * Narrow::WAVES), 0, s, c, b, a);
-        else if (a.tiles == 1) hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<true>>), dim3(a.ns * c.nkv, 1, n), dim3(64 * Wide<true>::WAVES), 0, s, c, b, a);
-        else hipLaunchKernelGGL((k_kv8_attention<h.value, Wide<false>>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide<false>::WAVES), 0, s, c, b, a);
+        if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value>), dim3(a.ns, c.nkv, n), dim3(64 * Narrow::WAVES), 0, s, c, b, a);
+        else if (a.tiles == 1) hipLaunchKernelGGL((k_kv8_attention_wide<h.value, true>), dim3(a.ns * c.nkv, 1, n), dim3(64 * Wide::WAVES), 0, s, c, b, a);
+        else hipLaunchKernelGGL((k_kv8_attention_wide<h.value, false>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide::WAVES), 0, s, c, b, a);
         // few chunks: a row a workgroup (of 64 rows or more, so that they fill the device)
         constexpr int LN = h.value / 4;
         const unsigned rows = (unsigned)a.most_q * a.heads;
