@@ -53,14 +53,32 @@ int check_not_capturing(const char* fn, gh_ctx* ctx) {
 }
 
 // Blocks a workgroup of the attention takes at most.  `most`: of the longest
-// tile; `work`: of all `wgs` (entry, kv head, row tile) together.
+// tile; `work`: of all `wgs` (entry, kv head, row tile) together.  A kv head's
+// keys are cut into chunks where there are too few workgroups to fill the
+// device, which costs a second launch of 4 us to join them.  Call times in us,
+// 128 dims and 8 kv heads unless said otherwise:
+//  - tile 4, a wave a block, eight of them side by side: uncut up to 16 blocks
+//    (1024 tokens, 256 dims: 22, by eights 24), or where the uncut workgroups
+//    fill the device in nearly whole rounds (32 sequences of 4096: 56, cut in
+//    two 60), if the longest is not far from the average; else as many chunks
+//    as fill it once, of 8 blocks at least (one sequence of 131072 tokens: 59,
+//    by eights 72, uncut 590; 64 of 4096 with one head of 256 dims: 40, by
+//    eights 43, uncut 58).
+//  - tile 16, four blocks a step: uncut up to two steps (a prompt of 300: 24,
+//    by fours 28) or from a workgroup a CU on (64 sequences of 1024, 4 tokens
+//    each: 30, in halves 37; a prompt of 1024: 31, in halves 48), but for long
+//    ones short of two a CU (16 sequences of 32768 with drafts of 5: 223 by 64
+//    blocks, 280 uncut); else as many as fill it twice (one of 32768 with a
+//    draft of 5: 36, by fours 45, uncut 243).
 int kv8_chunk(int hd, int tile, int most, int64_t work, int64_t wgs) {
+    const bool even = most * wgs <= 2 * work;
+    auto fill = [&](int64_t n, int least) { return (int)std::max<int64_t>(least, (work + n - 1) / n); };
     if (tile == 4) {
         const int64_t slots = hd <= 64 ? 512 : 256, rounds = (wgs + slots - 1) / slots;
-        const bool full = wgs * 10 >= 9 * rounds * slots && most * wgs * 10 <= 11 * work;
-        return most <= 16 || full ? std::max(most, 1) : (int)std::max<int64_t>(8, (work + 767) / 768);
+        return most <= 16 || (wgs * 10 >= 9 * rounds * slots && even) ? std::max(most, 1) : fill(slots, 8);
     }
-    return (int)std::max<int64_t>(4, (work + 511) / 512);
+    if (most <= 8 || (even && wgs >= (most <= 64 ? 256 : 512))) return std::max(most, 1);
+    return wgs < 256 ? fill(512, 4) : fill(2048, 64);
 }
 
 // How many of the entries from `at` on one launch takes, their sizes
