@@ -1,10 +1,22 @@
 // Host side of the batched sampler: the checks of its rules.
+#include <algorithm>
 #include <cmath>
 
 #include "host.h"
 #include "sampling.h"
 
 using namespace gh;
+
+namespace {
+
+// How much work a row is likely to be: weights of the whole row, a list of its
+// first elements, its largest one.
+int work_of(const gh_sampling& r) {
+    if (r.temperature == 0.0f) return 0;
+    return r.top_k == 0 || r.top_k > SMP_GROUPS / 4 ? 2 : 1;
+}
+
+}  // namespace
 
 extern "C" int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, int32_t vocab, const gh_sampling* rules,
                               int32_t* tokens_out) {
@@ -29,7 +41,14 @@ extern "C" int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, 
     for (int i = 0; i < n_rows; i += SMP_BATCH) {
         SmpRules b;
         const int m = std::min(n_rows - i, SMP_BATCH);
-        std::copy(rules + i, rules + i + m, b.r);
+        // Rows of like work one behind the other, so that each CU gets some of
+        // every kind: in the caller's order those with the same rules may meet
+        // on the same CUs (64 rows whose rules repeat every fourth: 86 us
+        // so, 76 in this).
+        int at = 0;
+        for (int work = 2; work >= 0; --work)
+            for (int j = 0; j < m; ++j)
+                if (work_of(rules[i + j]) == work) b.r[at++] = {rules[i + j], j};
         GH_CHECK(launch_sample_rows(logits + (size_t)i * vocab, m, vocab, b, (SmpRow*)scratch, tokens_out + i, ctx->stream));
     }
     return op_sync(ctx);

@@ -5,10 +5,14 @@
 
 namespace gh {
 
-// Rules of up to SMP_BATCH rows, by value in a kernel's arguments.
+// Up to SMP_BATCH rows in the order in which their workgroups start, by value
+// in a kernel's arguments: each one's rules, and which of the call's it is.
 constexpr int SMP_BATCH = 128;
+struct SmpRule : gh_sampling {
+    int row;
+};
 struct SmpRules {
-    gh_sampling r[SMP_BATCH];
+    SmpRule r[SMP_BATCH];
 };
 
 constexpr int SMP_MAX_VOCAB = 1 << 24;

@@ -21,8 +21,6 @@
 // run all steps in one kernel (k_smp_row).
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "sampling.h"
 
 namespace gh {
@@ -92,13 +90,52 @@ struct Bins {
     __device__ __forceinline__ int of(float l) const { return min((int)place(l), SMP_BINS - 1); }
 };
 
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int o) {
-    const unsigned lo = __shfl_xor((unsigned)v, o, 64), hi = __shfl_xor((unsigned)(v >> 32), o, 64);
+// Values of other lanes without a trip through LDS, whose latency the chains of
+// a sort or a sum would wait for at every step.  All lanes are active.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, ROWS == 0xF);
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR3 = 0x1B, DPP_XOR7 = 0x141, DPP_XOR8 = 0x128;
+constexpr int DPP_UP = 0x110, DPP_ROW_LAST = 0x142, DPP_HALF_LAST = 0x143;
+
+// v of lane ^ o; o a power of two below 64
+__device__ __forceinline__ unsigned lane_xor(unsigned v, int o) {
+    switch (o) {
+        case 1: return dpp<DPP_XOR1>(v);
+        case 2: return dpp<DPP_XOR2>(v);
+        case 4: return dpp<DPP_XOR3>(dpp<DPP_XOR7>(v));
+        case 8: return dpp<DPP_XOR8>(v);
+        case 16: {
+            const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+            return threadIdx.x & 16 ? r[0] : r[1];
+        }
+        default: {
+            const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+            return threadIdx.x & 32 ? r[0] : r[1];
+        }
+    }
+}
+__device__ __forceinline__ u64 lane_xor(u64 v, int o) {
+    const unsigned lo = lane_xor((unsigned)v, o), hi = lane_xor((unsigned)(v >> 32), o);
     return ((u64)hi << 32) | lo;
 }
-__device__ __forceinline__ u64 shfl_up64(u64 v, int o) {
-    const unsigned lo = __shfl_up((unsigned)v, o, 64), hi = __shfl_up((unsigned)(v >> 32), o, 64);
+__device__ __forceinline__ float lane_xor(float v, int o) { return __uint_as_float(lane_xor(__float_as_uint(v), o)); }
+
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ u64 dpp(u64 v) {
+    const unsigned lo = dpp<CTRL, ROWS>((unsigned)v), hi = dpp<CTRL, ROWS>((unsigned)(v >> 32));
     return ((u64)hi << 32) | lo;
+}
+// inclusive running sums over the wave's lanes
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp<DPP_UP + 1>(v);
+    v += dpp<DPP_UP + 2>(v);
+    v += dpp<DPP_UP + 4>(v);
+    v += dpp<DPP_UP + 8>(v);
+    v += dpp<DPP_ROW_LAST, 0xA>(v);
+    return v + dpp<DPP_HALF_LAST, 0xC>(v);
 }
 
 // LDS of a workgroup's reductions, of its bins, and of the list.
@@ -118,7 +155,7 @@ struct BinSums {
 template <int NT, class Op>
 __device__ __forceinline__ u64 block_reduce(u64 v, Small& sh, Op op) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, shfl_xor64(v, o));
+    for (int o = 32; o > 0; o >>= 1) v = op(v, lane_xor(v, o));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -132,12 +169,8 @@ __device__ __forceinline__ u64 block_reduce(u64 v, Small& sh, Op op) {
 template <int NT>
 __device__ __forceinline__ void block_scan(u64& m, unsigned& c, Small& sh) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 a = shfl_up64(m, o);
-        const unsigned b = __shfl_up(c, o, 64);
-        if (lane >= o) m += a, c += b;
-    }
+    m = wave_scan(m);
+    c = wave_scan(c);
     __syncthreads();
     if (lane == 63) sh.red[w] = m, sh.red32[w] = c;
     __syncthreads();
@@ -202,13 +235,9 @@ __device__ __forceinline__ void each_logit(const float* l, int i0, int i1, F&& f
 
 // largest over 16 lanes
 __device__ __forceinline__ float max16(float v) {
-    auto turned = [](float x, auto by) {
-        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + by.value, 0xF, 0xF, true));
-    };
-    v = fmaxf(v, turned(v, std::integral_constant<int, 8>{}));
-    v = fmaxf(v, turned(v, std::integral_constant<int, 4>{}));
-    v = fmaxf(v, turned(v, std::integral_constant<int, 2>{}));
-    return fmaxf(v, turned(v, std::integral_constant<int, 1>{}));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, lane_xor(v, o));
+    return v;
 }
 
 // dead: the distance from the largest at which a weight is zero.  Masked
@@ -266,8 +295,8 @@ __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, float
     unsigned bad = __any(nan);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-        first = min(first, shfl_xor64(first, o));
-        low = fminf(low, __shfl_xor(low, o, 64));
+        first = min(first, lane_xor(first, o));
+        low = fminf(low, lane_xor(low, o));
     }
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
@@ -504,12 +533,7 @@ __device__ __forceinline__ void scan_counts(unsigned* count, Small& sh) {
     unsigned c[PER], sum = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) sum += c[j] = count[b0 + j];
-    unsigned run = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned a = __shfl_up(run, o, 64);
-        if (lane >= o) run += a;
-    }
+    unsigned run = wave_scan(sum);
     if (lane == 63) sh.red32[w] = run;
     __syncthreads();
     run -= sum;
@@ -583,54 +607,74 @@ struct PickShared {
     int at[4];
 };
 
-// ascending, in LDS; n <= SMP_LIST.  Steps between elements of one wave's 64
-// need no barrier: the wave's own order suffices.
-__device__ __forceinline__ void sort_list(u64* list, int n) {
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += PT) list[i] = ~0ull;
-    __syncthreads();
-    const int tid = threadIdx.x;
-    if (size <= PT) {  // one element a thread
-        u64 x = tid < size ? list[tid] : ~0ull;
-        for (int k = 2; k <= size; k *= 2) {
-            for (int j = k / 2; j > 0; j /= 2) {
-                u64 y;
-                if (j >= 64) {
-                    __syncthreads();
-                    if (tid < size) list[tid] = x;
-                    __syncthreads();
-                    y = tid < size ? list[tid ^ j] : ~0ull;
-                } else {
-                    y = shfl_xor64(x, j);
-                }
-                const bool up = (tid & k) == 0, lower = (tid & j) == 0;
-                x = (x < y) == (up == lower) ? x : y;
-            }
-        }
-        __syncthreads();
-        if (tid < size) list[tid] = x;
-        __syncthreads();
-        return;
-    }
-    for (int k = 2; k <= size; k *= 2) {
-        for (int j = k / 2; j > 0; j /= 2) {
-            for (int t = tid; t < size / 2; t += PT) {
-                const int a = 2 * t - (t & (j - 1)), b = a + j;  // a has a 0 where b has a 1
-                const u64 x = list[a], y = list[b];
-                if ((x > y) == ((a & k) == 0)) list[a] = y, list[b] = x;
-            }
-            __syncthreads();
-        }
+// One merge of a bitonic sort within the wave's lanes: runs of k elements
+// around `at`, the distances of a half run and less.
+__device__ __forceinline__ void merge_lanes(u64& x, int k, int at) {
+#pragma unroll
+    for (int j = 32; j > 0; j >>= 1) {
+        if (j >= k) continue;
+        const u64 y = lane_xor(x, j);
+        const bool up = (at & k) == 0, lower = (at & j) == 0;
+        x = (x < y) == (up == lower) ? x : y;
     }
 }
 
-// The token, from the sorted list and the running sums of the bins in front
+// ascending, in LDS; n <= PER * PT.  A thread holds PER elements PT apart, so
+// that only the distances from 64 to PT / 2 pass through LDS.
+template <int PER>
+__device__ __forceinline__ void sort_list(u64* list, int n) {
+    const int tid = threadIdx.x;
+    int size = PER > 1 ? PER * PT : 64;
+    while (size < n) size *= 2;
+    u64 x[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x[e] = tid + e * PT < n ? list[tid + e * PT] : ~0ull;
+    for (int k = 2; k <= size; k *= 2) {
+        int j = k / 2;
+#pragma unroll
+        for (int half = PER / 2; half > 0; half /= 2) {
+            if (j < half * PT) continue;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                if (e & half) continue;
+                const bool up = ((tid + e * PT) & k) == 0;
+                const u64 lo = min(x[e], x[e + half]), hi = max(x[e], x[e + half]);
+                x[e] = up ? lo : hi;
+                x[e + half] = up ? hi : lo;
+            }
+            j = half * PT / 2;
+        }
+        for (; j >= 64; j /= 2) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                if (PER > 1 || tid < size) list[tid + e * PT] = x[e];
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const int i = tid + e * PT;
+                const u64 y = PER > 1 || tid < size ? list[i ^ j] : ~0ull;
+                const bool up = (i & k) == 0, lower = (i & j) == 0;
+                x[e] = (x[e] < y) == (up == lower) ? x[e] : y;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < PER; ++e) merge_lanes(x[e], k, tid + e * PT);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        if (PER > 1 || tid < size) list[tid + e * PT] = x[e];
+    __syncthreads();
+}
+
+// The token, from the list and the running sums of the bins in front
 // of its elements (LDS or global; none for a list that begins with the row's
 // first element and leaves none out), PER elements a thread.
 template <int PER>
 __device__ __forceinline__ int pick(const Weights& w, const Bins& bins, const gh_sampling& rule, const SmpCuts& cuts,
                                     const u64* mass, const unsigned* count, int n, PickShared& p, Small& sh) {
+    sort_list<PER>(p.list, n);
     auto bin_of = [&](float v) { return mass ? bins.of(v) : 0; };
     const int tid = threadIdx.x;
     u64 upto[PER];       // running mass up to and with the element
@@ -758,24 +802,12 @@ __device__ __forceinline__ int pick_wave(const Weights& w, const Bins& bins, con
     const int lane = threadIdx.x & 63;
     if (lane >= n) key = ~0ull;
 #pragma unroll 1
-    for (int k = 2; k <= 64; k *= 2) {
-#pragma unroll 1
-        for (int j = k / 2; j > 0; j /= 2) {
-            const u64 y = shfl_xor64(key, j);
-            const bool up = (lane & k) == 0, lower = (lane & j) == 0;
-            key = (key < y) == (up == lower) ? key : y;
-        }
-    }
+    for (int k = 2; k <= 64; k *= 2) merge_lanes(key, k, lane);
     const bool in = lane < n;
     const float val = in ? key_value((unsigned)(key >> 32)) : 0.0f;
     const double real = in ? w.real(val) : 0.0;
     const u64 m = in ? w.fixed(val) : 0;
-    u64 upto = m;
-#pragma unroll 1
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 a = shfl_up64(upto, o);
-        if (lane >= o) upto += a;
-    }
+    u64 upto = wave_scan(m);
     const u64 listed = ((u64)(unsigned)__shfl((int)(upto >> 32), 63, 64) << 32) | (unsigned)__shfl((int)upto, 63, 64);
     int rank = lane + 1;
     if (mass) {  // on top of the bins in front: what the bin's first element lacks, for those behind it too
@@ -922,12 +954,13 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
     } u;
     __shared__ u64 near[SMP_BINS];
     __shared__ unsigned listed_row;
-    const gh_sampling rule = rules.r[blockIdx.x];
-    const float* l = logits + (size_t)blockIdx.x * n;
+    const SmpRule rule = rules.r[blockIdx.x];
+    const int at = rule.row;
+    const float* l = logits + (size_t)at * n;
     const int tid = threadIdx.x;
     const Stat s = range_stat<PT>(l, 0, n, dead_of(bits, rule.temperature), sh);
     if (!drawn(s, rule)) {
-        if (tid == 0) tokens[blockIdx.x] = token_of_undrawn(s);
+        if (tid == 0) tokens[at] = token_of_undrawn(s);
         return;
     }
     const Weights w = weights_of(s, rule, bits);
@@ -956,13 +989,12 @@ __global__ __launch_bounds__(PT) void k_smp_row(const float* logits, int n, int 
         if (tid >= 64) return;
         t = pick_wave(w, bins, rule, cuts, mass, h.count, u.p.list[tid], listed);
     } else if (listed <= SMP_LIST) {
-        sort_list(u.p.list, listed);
         t = listed <= PT ? pick<1>(w, bins, rule, cuts, mass, h.count, listed, u.p, sh)
                          : pick<SMP_LIST / PT>(w, bins, rule, cuts, mass, h.count, listed, u.p, sh);
     } else {
         t = slow_row(l, n, w, bins, rule, u.slow, sh);
     }
-    if (tid == 0) tokens[blockIdx.x] = t;
+    if (tid == 0) tokens[at] = t;
 }
 
 __device__ __forceinline__ int chunk_begin(int n, int c, int chunks) { return (int)((int64_t)n * c / chunks); }
@@ -975,10 +1007,11 @@ __global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, int
     const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
     SmpRow& r = rows[blockIdx.y];
     for (int b = c * CT + tid; b < SMP_BINS; b += chunks * CT) r.mass[b] = 0, r.count[b] = 0;
-    const Stat s = range_stat<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks),
-                                   dead_of(bits, rules.r[blockIdx.y].temperature), sh);
+    const SmpRule rule = rules.r[blockIdx.y];
+    const Stat s = range_stat<CT>(logits + (size_t)rule.row * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks),
+                                  dead_of(bits, rule.temperature), sh);
     float own = s.own;
-    for (int o = 1; o < group; o <<= 1) own = fmaxf(own, __shfl_xor(own, o, 64));
+    for (int o = 1; o < group; o <<= 1) own = fmaxf(own, lane_xor(own, o));
     if (tid % group == 0) r.group_max[(c * CT + tid) / group] = own;
     if (tid == 0) {
         r.first[c] = s.first;
@@ -997,8 +1030,8 @@ __device__ __forceinline__ Stat row_stat(const SmpRow& r, int chunks) {
     const bool nan = __any(in && r.nan[lane]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-        first = min(first, shfl_xor64(first, o));
-        low = fminf(low, __shfl_xor(low, o, 64));
+        first = min(first, lane_xor(first, o));
+        low = fminf(low, lane_xor(low, o));
     }
     return {first, low, nan, 0.0f};
 }
@@ -1008,13 +1041,13 @@ __global__ __launch_bounds__(CT) void k_smp_hist(const float* logits, int n, int
     __shared__ Small sh;
     __shared__ BinSums h;
     const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
-    const gh_sampling rule = rules.r[blockIdx.y];
+    const SmpRule rule = rules.r[blockIdx.y];
     SmpRow& r = rows[blockIdx.y];
     const Stat s = row_stat(r, chunks);
     if (!drawn(s, rule)) return;
     const Weights w = weights_of(s, rule, bits);
     const Bins bins = bins_of(s, w);
-    const float* l = logits + (size_t)blockIdx.y * n;
+    const float* l = logits + (size_t)rule.row * n;
     const int i0 = chunk_begin(n, c, chunks), i1 = chunk_begin(n, c + 1, chunks);
     const Short row = short_row<CT>(r.group_max, groups, w, bins, rule, h, sh);
     if (tid == 0) sh.n_list = 0;
@@ -1039,7 +1072,7 @@ __global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, i
     __shared__ Small sh;
     __shared__ u64 near[SMP_BINS];
     const int c = blockIdx.x, chunks = gridDim.x, tid = threadIdx.x;
-    const gh_sampling rule = rules.r[blockIdx.y];
+    const SmpRule rule = rules.r[blockIdx.y];
     SmpRow& r = rows[blockIdx.y];
     const Stat s = row_stat(r, chunks);
     if (!drawn(s, rule) || r.is_short) return;
@@ -1053,7 +1086,7 @@ __global__ __launch_bounds__(CT) void k_smp_gather(const float* logits, int n, i
     }
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
-    range_gather<CT>(logits + (size_t)blockIdx.y * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
+    range_gather<CT>(logits + (size_t)rule.row * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks), bins, cuts,
                      r.list, &r.n_list, near, sh);
 }
 
@@ -1064,14 +1097,14 @@ __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int
         PickShared p;
         SlowShared slow;
     } u;
-    const gh_sampling rule = rules.r[blockIdx.x];
+    const SmpRule rule = rules.r[blockIdx.x];
     const SmpRow& r = rows[blockIdx.x];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, at = rule.row;
     const u64 key = r.list[tid];
     const Stat s = row_stat(r, chunks);
     const unsigned listed = r.n_list;
     if (!drawn(s, rule)) {
-        if (tid == 0) tokens[blockIdx.x] = token_of_undrawn(s);
+        if (tid == 0) tokens[at] = token_of_undrawn(s);
         return;
     }
     const Weights w = weights_of(s, rule, bits);
@@ -1086,13 +1119,12 @@ __global__ __launch_bounds__(PT) void k_smp_pick(const float* logits, int n, int
     } else if (listed <= SMP_LIST) {
         for (int i = tid; i < (int)listed; i += PT) u.p.list[i] = i < PT ? key : r.list[i];
         __syncthreads();
-        sort_list(u.p.list, listed);
         t = listed <= PT ? pick<1>(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh)
                          : pick<SMP_LIST / PT>(w, bins, rule, cuts, mass, r.run_count, listed, u.p, sh);
     } else {
-        t = slow_row(logits + (size_t)blockIdx.x * n, n, w, bins, rule, u.slow, sh);
+        t = slow_row(logits + (size_t)at * n, n, w, bins, rule, u.slow, sh);
     }
-    if (tid == 0) tokens[blockIdx.x] = t;
+    if (tid == 0) tokens[at] = t;
 }
 
 }  // namespace
