@@ -43,7 +43,7 @@ extern "C" int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, 
         const int m = std::min(n_rows - i, SMP_BATCH);
         // Rows of like work one behind the other, so that each CU gets some of
         // every kind: in the caller's order those with the same rules may meet
-        // on the same CUs (64 rows whose rules repeat every fourth: 86 us
+        // on the same CUs (64 rows whose rules repeat: 86 us
         // so, 76 in this).
         int at = 0;
         for (int work = 2; work >= 0; --work)

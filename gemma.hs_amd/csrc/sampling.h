@@ -46,12 +46,16 @@ struct SmpRow {
     SmpCuts cuts;
     unsigned n_list;
     int is_short;  // 0: long; 1: the list has all the mass that counts; 2: mass[0] has the row's
-    unsigned pad[4];
 };
 
-// Workgroups a row; 0: one, which runs every step (no scratch).
+// Workgroups a row; 0: one, which runs every step in one launch (no scratch).
+// It saves three launches, and reads the row three times alone: 8 rows of
+// 16384 logits take 30 us so and 36 by chunks, a single one of 32000 37 and 31
+// (top-k 26 and 29), 64 of 32000 38 and 40.  Each chunk clears, fills and adds
+// up bins of its own: 4096 logits for a few rows (one of 262144 33.2 us, by
+// 8192 33.9), 8192 for more (16 rows 43, by 4096 49, by 16384 44).
 inline int smp_chunks(int n_rows, int vocab) {
-    if (vocab <= 16384) return 0;
+    if (vocab <= (n_rows <= 4 ? 20000 : 32768)) return 0;
     const int least = n_rows <= 4 ? 4096 : 8192;  // logits a workgroup
     return std::max(1, std::min({SMP_CHUNKS, 1024 / n_rows, (vocab + least - 1) / least}));
 }

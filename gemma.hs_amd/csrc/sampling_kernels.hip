@@ -1011,7 +1011,9 @@ __global__ __launch_bounds__(CT) void k_smp_stat(const float* logits, int n, int
     const Stat s = range_stat<CT>(logits + (size_t)rule.row * n, chunk_begin(n, c, chunks), chunk_begin(n, c + 1, chunks),
                                   dead_of(bits, rule.temperature), sh);
     float own = s.own;
-    for (int o = 1; o < group; o <<= 1) own = fmaxf(own, lane_xor(own, o));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+        if (o < group) own = fmaxf(own, lane_xor(own, o));
     if (tid % group == 0) r.group_max[(c * CT + tid) / group] = own;
     if (tid == 0) {
         r.first[c] = s.first;

@@ -119,7 +119,7 @@ int launch_sample_rows(const float* l, int n_rows, int vocab, const SmpRules&, S
     ++launches;
     WANT(l && t && n_rows > 0 && n_rows <= SMP_BATCH);
     const int chunks = smp_chunks(n_rows, vocab);
-    WANT(chunks <= SMP_CHUNKS && (chunks == 0) == (vocab <= 16384));
+    WANT(chunks <= SMP_CHUNKS && (chunks > 0 || vocab <= 32768));
     if (chunks) {
         WANT(scratch != nullptr);
         if (scratch) std::memset(scratch, 0, sizeof(SmpRow) * n_rows);

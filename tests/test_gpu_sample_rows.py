@@ -71,7 +71,7 @@ def mixed(rng, rows, vocab):
 
 
 @pytest.mark.parametrize("ties", [False, True])
-@pytest.mark.parametrize("vocab", [1, 2, 3, 63, 64, 65, 1000, 1024, 4097, 32003])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 63, 64, 65, 1000, 1024, 4097, 32003, 40007])
 def test_mixed_rules(ctx, vocab, ties):
     rng = np.random.default_rng(vocab + ties)
     check(ctx, logits(rng, 40, vocab, ties=ties), mixed(rng, 40, vocab))
