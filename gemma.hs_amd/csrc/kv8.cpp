@@ -14,7 +14,8 @@ constexpr int MAX_SEQ = 1 << 22;   // tokens a sequence
 constexpr int MAX_ROWS = 1 << 20;  // query rows a kv head and sequence
 constexpr int MAX_GROUP = 1024;    // heads a kv head: rows * group stays below 2^32 (Att8::group_inv)
 constexpr int WASTE = 4096;        // empty workgroups that cost about what another launch does
-constexpr int MAX_GRID = 1 << 23;  // workgroups of 256 threads in a grid's x (2^32 threads at most)
+constexpr int64_t MAX_QUERIES = 1 << 27;  // query rows of a sequence, all heads: 2^23 tiles
+constexpr int64_t MAX_GRID = (1 << 24) - 1;  // workgroups of 256 threads in a grid's x (below 2^32 threads)
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -81,23 +82,6 @@ int kv8_chunk(int hd, int tile, int most, int64_t work, int64_t wgs) {
     return wgs < 256 ? fill(512, 4) : fill(2048, 64);
 }
 
-// How many of the entries from `at` on one launch takes, their sizes
-// descending: its grid has as many workgroups for each as for the first, so
-// that small ones behind a large one would be passed over in empty workgroups,
-// a microsecond a thousand.  A prompt of 16384 tokens among 239 single ones
-// is appended in 591 us by one launch, in 107 by these.
-// `heads`: workgroups of size 1.
-int launch_end(const int* size, int at, int n, int64_t heads) {
-    int64_t sum = size[at];
-    int end = at + 1;
-    for (; end < n; ++end) {
-        const int64_t grid = (int64_t)size[at] * (end + 1 - at);
-        sum += size[end];
-        if ((grid - sum) * heads > std::max<int64_t>(sum * heads, WASTE)) break;
-    }
-    return end;
-}
-
 int blocks_of(int begin, int end) {  // blocks that [begin, end) touches
     return end > begin ? (end - 1) / KV8_BLOCK - begin / KV8_BLOCK + 1 : 0;
 }
@@ -105,7 +89,8 @@ int blocks_of(int begin, int end) {  // blocks that [begin, end) touches
 // One entry of an append, a read or an attention.
 struct Entry {
     int seq, pos, off, cnt;  // as in Kv8Batch
-    int size, blocks;        // of the grid, and (attention) of the keys
+    int x, y;                // extents in the grid
+    int blocks;              // attention: of keys
 };
 
 void to_batch(const Entry* e, int n, Kv8Batch& b) {
@@ -120,30 +105,43 @@ void to_batch(const Entry* e, int n, Kv8Batch& b) {
     }
 }
 
-int most_blocks(const Entry* e, int n) {
-    int most = 0;
-    for (int i = 0; i < n; ++i) most = std::max(most, e[i].size);
-    return most;
-}
-
-// launch(entries, n) of the entries that have tokens, in launches of like sizes.
+// launch(entries, n) of the entries that have tokens, in launches of like
+// sizes: a grid has as many workgroups for each as for the largest, so that
+// small ones beside a large one would be passed over in empty workgroups, a
+// microsecond a thousand.  A prompt of 16384 tokens among 239 single ones is
+// appended in 591 us by one launch, in 107 so.  A size is the product of two
+// extents of the grid; `heads` is its third.
 template <class F>
 int launch_by_size(Entry* e, int n, int64_t heads, F&& launch) {
-    int size[KV8_BATCH], most = 0;
-    int64_t sum = 0;
     n = (int)(std::remove_if(e, e + n, [](const Entry& x) { return x.cnt == 0; }) - e);
+    auto wasted = [&](int64_t grid, int64_t sum) { return (grid - sum) * heads > std::max<int64_t>(sum * heads, WASTE); };
+    int64_t x = 0, y = 0, sum = 0;
     for (int i = 0; i < n; ++i) {
-        most = std::max(most, e[i].size);
-        sum += e[i].size;
+        x = std::max<int64_t>(x, e[i].x);
+        y = std::max<int64_t>(y, e[i].y);
+        sum += (int64_t)e[i].x * e[i].y;
     }
-    const bool one = ((int64_t)most * n - sum) * heads <= std::max<int64_t>(sum * heads, WASTE);
-    if (!one) std::stable_sort(e, e + n, [](const Entry& x, const Entry& y) { return x.size > y.size; });
-    for (int i = 0; i < n; ++i) size[i] = e[i].size;
+    if (n == 0 || !wasted(x * y * n, sum)) return n ? launch(e, n) : GH_OK;
+    std::stable_sort(e, e + n, [](const Entry& a, const Entry& b) { return (int64_t)a.x * a.y > (int64_t)b.x * b.y; });
     for (int at = 0, end; at < n; at = end) {
-        end = one ? n : launch_end(size, at, n, heads);
+        x = y = sum = 0;
+        for (end = at; end < n; ++end) {
+            const int64_t x1 = std::max<int64_t>(x, e[end].x), y1 = std::max<int64_t>(y, e[end].y);
+            const int64_t sum1 = sum + (int64_t)e[end].x * e[end].y;
+            if (end > at && wasted(x1 * y1 * (end + 1 - at), sum1)) break;
+            x = x1;
+            y = y1;
+            sum = sum1;
+        }
         GH_CHECK(launch(e + at, end - at));
     }
     return GH_OK;
+}
+
+int most_blocks(const Entry* e, int n) {
+    int most = 0;
+    for (int i = 0; i < n; ++i) most = std::max(most, e[i].x);
+    return most;
 }
 
 // Key blocks that a row tile of the entry may see: up to the window and the
@@ -155,26 +153,38 @@ int keys_of(const Entry& e, const Att8& a, int tile) {
 
 int tiles_of(const Entry& e, const Att8& a, int tile) { return (e.cnt * a.group + tile - 1) / tile; }
 
+// Sums over some entries, whose blocks and row tiles are set, and the chunks
+// that follow.
+struct Work {
+    int most = 0, tiles = 0;    // blocks of the longest row tile, tiles of the longest entry
+    int64_t work = 0, wgs = 0;  // blocks of all row tiles, and these
+    int chunk = 1;
+    Work(const gh_kv8* kv, const Entry* e, int n, int tile) {
+        for (int i = 0; i < n; ++i) {
+            most = std::max(most, e[i].blocks);
+            tiles = std::max(tiles, e[i].x);
+            wgs += (int64_t)e[i].x * kv->nkv;
+            work += (int64_t)e[i].x * kv->nkv * e[i].blocks;
+        }
+        chunk = kv8_chunk(kv->hd, tile, most, work, wgs);
+    }
+    int parts(int blocks) const { return std::max(1, (blocks + chunk - 1) / chunk); }
+};
+
 // One launch (and one that joins the chunks) for entries with query tokens.
 int attention_launch(gh_kv8* kv, Entry* e, int n, int tile, Att8 a) {
-    a.tile = tile;
-    int most = 0;               // blocks of the longest row tile
-    int64_t work = 0, wgs = 0;  // blocks of all row tiles, and these
+    Work w(kv, e, n, tile);
     for (int i = 0; i < n; ++i) {
-        e[i].blocks = keys_of(e[i], a, tile);
-        most = std::max(most, e[i].blocks);
-        const int t = tiles_of(e[i], a, tile);
-        a.tiles = std::max(a.tiles, t);
         a.most_q = std::max(a.most_q, e[i].cnt);
         a.rows += (size_t)e[i].cnt * a.heads;
-        wgs += (int64_t)t * kv->nkv;
-        work += (int64_t)t * kv->nkv * e[i].blocks;
     }
-    a.chunk = kv8_chunk(kv->hd, tile, most, work, wgs);
-    if ((int64_t)a.most_q * a.heads * (kv->hd / 32) > MAX_GRID) a.chunk = std::max(most, 1);  // nothing to join
-    a.ns = std::max(1, (most + a.chunk - 1) / a.chunk);
-    if ((int64_t)a.ns * a.tiles * kv->nkv > MAX_GRID)
-        return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query rows in one call", a.most_q * a.group);
+    // nothing to join where a grid would be too large for it
+    if ((int64_t)a.most_q * a.heads * (kv->hd / 32) > MAX_GRID || (int64_t)w.parts(w.most) * w.tiles * kv->nkv > MAX_GRID)
+        w.chunk = std::max(w.most, 1);
+    a.tile = tile;
+    a.tiles = w.tiles;
+    a.chunk = w.chunk;
+    a.ns = w.parts(w.most);
     if (a.ns > 1) {
         void* part = nullptr;
         GH_CHECK(ctx_scratch(kv->ctx, a.rows * a.ns * (kv->hd + 2) * sizeof(float), &part));
@@ -187,6 +197,16 @@ int attention_launch(gh_kv8* kv, Entry* e, int n, int tile, Att8 a) {
     return launch_kv8_attention(dev(kv), kv->hd, b, n, a, kv->ctx->stream);
 }
 
+int attention_launches(gh_kv8* kv, Entry* e, int n, int tile, const Att8& a) {
+    for (int i = 0; i < n; ++i) {
+        e[i].x = tiles_of(e[i], a, tile);
+        e[i].blocks = keys_of(e[i], a, tile);
+    }
+    const Work w(kv, e, n, tile);
+    for (int i = 0; i < n; ++i) e[i].y = w.parts(e[i].blocks);
+    return launch_by_size(e, n, kv->nkv, [&](Entry* x, int c) { return attention_launch(kv, x, c, tile, a); });
+}
+
 // Entries of up to four query rows a kv head (decoding) have a kernel of their
 // own, but join the others where one row tile holds any of these (drafts): 64
 // sequences of 4096 tokens, half of them with drafts of 4, take 97 us joined
@@ -195,12 +215,9 @@ int attention_launch(gh_kv8* kv, Entry* e, int n, int tile, Att8 a) {
 int attention_batch(gh_kv8* kv, Entry* e, int n, const Att8& a) {
     n = (int)(std::remove_if(e, e + n, [](const Entry& x) { return x.cnt == 0; }) - e);
     Entry* wide = std::stable_partition(e, e + n, [&](const Entry& x) { return x.cnt * a.group <= 4; });
-    int most = 0;
-    for (Entry* x = e; x < e + n; ++x) most = std::max(most, x->size = tiles_of(*x, a, 16));
-    if (most == 1 && wide < e + n) wide = e;
-    if (wide > e) GH_CHECK(attention_launch(kv, e, (int)(wide - e), 4, a));
-    return launch_by_size(wide, (int)(e + n - wide), kv->nkv,
-                          [&](Entry* x, int c) { return attention_launch(kv, x, c, 16, a); });
+    if (std::all_of(wide, e + n, [&](const Entry& x) { return tiles_of(x, a, 16) == 1; }) && wide < e + n) wide = e;
+    GH_CHECK(attention_launches(kv, e, (int)(wide - e), 4, a));
+    return attention_launches(kv, wide, (int)(e + n - wide), 16, a);
 }
 
 }  // namespace
@@ -313,7 +330,7 @@ extern "C" int gh_kv8_append(gh_kv8* kv, int32_t n, const int32_t* seqs, const i
         int rows = 0;
         for (int i = 0; i < m; ++i) {
             const int s = seqs[i0 + i], t = n_tok[i0 + i];
-            e[i] = {s, kv->len[s], rows, t, blocks_of(kv->len[s], kv->len[s] + t), 0};
+            e[i] = {s, kv->len[s], rows, t, blocks_of(kv->len[s], kv->len[s] + t), 1, 0};
             rows += t;
         }
         GH_CHECK(launch_by_size(e, m, 2 * kv->nkv, [&](const Entry* x, int c) {
@@ -383,7 +400,7 @@ extern "C" int gh_kv8_read(gh_kv8* kv, int32_t n, const int32_t* seqs, const int
         int rows = 0;
         for (int i = 0; i < m; ++i) {
             const int at = begins[i0 + i], end = ends[i0 + i];
-            e[i] = {seqs[i0 + i], at, rows, end - at, blocks_of(at, end), 0};
+            e[i] = {seqs[i0 + i], at, rows, end - at, blocks_of(at, end), 1, 0};
             rows += end - at;
         }
         GH_CHECK(launch_by_size(e, m, 2 * kv->nkv, [&](const Entry* x, int c) {
@@ -411,7 +428,7 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
     int64_t total = 0;
     for (int i = 0; i < n; ++i) {
         if (n_q[i] < 0) return set_error(GH_ERR_INVALID, "gh_kv8_attention: %d query tokens", n_q[i]);
-        if ((int64_t)n_q[i] * group > MAX_ROWS)
+        if ((int64_t)n_q[i] * group > MAX_ROWS || (int64_t)n_q[i] * n_heads > MAX_QUERIES)
             return set_error(GH_ERR_RANGE, "gh_kv8_attention: %d query tokens of %d heads a kv head", n_q[i], group);
         total += n_q[i];
     }
@@ -431,7 +448,7 @@ extern "C" int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, cons
         int tokens = 0;
         for (int i = 0; i < m; ++i) {
             const int s = seqs[i0 + i], t = n_q[i0 + i];
-            e[i] = {s, kv->len[s], tokens, t, 0, 0};
+            e[i] = {s, kv->len[s], tokens, t, 0, 0, 0};
             tokens += t;
         }
         GH_CHECK(attention_batch(kv, e, m, a));

@@ -56,7 +56,9 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
 
 // A block as one workgroup takes it, 16 values a thread.  K: 4 dims of rows
 // row, row + 16, ..., whole rows a load instruction; V: 16 rows of one dim,
-// whose codes are 16 consecutive bytes (the layout in kv8.h).
+// whose codes are 16 consecutive bytes (the layout in kv8.h).  The f32 rows
+// pass by the caches, which have no use for them: prompts of 16 sequences
+// appended and read back in 125 us, 146 without.
 template <int HD, bool V>
 struct Item {
     static constexpr int N = 4 * HD;  // the workgroup's threads
@@ -216,7 +218,10 @@ __device__ __forceinline__ void append_block(int8_t* block, float* scale, float*
 }
 
 // One workgroup per block that the new tokens touch, kv head and K or V.
-// Reads 4 bytes an element and writes 1: bound by memory.
+// Reads 4 bytes an element and writes 1: bound by memory.  Prompts of up to
+// 1920 tokens for 16 sequences, 4 kv heads of 256 dims: 54 us, 5.1 TB/s of
+// both (a large copy reaches 5.1).  One token is the latency of its loads and
+// barriers, 3.3 us.
 template <int HD>
 __global__ __launch_bounds__(4 * HD, 8) void k_kv8_append(Kv8Dev c, Kv8Batch b, const float* k, const float* v) {
     __shared__ uint32_t slot[16];
@@ -266,6 +271,8 @@ __device__ __forceinline__ void truncate_block(int8_t* block, float* scale, floa
     }
 }
 
+// One workgroup per kv head and K or V: latency, 3.9 us for one sequence, 6.6
+// for 31 of 4 kv heads.
 template <int HD>
 __global__ __launch_bounds__(4 * HD, 8) void k_kv8_truncate(Kv8Dev c, Kv8Batch b) {
     __shared__ uint32_t slot[16];
@@ -280,6 +287,7 @@ __global__ __launch_bounds__(4 * HD, 8) void k_kv8_truncate(Kv8Dev c, Kv8Batch b
                                   slot);
 }
 
+// As k_kv8_append, 1 byte read and 4 written: 41 us for its prompts, 6.6 TB/s.
 template <int HD>
 __global__ __launch_bounds__(4 * HD, 8) void k_kv8_read(Kv8Dev c, Kv8Batch b, float* k, float* v) {
     const int i = blockIdx.z, h = blockIdx.y >> 1;
@@ -505,17 +513,26 @@ struct Narrow {
 //                 16 probabilities (the layout of V has their order)
 // The codes of the next block are on their way while the present one is
 // worked on, as far as the registers reach.
+// Bound by memory where there are enough sequences: 64 of up to 4096 tokens, 4
+// kv heads of 256 dims 91 us, 6.1 TB/s (a plain read reaches 6.8 to 7.2);
+// their codes pass by the caches (117 us a call without, 107 so).  Else by the
+// chain from a load to the output: 7 us for 512 tokens of one kv head, 13 for
+// 32768 in 128 chunks, and 4 to join these.
 template <int HD>
 __global__ __launch_bounds__(64 * Narrow::WAVES, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
     constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Narrow::ROWS, WAVES = Narrow::WAVES;
-    constexpr bool LATE_K = HD >= 128;
+    constexpr bool LATE_K = HD == 256;  // K and V early do not fit its registers
     __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
     __shared__ uint32_t qmax[ROWS];
     __shared__ i32x4 qs[1][KD][64];
     __shared__ __align__(16) float ob[WAVES][ROWS][HD + 4];
-    // grid: chunks, kv heads, entries
+    // grid: chunks, kv heads, entries.  Neighbours in the grid go to different
+    // XCDs; each entry and head begins with another chunk, so that those of
+    // one chunk do not all meet on one (31 sequences of 1000 tokens beside one
+    // of 32768, 8 kv heads: 142 us, turned 51).
     const int i = blockIdx.z, h = blockIdx.y;
-    const Tile<ROWS> tile(b, a, i, h, blockIdx.x, 0);
+    const unsigned turned = blockIdx.x + (blockIdx.y + blockIdx.z) % (unsigned)a.ns;
+    const Tile<ROWS> tile(b, a, i, h, turned < (unsigned)a.ns ? turned : turned - a.ns, 0);
     const int rows = tile.rows, blk1 = tile.blk1;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4;
     const Narrow col(lane & 15);
@@ -675,14 +692,14 @@ struct Wide {
 // more than a quarter of the output, and nothing is joined at the end.
 // The probabilities are relative to the step's largest, and carry the block's
 // share of the largest scale of V.
-// Bound by the conversions around the products and by the latency of one
-// phase behind the other, two workgroups a CU (256 dims; three and four for
-// 128 and 64): the matrix cores are busy for a third of the time, L2 gives 12
-// of the 33 TB/s that it could.  8192 tokens of 4 heads of 256 dims over one
-// kv head 334 us (430 TFLOP/s of the formula's), 4096 of 32 of 128 over 8: 370.
-// Four waves with blocks and outputs of their own, joined at the end: 325 and
-// 426; a prompt of 1907 tokens in a window of 1024 53 us (here 50), drafts for
-// 16 sequences of 2011 32 us (here 30).
+// Bound by the conversions around the products and by one phase waiting for
+// the other, two workgroups a CU (256 dims; three and four for 128 and 64):
+// the matrix cores are busy for a third of the time, L2 gives 12 TB/s of the
+// 33 that it could.  A prompt of 1907 tokens in a window of 1024, 8 heads of
+// 256 dims over 4: 42 us, 4096 tokens of 32 heads of 128 over 8: 310 (445
+// TFLOP/s of the formula's products; a large bf16 product reaches 1234).  By
+// four waves with blocks and outputs of their own, joined at the end: 45 and
+// 360, and drafts for 16 sequences of 2011 tokens 14 us (here 12.5).
 // ONCE: one tile a kv head, each code is read once a call.
 template <int HD, bool ONCE>
 __global__ __launch_bounds__(64 * Wide::WAVES, HD == 256 ? 2 : HD == 128 ? 3 : 4) void k_kv8_attention_wide(Kv8Dev c, Kv8Batch b, Att8 a) {
@@ -691,12 +708,14 @@ __global__ __launch_bounds__(64 * Wide::WAVES, HD == 256 ? 2 : HD == 128 ? 3 : 4
     __shared__ float st_m[WAVES][ROWS], st_l[WAVES][ROWS];
     __shared__ uint32_t qmax[ROWS];
     __shared__ i32x4 qs[3][KD][64], ps[WAVES][3][64];
-    // grid: kv heads, then the chunks, then the tiles, the longest (last) first; entries
+    // grid: kv heads, then the chunks (turned as above), then the tiles, the longest (last) first; entries
     const int i = blockIdx.z;
     const unsigned by_head = blockIdx.x / (unsigned)c.nkv, by_chunk = a.ns > 1 ? by_head / (unsigned)a.ns : by_head;
     const int h = blockIdx.x - by_head * c.nkv, t0 = a.tiles - 1 - by_chunk;
     if (t0 * ROWS >= b.cnt[i] * a.group) return;
-    const Tile<ROWS> tile(b, a, i, h, by_head - by_chunk * a.ns, t0);
+    unsigned chunk = by_head - by_chunk * a.ns;
+    if (a.ns > 1) chunk = (chunk + blockIdx.z) % (unsigned)a.ns;
+    const Tile<ROWS> tile(b, a, i, h, chunk, t0);
     const int blk1 = tile.blk1;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, row = lane & 15;
     if (tile.blk0 >= blk1) return tile.put_nothing<HD>(tid, 64 * WAVES);
@@ -943,7 +962,8 @@ int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, cons
         if (a.tile == 4) hipLaunchKernelGGL((k_kv8_attention<h.value>), dim3(a.ns, c.nkv, n), dim3(64 * Narrow::WAVES), 0, s, c, b, a);
         else if (a.tiles == 1) hipLaunchKernelGGL((k_kv8_attention_wide<h.value, true>), dim3(a.ns * c.nkv, 1, n), dim3(64 * Wide::WAVES), 0, s, c, b, a);
         else hipLaunchKernelGGL((k_kv8_attention_wide<h.value, false>), dim3(a.ns * a.tiles * c.nkv, 1, n), dim3(64 * Wide::WAVES), 0, s, c, b, a);
-        // few chunks: a row a workgroup (of 64 rows or more, so that they fill the device)
+        // few chunks: a row a workgroup (of 64 rows or more, so that they fill
+        // the device): drafts of 16 sequences 31 us so, 32 by 32 dims
         constexpr int LN = h.value / 4;
         const unsigned rows = (unsigned)a.most_q * a.heads;
         if (a.ns > 1 && (a.ns > 4 * (NT / LN) || a.rows < 64)) hipLaunchKernelGGL((k_kv8_combine<h.value, 8>), dim3(rows * (h.value / 32), n), dim3(NT), 0, s, b, a);

@@ -196,7 +196,8 @@ typedef struct gh_sampling {
  * ones).  tokens_out[n_rows] is device memory; a row with a NaN, or with
  * nothing above -inf, gets -1.  Launch-only.  GH_ERR_RANGE for a rule outside
  * its range (temperature not finite or negative, top_k < 0, top_p or min_p
- * outside [0, 1], u outside [0, 1)); GH_ERR_INVALID for vocab above 2^24. */
+ * outside [0, 1], u outside [0, 1)); GH_ERR_INVALID for vocab above 2^24 or
+ * addresses that are no multiple of 4. */
 int gh_sample_rows(gh_ctx* ctx, const float* logits, int32_t n_rows, int32_t vocab, const gh_sampling* rules,
                    int32_t* tokens_out);
 
@@ -251,8 +252,10 @@ int gh_kv8_read(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* begin
  * gh_attention_decode.  q, out [sum n_q][n_heads][head_dim] f32, not
  * overlapping.  A decode step of a batch has n_q 1, a draft a few, a prompt
  * all its tokens.  Launch-only (a captured call keeps the lengths that the
- * cache had then).  GH_ERR_RANGE where n_heads / n_kv_heads * n_q passes
- * 2^20 for a sequence. */
+ * cache had then).  Sequences of very different lengths and n_q may share a
+ * call, and a sequence may come twice.  GH_ERR_RANGE where n_heads /
+ * n_kv_heads passes 1024, or times n_q 2^20 for a sequence, or n_heads * n_q
+ * 2^27. */
 int gh_kv8_attention(gh_kv8* kv, int32_t n, const int32_t* seqs, const int32_t* n_q, const float* q, int32_t n_heads,
                      int32_t window, float* out);
 

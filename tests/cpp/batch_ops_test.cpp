@@ -94,7 +94,7 @@ int launch_kv8_attention(const Kv8Dev& c, int hd, const Kv8Batch& b, int n, cons
         most_q = std::max(most_q, b.cnt[i]);
     }
     WANT((size_t)part * a.heads == a.rows && most_q == a.most_q);
-    WANT((int64_t)a.ns * a.tiles * c.nkv <= 1 << 23);
+    WANT((int64_t)a.ns * a.tiles * c.nkv < 1 << 24);
     if (a.tile == 4) WANT(a.tiles == 1);
     if (a.ns > 1) {  // the scratch holds every state
         WANT(a.part != nullptr);

@@ -346,6 +346,18 @@ def test_a_prompt_and_drafts_among_single_tokens(ctx):
         _check(c.attention(order, new[order], q, nq, window), *stored, q, new[order], window, order)
 
 
+@pytest.mark.parametrize("t", [1, 3])
+def test_a_long_sequence_among_short_ones(ctx, t):
+    rng = np.random.default_rng(32 + t)
+    lens = rng.integers(0, 100, 180)
+    lens[77], lens[5] = 20000, 3000
+    c = gh.KVCache8(ctx, 180, 20000, 2, 32)
+    ks, vs = _fill(c, rng, lens)
+    q = rows(rng, 180 * t, 4, 32)
+    for window in (0, 4000):
+        _check(c.attention(np.arange(180), [t] * 180, q, 4, window), ks, vs, q, [t] * 180, window)
+
+
 def test_tokens_that_were_truncated_away_are_not_seen(ctx):
     """Stale codes behind a sequence's end, and a block whose scale is NaN
     behind it, take no part."""
