@@ -244,9 +244,13 @@ class _OnDevice:
         return b.ptr
 
 
+_INT32 = np.dtype(np.int32)
+
+
 def _ints(*arrays):
-    """The arrays as contiguous int32 vectors of one length."""
-    out = [np.ascontiguousarray(a, dtype=np.int32) for a in arrays]
+    """The arrays as int32 vectors of one length.  Calls take their bytes
+    (tobytes: a fifth of what ctypes asks for an array's address)."""
+    out = [np.asarray(a, _INT32) for a in arrays]
     n = out[0].size
     for a in out:
         if a.ndim != 1 or a.size != n:
@@ -337,12 +341,12 @@ def sample_rows(ctx: Context, logits, vocab: int, rules: np.ndarray, out=None):
         raise ValueError("rules must be a one-dimensional array of gemma_hip.SAMPLING")
     n = rules.size
     if type(logits) is int and type(out) is int:
-        check(lib().gh_sample_rows(ctx.h, logits, n, vocab, rules.ctypes.data, out))
+        check(lib().gh_sample_rows(ctx.h, logits, n, vocab, rules.tobytes(), out))
         return out
     with _OnDevice(ctx) as dev:
         lp = dev(logits, n * vocab)
         tb = dev.new(4 * n) if out is None else None
-        check(lib().gh_sample_rows(ctx.h, lp, n, vocab, rules.ctypes.data, tb.ptr if tb else dev(out, n)))
+        check(lib().gh_sample_rows(ctx.h, lp, n, vocab, rules.tobytes(), tb.ptr if tb else dev(out, n)))
         return tb.numpy(np.int32, n) if tb else out
 
 
@@ -609,16 +613,16 @@ class KVCache8:
         """Append n_tok[i] tokens to sequence seqs[i]; k, v [sum n_tok, n_kv_heads, head_dim]."""
         seqs, n_tok = _ints(seqs, n_tok)
         if type(k) is int and type(v) is int:
-            check(lib().gh_kv8_append(self.h, seqs.size, seqs.ctypes.data, n_tok.ctypes.data, k, v))
+            check(lib().gh_kv8_append(self.h, seqs.size, seqs.tobytes(), n_tok.tobytes(), k, v))
             return
         count = self._count(n_tok, self.n_kv_heads)
         with _OnDevice(self.ctx) as dev:
-            check(lib().gh_kv8_append(self.h, seqs.size, seqs.ctypes.data, n_tok.ctypes.data, dev(k, count), dev(v, count)))
+            check(lib().gh_kv8_append(self.h, seqs.size, seqs.tobytes(), n_tok.tobytes(), dev(k, count), dev(v, count)))
 
     def truncate(self, seqs, lens) -> None:
         """Rewind sequence seqs[i] to its first lens[i] tokens."""
         seqs, lens = _ints(seqs, lens)
-        check(lib().gh_kv8_truncate(self.h, seqs.size, seqs.ctypes.data, lens.ctypes.data))
+        check(lib().gh_kv8_truncate(self.h, seqs.size, seqs.tobytes(), lens.tobytes()))
 
     def read(self, seqs, begins, ends, k_out=None, v_out=None):
         """The f32 values of tokens [begins[i], ends[i]) of sequence seqs[i]:
@@ -627,7 +631,7 @@ class KVCache8:
         seqs, begins, ends = _ints(seqs, begins, ends)
 
         def call(kp, vp):
-            check(lib().gh_kv8_read(self.h, seqs.size, seqs.ctypes.data, begins.ctypes.data, ends.ctypes.data, kp, vp))
+            check(lib().gh_kv8_read(self.h, seqs.size, seqs.tobytes(), begins.tobytes(), ends.tobytes(), kp, vp))
 
         if type(k_out) is int and type(v_out) is int:
             call(k_out, v_out)
@@ -650,7 +654,7 @@ class KVCache8:
         seqs, n_q = _ints(seqs, n_q)
 
         def call(qp, op):
-            check(lib().gh_kv8_attention(self.h, seqs.size, seqs.ctypes.data, n_q.ctypes.data, qp, n_heads, window, op))
+            check(lib().gh_kv8_attention(self.h, seqs.size, seqs.tobytes(), n_q.tobytes(), qp, n_heads, window, op))
 
         if type(q) is int and type(out) is int:
             call(q, out)
