@@ -1151,8 +1151,10 @@ int launch_sample_rows(const float* logits, int n_rows, int vocab, const SmpRule
         int group = 1;
         while (chunks * CT / group >= SMP_GROUPS) group *= 2;
         hipLaunchKernelGGL(k_smp_stat, grid, dim3(CT), 0, s, logits, vocab, bits, group, rules, scratch);
-        hipLaunchKernelGGL(k_smp_hist, grid, dim3(CT), 0, s, logits, vocab, bits, chunks * CT / group, rules, scratch);
-        hipLaunchKernelGGL(k_smp_gather, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
+        // rows are in the order of their work: where the first takes the largest logit, all do
+        const bool greedy = rules.r[0].temperature == 0.0f;
+        if (!greedy) hipLaunchKernelGGL(k_smp_hist, grid, dim3(CT), 0, s, logits, vocab, bits, chunks * CT / group, rules, scratch);
+        if (!greedy) hipLaunchKernelGGL(k_smp_gather, grid, dim3(CT), 0, s, logits, vocab, bits, rules, scratch);
         hipLaunchKernelGGL(k_smp_pick, dim3(n_rows), dim3(PT), 0, s, logits, vocab, bits, rules, (const SmpRow*)scratch, chunks,
                            tokens);
     }

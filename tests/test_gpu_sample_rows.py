@@ -103,6 +103,21 @@ def test_all_logits_equal(ctx, vocab):
     assert got[0] == int(0.70703125 * vocab) and got[1] == int(0.70703125 * k)
 
 
+@pytest.mark.parametrize("rows", [1, 7, 130])
+def test_greedy_rows(ctx, rows):
+    """All rows at temperature 0, and all but one; ties go to the lowest index."""
+    rng = np.random.default_rng(11)
+    l = logits(rng, rows, 40007, ties=True)
+    l[0, 5] = np.nan
+    if rows > 2:
+        l[1], l[2, 30000:] = -np.inf, l[2].max() + 1
+    r = gh.sampling(rows, 0.0, rng.integers(0, 50, rows), 0.5, 0.1, 0.25)
+    got = check(ctx, l, r)
+    assert got[0] == -1 and (rows < 3 or (got[1] == -1 and got[2] == 30000))
+    r["temperature"][rows - 1] = 0.8
+    check(ctx, l, r)
+
+
 def test_borders_that_are_exact(ctx):
     """Powers of two as weights (T = 1 / ln 2 would round; equal logits do
     not): a mass that is exactly top_p of the whole is enough, a running mass
