@@ -17,6 +17,8 @@ sum over up to 33 blocks and the scales are a further 44 e:
   max|V| (2 ds + 300 e), which `attend` computes from the case's own scores."""
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 
@@ -513,3 +515,65 @@ def test_captured_attention_and_reads_replay(ctx):
     finally:
         for b in (qb, ob, kb):
             b.free()
+
+
+def test_a_captured_call_of_several_launches_replays(ctx):
+    """Chunks that are joined, a prompt and single tokens in one captured call:
+    its launches share the context's scratch one after the other."""
+    rng = np.random.default_rng(61)
+    lens = [3000, 600, 40, 2000] + [30] * 60
+    counts = [1, 600, 7, 4] + [1] * 60
+    c = gh.KVCache8(ctx, len(lens), 3000, 2, 64)
+    ks, vs = _fill(c, rng, lens)
+    q = rows(rng, sum(counts), 4, 64)
+    seqs = np.arange(len(lens))
+    eager = c.attention(seqs, counts, q, 4)
+    _check(eager, ks, vs, q, counts, 0)
+    qb, ob = gh.DeviceBuffer.from_numpy(ctx, q), gh.DeviceBuffer(ctx, q.nbytes)
+    try:
+        for _ in range(2):
+            ob.upload(np.full(q.shape, 7, F32))
+            ctx.capture_begin()
+            c.attention(seqs, counts, qb, 4, out=ob)
+            ctx.capture_replay(3)
+            assert np.array_equal(ob.numpy().reshape(q.shape), eager)
+            assert np.array_equal(c.attention(seqs, counts, q, 4), eager)
+    finally:
+        qb.free()
+        ob.free()
+
+
+def test_threads_share_a_context(ctx):
+    """Calls of several threads, on one cache and on caches of their own, give
+    what they give alone."""
+    rng = np.random.default_rng(67)
+    lens = [2500, 90, 700]
+    c = gh.KVCache8(ctx, 3, 2500, 2, 128)
+    _fill(c, rng, lens)
+    jobs = [([0, 1], [1, 1]), ([2], [300]), ([1, 2, 0], [3, 1, 5]), ([0], [40])]
+    qs = [rows(rng, sum(n), 8, 128) for _, n in jobs]
+    logits = rng.normal(size=(4, 50000)).astype(F32)
+    rules = gh.sampling(4, 0.9, [0, 40, 0, 3], 0.9, 0.0, rng.random(4).astype(F32))
+    alone = [c.attention(s, n, q, 8) for (s, n), q in zip(jobs, qs)]
+    tokens = gh.sample_rows(ctx, logits, 50000, rules)
+    wrong = []
+
+    def work(i):
+        own = gh.KVCache8(ctx, 1, 200, 1, 32)
+        x = rows(np.random.default_rng(i), 130, 1, 32)
+        for turn in range(10):
+            if not np.array_equal(c.attention(*jobs[i], qs[i], 8), alone[i]):
+                wrong.append((i, turn, "attention"))
+            if not np.array_equal(gh.sample_rows(ctx, logits, 50000, rules), tokens):
+                wrong.append((i, turn, "tokens"))
+            own.append([0], [13], x[13 * turn:13 * turn + 13], x[13 * turn:13 * turn + 13])
+        if not same_bits(own.read([0], [0], [130])[0], quantise(x)[2]):
+            wrong.append((i, "read"))
+        own.close()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
