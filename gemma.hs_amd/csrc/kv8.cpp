@@ -59,18 +59,18 @@ int check_not_capturing(const char* fn, gh_ctx* ctx) {
 // device, which costs a second launch of 4 us to join them.  Call times in us,
 // 128 dims and 8 kv heads unless said otherwise:
 //  - tile 4, a wave a block, eight of them side by side: uncut up to 16 blocks
-//    (1024 tokens, 256 dims: 22, by eights 24), or where the uncut workgroups
+//    (1024 tokens, 256 dims: 21, by eights 23), or where the uncut workgroups
 //    fill the device in nearly whole rounds (32 sequences of 4096: 56, cut in
 //    two 60), if the longest is not far from the average; else as many chunks
-//    as fill it once, of 8 blocks at least (one sequence of 131072 tokens: 59,
-//    by eights 72, uncut 590; 64 of 4096 with one head of 256 dims: 40, by
-//    eights 43, uncut 58).
-//  - tile 16, four blocks a step: uncut up to two steps (a prompt of 300: 24,
-//    by fours 28) or from a workgroup a CU on (64 sequences of 1024, 4 tokens
-//    each: 30, in halves 37; a prompt of 1024: 31, in halves 48), but for long
-//    ones short of two a CU (16 sequences of 32768 with drafts of 5: 223 by 64
-//    blocks, 280 uncut); else as many as fill it twice (one of 32768 with a
-//    draft of 5: 36, by fours 45, uncut 243).
+//    as fill it once, of 8 blocks at least (one sequence of 131072 tokens: 58,
+//    by eights 73, uncut 589; 64 of 4096 with one head of 256 dims: 39, by
+//    eights 43, uncut 57).
+//  - tile 16, four blocks a step: uncut up to two steps (a prompt of 300: 23,
+//    by fours 27) or from a workgroup a CU on (64 sequences of 1024, 4 tokens
+//    each: 29, in halves 36; a prompt of 1024: 30, in halves 47), but for long
+//    ones short of two a CU (16 sequences of 32768 with drafts of 5: 225 by 64
+//    blocks, 285 uncut); else as many as fill it twice (one of 32768 with a
+//    draft of 5: 34, by fours 43, uncut 240).
 int kv8_chunk(int hd, int tile, int most, int64_t work, int64_t wgs) {
     const bool even = most * wgs <= 2 * work;
     auto fill = [&](int64_t n, int least) { return (int)std::max<int64_t>(least, (work + n - 1) / n); };

@@ -58,7 +58,7 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
 // row, row + 16, ..., whole rows a load instruction; V: 16 rows of one dim,
 // whose codes are 16 consecutive bytes (the layout in kv8.h).  The f32 rows
 // pass by the caches, which have no use for them: prompts of 16 sequences
-// appended and read back in 125 us, 146 without.
+// appended and read back in 120 us, 141 without.
 template <int HD, bool V>
 struct Item {
     static constexpr int N = 4 * HD;  // the workgroup's threads
@@ -513,9 +513,9 @@ struct Narrow {
 //                 16 probabilities (the layout of V has their order)
 // The codes of the next block are on their way while the present one is
 // worked on, as far as the registers reach.
-// Bound by memory where there are enough sequences: 64 of up to 4096 tokens, 4
+// Bound by memory where there are enough sequences: 64 of some 4000 tokens, 4
 // kv heads of 256 dims 91 us, 6.1 TB/s (a plain read reaches 6.8 to 7.2);
-// their codes pass by the caches (117 us a call without, 107 so).  Else by the
+// their codes pass by the caches (116 us a call without, 106 so).  Else by the
 // chain from a load to the output: 7 us for 512 tokens of one kv head, 13 for
 // 32768 in 64 chunks, and 4 to join these.
 template <int HD>

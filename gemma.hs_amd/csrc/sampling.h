@@ -27,7 +27,7 @@ inline int smp_bits(int n) {
 // Steps between a row's largest and smallest logit, elements that the exact
 // search sorts, workgroups a row and groups a row at most.  Of 2048 steps one
 // holds some 600 of 262144 normal logits, a list of 4096 leaves room for ties
-// and for three searches at once (64 rows of mixed rules 71 us; by 1024 steps
+// and for three searches at once (64 rows of mixed rules 70 us; by 1024 steps
 // 81).
 constexpr int SMP_BINS = 2048, SMP_LIST = 4096, SMP_CHUNKS = 64, SMP_GROUPS = 1024;
 
