@@ -2,6 +2,7 @@
 // the split of an attention call into workgroups.
 #include <algorithm>
 #include <memory>
+#include <new>
 
 #include "host.h"
 #include "kv8.h"
@@ -236,7 +237,8 @@ extern "C" int gh_kv8_create(gh_ctx* ctx, int32_t n_seq, int32_t max_seq, int32_
     if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
         return set_error(GH_ERR_INVALID, "gh_kv8_create: head_dim %d is not 32, 64, 128 or 256", head_dim);
     Lock lk(ctx->mu);
-    std::unique_ptr<gh_kv8> kv(new gh_kv8);
+    std::unique_ptr<gh_kv8> kv(new (std::nothrow) gh_kv8);
+    if (!kv) return set_error(GH_ERR_OOM, "gh_kv8_create: host memory");
     kv->ctx = ctx;
     kv->n_seq = n_seq;
     kv->max_seq = max_seq;
@@ -265,9 +267,13 @@ extern "C" int gh_kv8_create(gh_ctx* ctx, int32_t n_seq, int32_t max_seq, int32_
         *p.p = at;
         at += (p.bytes + 255) / 256 * 256;
     }
-    kv->len.assign(n_seq, 0);
-    kv->mark.assign(n_seq, 0);
-    ctx->kv8s.push_back(kv.get());
+    try {
+        kv->len.assign(n_seq, 0);
+        kv->mark.assign(n_seq, 0);
+        ctx->kv8s.push_back(kv.get());
+    } catch (const std::bad_alloc&) {  // no exception leaves a C entry
+        return set_error(GH_ERR_OOM, "gh_kv8_create: host memory for %d sequences", n_seq);
+    }
     *out = kv.release();
     handle_add(*out, HK_KV8);
     return GH_OK;

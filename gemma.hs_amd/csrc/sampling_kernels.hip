@@ -271,7 +271,7 @@ __device__ __forceinline__ Stat range_stat(const float* l, int i0, int i1, float
         f32x4 v[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) v[j] = r.p[min(q + j * NT, r.quads - 1)];
-        if (q == threadIdx.x) {
+        if (q == (int)threadIdx.x) {
             float m = -INFINITY;
 #pragma unroll
             for (int j = 0; j < U; ++j) m = fmaxf(m, fmaxf(fmaxf(v[j].x, v[j].y), fmaxf(v[j].z, v[j].w)));
