@@ -65,7 +65,9 @@ int check_not_capturing(const char* fn, gh_ctx* ctx) {
 //    two 60), if the longest is not far from the average; else as many chunks
 //    as fill it once, of 8 blocks at least (one sequence of 131072 tokens: 58,
 //    by eights 73, uncut 589; 64 of 4096 with one head of 256 dims: 39, by
-//    eights 43, uncut 57).
+//    eights 43, uncut 57), or of 4 while these leave CUs to fill: a CU's share
+//    of the bandwidth counts (32768 tokens of one head of 256 dims: 23, by
+//    eights 25; 131072 of it 35 and 29).
 //  - tile 16, four blocks a step: uncut up to two steps (a prompt of 300: 23,
 //    by fours 27) or from a workgroup a CU on (64 sequences of 1024, 4 tokens
 //    each: 29, in halves 36; a prompt of 1024: 30, in halves 47), but for long
@@ -77,7 +79,7 @@ int kv8_chunk(int hd, int tile, int most, int64_t work, int64_t wgs) {
     auto fill = [&](int64_t n, int least) { return (int)std::max<int64_t>(least, (work + n - 1) / n); };
     if (tile == 4) {
         const int64_t slots = hd <= 64 ? 512 : 256, rounds = (wgs + slots - 1) / slots;
-        return most <= 16 || (wgs * 10 >= 9 * rounds * slots && even) ? std::max(most, 1) : fill(slots, 8);
+        return most <= 16 || (wgs * 10 >= 9 * rounds * slots && even) ? std::max(most, 1) : fill(slots, work <= 1024 ? 4 : 8);
     }
     if (most <= 8 || (even && wgs >= (most <= 64 ? 256 : 512))) return std::max(most, 1);
     return wgs < 256 ? fill(512, 4) : fill(2048, 64);

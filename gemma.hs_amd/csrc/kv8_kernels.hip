@@ -517,7 +517,7 @@ struct Narrow {
 // kv heads of 256 dims 91 us, 6.1 TB/s (a plain read reaches 6.8 to 7.2);
 // their codes pass by the caches (116 us a call without, 106 so).  Else by the
 // chain from a load to the output: 7 us for 512 tokens of one kv head, 13 for
-// 32768 in 64 chunks, and 4 to join these.
+// 32768 of four in 64 chunks each, and 4 to join these.
 template <int HD>
 __global__ __launch_bounds__(64 * Narrow::WAVES, 2) void k_kv8_attention(Kv8Dev c, Kv8Batch b, Att8 a) {
     constexpr int KR = kv8_k_row(HD), KD = KR / 64, VD = HD / 16, ROWS = Narrow::ROWS, WAVES = Narrow::WAVES;
