@@ -691,7 +691,7 @@ struct Wide {
 // LDS.  So the integer sums of four blocks become floats once, no wave holds
 // more than a quarter of the output, and nothing is joined at the end.
 // The probabilities are relative to the step's largest, and carry the block's
-// share of the largest scale of V.
+// share of the largest scale of V that the row sees.
 // Bound by the conversions around the products and by one phase waiting for
 // the other, two workgroups a CU (256 dims; three and four for 128 and 64):
 // the matrix cores are busy for a third of the time, L2 gives 12 TB/s of the
@@ -753,14 +753,10 @@ __global__ __launch_bounds__(64 * Wide::WAVES, HD == 256 ? 2 : HD == 128 ? 3 : 4
     for (int base = tile.blk0; base < blk1; base += WAVES) {
         const int blk = base + wave, blocks = min(blk1 - base, WAVES);
         if (has_dims) load_v(base);
-        // the blocks' scales of V relative to the largest; one that is NaN is left out, and spoils the rows' sums instead
         const float ks = scalar_load(c.ks + head + min(blk, blk1 - 1));
-        float vs[WAVES], top_vs = 0.0f;
+        float vs[WAVES];
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            vs[w] = scalar_load(c.vs + head + min(base + w, blk1 - 1));
-            top_vs = fmaxf(top_vs, vs[w]);
-        }
+        for (int w = 0; w < WAVES; ++w) vs[w] = scalar_load(c.vs + head + min(base + w, blk1 - 1));
         float s[16], mb = -INFINITY, f = 0.0f;
         if (blk < blk1) {
             f = qscale * ks;
@@ -803,7 +799,16 @@ __global__ __launch_bounds__(64 * Wide::WAVES, HD == 256 ? 2 : HD == 128 ? 3 : 4
         }
         if (g == 0) st_m[wave][row] = mb;
         __syncthreads();
-        const float ms = fmaxf(fmaxf(st_m[0][row], st_m[1][row]), fmaxf(st_m[2][row], st_m[3][row]));
+        // The row's maximum, and its largest scale of V: of the blocks that it
+        // sees, whose values alone set what may be lost.  A scale that is NaN
+        // is left out, and spoils the sums of the rows that see it instead.
+        float ms = -INFINITY, top_vs = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float m = st_m[w][row];
+            ms = fmaxf(ms, m);
+            top_vs = fmaxf(top_vs, m != -INFINITY ? vs[w] : 0.0f);
+        }
         // A row that sees nothing of the step has -inf for all its scores; one
         // whose scores are all NaN has the same maximum, and its sum becomes NaN.
         const float top = ms == -INFINITY ? 0.0f : ms;
@@ -813,7 +818,7 @@ __global__ __launch_bounds__(64 * Wide::WAVES, HD == 256 ? 2 : HD == 128 ? 3 : 4
         m_run = m_new;
         if (blk < blk1) {
             const float mine = wave == 0 ? vs[0] : wave == 1 ? vs[1] : wave == 2 ? vs[2] : vs[3];
-            const float share = mine == mine ? mine / top_vs * DIGIT_MAX : 0.0f;
+            const float share = mine == mine ? fminf(mine / fmaxf(top_vs, 0x1p-100f), 1.0f) * DIGIT_MAX : 0.0f;
             float lb = 0.0f;
             uint32_t pd[16];
 #pragma unroll

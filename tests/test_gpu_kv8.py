@@ -49,8 +49,9 @@ def quantise(x):
     return codes, scales, vals
 
 
-def attend(q, k, v, n_q, window):
-    """(out, bound) in 64 bits; q [n_q, nq, hd], k, v [L, nkv, hd] as stored."""
+def attend(q, k, v, n_q, window, top=None):
+    """(out, bound) in 64 bits; q [n_q, nq, hd], k, v [L, nkv, hd] as stored.
+    top [L, nkv]: what stands for a token's largest |v| in the bound."""
     L, nkv, hd = k.shape
     nq = q.shape[1]
     out = np.zeros((n_q, nq, hd))
@@ -68,7 +69,8 @@ def attend(q, k, v, n_q, window):
             out[t, h] = p @ vv / p.sum()
             eps = 2.0 ** -24
             ds = eps * ((np.abs(kk).sum(1).max() + 4 * np.abs(kk).max()) * np.abs(q64[t, h]).max() / np.sqrt(hd) + 4 * np.abs(s).max())
-            bound[t, h] = np.abs(vv).max() * (2 * ds + 300 * eps)
+            largest = np.abs(vv).max() if top is None else top[lo:pos + 1, h // (nq // nkv)].max()
+            bound[t, h] = largest * (2 * ds + 300 * eps)
     return out, bound
 
 
@@ -297,6 +299,29 @@ def test_attention_of_several_tokens_is_causal(ctx, nq, nkv, hd, n, t):
     q = rows(rng, t, nq, hd, 1.5)
     for window in (0, 40, 65):
         _check(c.attention([0], [t], q, nq, window), ks, vs, q, [t], window)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 1, 256), (16, 2, 128), (4, 1, 32)])
+@pytest.mark.parametrize("up", [True, False])
+def test_values_that_a_row_does_not_see_cost_it_no_precision(ctx, nq, nkv, hd, up):
+    """V a thousand times as large, or as small, every 64 tokens (from the
+    start, or from the end and so inside a block).  A probability is rounded to
+    2^-24 of the largest, in units of the largest scale among the blocks that
+    the row sees; times a code of at most 127 that is 2^-24 of the largest
+    value of a block that it sees, be that one itself in sight or not: the
+    bound goes by it, and by no block that the row does not see."""
+    rng = np.random.default_rng(hd + up)
+    n, t = 300, 300
+    size = 1e3 ** (np.arange(n) // B - 2.0)
+    k, v = rows(rng, n, nkv, hd), (rows(rng, n, nkv, hd) * (size if up else size[::-1])[:, None, None]).astype(F32)
+    c = gh.KVCache8(ctx, 1, n, nkv, hd)
+    c.append([0], [n], k, v)
+    q = rows(rng, t, nq, hd)
+    top = np.concatenate([np.broadcast_to(np.abs(v[b:b + B]).max((0, 2)), (len(v[b:b + B]), nkv)) for b in range(0, n, B)])
+    for window in (0, 30):
+        want, bound = attend(q, quantise(k)[2], quantise(v)[2], t, window, top)
+        err = np.abs(c.attention([0], [t], q, nq, window) - want)
+        assert np.all(err <= bound), float((err / bound).max())
 
 
 def test_attention_of_a_ragged_batch_in_any_order_the_same_sequence_twice(ctx):
